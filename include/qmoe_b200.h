@@ -451,6 +451,132 @@ QMOE_API int qmoe_layer_forward_ep_return(qmoe_layer *layer, qmoe_ep_peer *p, co
  * (-1: none) + extra[t] (nullable), T <= capacity, device pointers. */
 QMOE_API int qmoe_ep_finish(qmoe_ep_peer *p, const int32_t *slot_pos, int64_t T, const void *extra, void *out);
 
+/* ---- attention half of a decoder layer in 8 bits --------------------------
+ *
+ * The operators in front of qmoe_layer_forward_block: quantised projections,
+ * the paged cache of keys and values, and attention over it.  qmoe-rs keeps
+ * f32 matrices and a cache grown by concatenation for these
+ * (src/model.rs:86-308).  All data pointers of this section are device
+ * pointers unless said otherwise, the calls are asynchronous on the context's
+ * stream, allocate nothing and read nothing back, so they can be captured
+ * into a CUDA graph; a call's workspace is the caller's and may be reused by
+ * the next call of the same stream.
+ *
+ * A value in 8 bits: with r the largest magnitude of a row (or of a block of
+ * tokens and head), at least 127 * 2^-64, a code is 127 x / r rounded to the
+ * nearest whole number (ties to even) and stands for code * r / 127.  Where
+ * an element is not finite, r is NaN and the codes are 0. */
+
+/* Rows of x [rows, cols] (f32 or bf16, row_stride elements apart) to codes
+ * [rows, cols] and scales [rows] = r / 127. */
+QMOE_API int qmoe_quantize_int8(qmoe_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols,
+                                int64_t row_stride, int8_t *codes, float *scales);
+
+/* A weight matrix in 8 bits: codes [out_features, in_features] and one f32
+ * scale per output channel, copied to memory the handle owns (rows padded to
+ * 128 bytes).  in_features <= QMOE_INT8_MAX_IN_FEATURES, so that a sum of
+ * products fits 32 bits. */
+#define QMOE_INT8_MAX_IN_FEATURES 131072
+typedef struct qmoe_int8 qmoe_int8;
+QMOE_API int qmoe_int8_create(qmoe_ctx *ctx, const int8_t *codes, const float *scales,
+                              int64_t out_features, int64_t in_features, int ptr_kind, qmoe_int8 **out);
+QMOE_API int qmoe_int8_destroy(qmoe_int8 *t);
+QMOE_API int qmoe_int8_shape(const qmoe_int8 *t, int64_t *out_features, int64_t *in_features);
+/* Workspace bytes of a forward of `batch` rows. */
+QMOE_API int qmoe_int8_workspace(const qmoe_int8 *t, int64_t batch, int64_t *bytes);
+/* y[t, n] = (sum_k cx[t, k] * codes[n, k]) * sx[t] * scales[n] (+ residual[t, n]):
+ * x [batch, in_features] (row_stride elements apart) is quantised by row as
+ * qmoe_quantize_int8 does, the sum is exact, the rest f32, rounded once to
+ * dtype.  residual and y are [batch, out_features] in dtype, contiguous;
+ * residual may be NULL or y itself.  workspace must be 128-byte aligned.  A
+ * row of x with a non-finite element gives a row of NaN. */
+QMOE_API int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t batch, int64_t row_stride,
+                               const void *residual, void *y, void *workspace, int64_t workspace_bytes);
+
+/* Block table and slot map of a step, from request lengths.  Request r has
+ * cached_lens[r] tokens in the cache, in the blocks of its row of block_table
+ * [requests, max_blocks], and gets new_lens[r] more; the rows of the token
+ * buffer are the requests' new tokens in order.  A request lacks
+ * ceil((cached + new) / block_size) - ceil(cached / block_size) blocks and
+ * takes them from free_blocks, in order.  It is denied, without taking any,
+ * when a length is negative, its tokens do not fit its row of the table or
+ * the `capacity` rows, or (lacking any) the blocks lacking up to and
+ * including it are more than n_free; requests of the former kinds do not
+ * count there.
+ *   block_table  the new blocks' entries are written, the others kept
+ *   q_start   [requests + 1]  first row of each request, then the row count
+ *   kv_lens   [requests]      cached + new, 0 for a denied request
+ *   slots     [capacity]      block * block_size + offset of each row's
+ *                             token; -1 for rows of denied requests, rows
+ *                             behind the last request, and where a table
+ *                             entry is not in 0 .. num_blocks - 1
+ *   positions [capacity]      the token's place in its request, -1 likewise
+ *   taken     [1]             blocks taken of free_blocks
+ *   scratch   [requests]
+ * The sum of new_lens must be below 2^31.  block_size: 16, 32, ... 256. */
+QMOE_API int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
+                          int32_t block_size, const int32_t *free_blocks, int64_t n_free, int64_t num_blocks,
+                          int32_t *block_table, int64_t max_blocks, int64_t capacity, int32_t *q_start,
+                          int32_t *kv_lens, int32_t *slots, int32_t *positions, int32_t *taken, int32_t *scratch);
+
+/* The cache: codes in blocks of block_size tokens and one f32 range (the r
+ * above) per block and head, in memory of the caller, 16-byte aligned:
+ *   k        [num_blocks, kv_heads, k_dim / 64, block_size, 64]
+ *   v        [num_blocks, kv_heads, block_size / 16, v_dim, 16]
+ *   k_range, v_range [num_blocks, kv_heads]
+ * (k_dim, v_dim): (64, 64), (128, 128) or (192, 128); block_size 16, 32, ...
+ * 256; num_blocks * block_size < 2^31.  Nothing needs clearing. */
+typedef struct qmoe_kv_cache {
+    int8_t *k;
+    int8_t *v;
+    float *k_range;
+    float *v_range;
+    int64_t num_blocks;
+    int32_t block_size;
+    int32_t kv_heads;
+    int32_t k_dim;
+    int32_t v_dim;
+} qmoe_kv_cache;
+
+/* Append: row t of k [T, kv_heads, k_dim] and v [T, kv_heads, v_dim] (tokens
+ * k_stride / v_stride elements apart) goes to slots[t]; rows whose slot is
+ * not in the cache (-1) are skipped and may hold anything.  The tokens of a
+ * block that one call writes are consecutive rows and slots (qmoe_kv_plan's
+ * are), and offsets before the first of them hold the block's earlier tokens:
+ * when the new tokens raise the block's range, the earlier codes c become
+ * c * r_old / r rounded likewise.  A call that writes a block from its first
+ * offset starts it anew.  A block written through two runs of one call, or
+ * by two calls at a time, holds undefined codes. */
+QMOE_API int qmoe_kv_append(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *k, const void *v, int dtype,
+                            int64_t T, int64_t k_stride, int64_t v_stride, const int32_t *slots);
+
+/* Attention: rows q_start[r] .. q_start[r + 1] - 1 of q [T, heads, k_dim]
+ * (tokens q_stride elements apart) are the last n tokens of request r, whose
+ * kv_lens[r] tokens are in the blocks of its row of block_table; the i-th
+ * attends to the tokens 0 .. kv_lens[r] - n + i:
+ *   out[row, h] = sum_j softmax_j(scale * q[row, h] . k[j, h / (heads / kv_heads)]) v[j, ...]
+ * One token a request is the decode step, more a prompt or a chunk of one.  A
+ * row that sees no token (kv_lens 0) gives zeros; rows from q_start[requests]
+ * on are left as they were; a table entry that is not a block of the cache
+ * hides its tokens.  out [T, heads, v_dim], tokens out_stride elements apart.
+ * heads is a multiple of kv_heads.  max_kv: the longest kv_lens if the caller
+ * knows it, else 0 (max_blocks * block_size is taken); only the time depends
+ * on it.  Repeated calls give the same bits. */
+QMOE_API int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int64_t T, int64_t requests, int32_t heads,
+                                      int64_t max_blocks, int64_t max_kv, int64_t *bytes);
+QMOE_API int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int dtype, int64_t T,
+                            int64_t q_stride, int32_t heads, const int32_t *q_start, const int32_t *kv_lens,
+                            int64_t requests, const int32_t *block_table, int64_t max_blocks, int64_t max_kv,
+                            float scale, void *out, int64_t out_stride, void *workspace,
+                            int64_t workspace_bytes);
+
+/* The LayerNorm of qmoe_layer_forward_block on its own (the attention half's
+ * input_layernorm, src/model.rs:372-378): out = LN(x) for x, out
+ * [T, hidden_dim] in dtype, weight and bias [hidden_dim] f32; hidden_dim a
+ * multiple of 64. */
+QMOE_API int qmoe_layer_norm(qmoe_ctx *ctx, const void *x, int dtype, int64_t T, int64_t hidden_dim,
+                             const float *weight, const float *bias, float eps, void *out);
+
 /* ---- tracing ----------------------------------------------------------- */
 
 /* Stage timing, the device-side counterpart of the Instant-based breakdown

@@ -2119,6 +2119,280 @@ int qmoe_layer_stage_times(qmoe_layer *L, float *ms, int capacity, int *count) {
     return QMOE_OK;
 }
 
+// ---------------------------------------------------------------------------
+// attention half of a decoder layer in 8 bits
+// ---------------------------------------------------------------------------
+
+struct qmoe_int8 {
+    qmoe_ctx *ctx = nullptr;
+    int64_t out_f = 0, in_f = 0, k_pad = 0;   // rows of k_pad codes, the padding 0
+    int8_t *w = nullptr;
+    float *s = nullptr;
+    CUtensorMap tm;
+};
+
+int qmoe_quantize_int8(qmoe_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                       int8_t *codes, float *scales) {
+    if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
+    QTRY(check_dtype(dtype));
+    if (rows < 0 || rows > INT32_MAX || cols <= 0 || cols > INT32_MAX || (rows > 1 && row_stride < cols))
+        return fail(QMOE_ERR_INVALID, "rows %lld, cols %lld, row_stride %lld", (long long)rows, (long long)cols,
+                    (long long)row_stride);
+    if (rows == 0) return QMOE_OK;
+    if (!x || !codes || !scales) return fail(QMOE_ERR_INVALID, "NULL argument");
+    DeviceGuard g(ctx->device);
+    Int8RowsParams p{x, dtype, rows, row_stride, (int)cols, (int)cols, codes, scales};
+    QTRY_CUDA(launch_quant_rows(p, ctx->stream));
+    return QMOE_OK;
+}
+
+int qmoe_int8_create(qmoe_ctx *ctx, const int8_t *codes, const float *scales, int64_t out_features,
+                     int64_t in_features, int ptr_kind, qmoe_int8 **out) {
+    if (!ctx || !codes || !scales || !out) return fail(QMOE_ERR_INVALID, "NULL argument");
+    *out = nullptr;
+    QTRY(check_ptr_kind(ptr_kind));
+    if (out_features <= 0 || in_features <= 0)
+        return fail(QMOE_ERR_INVALID, "shape (%lld, %lld): both dimensions must be > 0", (long long)out_features,
+                    (long long)in_features);
+    if (in_features > QMOE_INT8_MAX_IN_FEATURES || out_features > (1LL << 30))
+        return fail(QMOE_ERR_UNSUPPORTED, "shape (%lld, %lld) too large (in_features <= %d)", (long long)out_features,
+                    (long long)in_features, QMOE_INT8_MAX_IN_FEATURES);
+    DeviceGuard g(ctx->device);
+    qmoe_int8 *t = new (std::nothrow) qmoe_int8;
+    if (!t) return fail(QMOE_ERR_NOMEM, "host allocation failed");
+    t->ctx = ctx;
+    t->out_f = out_features;
+    t->in_f = in_features;
+    t->k_pad = (in_features + 127) / 128 * 128;
+    const size_t wb = (size_t)out_features * t->k_pad;
+    cudaError_t e = cudaMalloc(&t->w, wb);
+    if (e == cudaSuccess) e = cudaMalloc(&t->s, sizeof(float) * out_features);
+    if (e == cudaSuccess && t->k_pad != in_features) e = cudaMemsetAsync(t->w, 0, wb, ctx->stream);
+    if (e == cudaSuccess)
+        e = cudaMemcpy2DAsync(t->w, (size_t)t->k_pad, codes, (size_t)in_features, (size_t)in_features,
+                              (size_t)out_features, kind_in(ptr_kind), ctx->stream);
+    if (e == cudaSuccess)
+        e = cudaMemcpyAsync(t->s, scales, sizeof(float) * out_features, kind_in(ptr_kind), ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+        qmoe_int8_destroy(t);
+        return fail(e == cudaErrorMemoryAllocation ? QMOE_ERR_NOMEM : QMOE_ERR_CUDA, "8-bit upload failed: %s",
+                    cudaGetErrorString(e));
+    }
+    if (!make_tmap_u8(&t->tm, t->w, (uint64_t)t->k_pad, (uint64_t)out_features, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) {
+        qmoe_int8_destroy(t);
+        return fail(QMOE_ERR_CUDA, "tensor map encoding failed");
+    }
+    *out = t;
+    return QMOE_OK;
+}
+
+int qmoe_int8_destroy(qmoe_int8 *t) {
+    if (!t) return QMOE_OK;
+    DeviceGuard g(t->ctx->device);
+    if (t->w) cudaFree(t->w);
+    if (t->s) cudaFree(t->s);
+    delete t;
+    return QMOE_OK;
+}
+
+int qmoe_int8_shape(const qmoe_int8 *t, int64_t *out_features, int64_t *in_features) {
+    if (!t) return fail(QMOE_ERR_INVALID, "tensor is NULL");
+    if (out_features) *out_features = t->out_f;
+    if (in_features) *in_features = t->in_f;
+    return QMOE_OK;
+}
+
+// codes [batch, k_pad], then scales [batch]
+int qmoe_int8_workspace(const qmoe_int8 *t, int64_t batch, int64_t *bytes) {
+    if (!t || !bytes) return fail(QMOE_ERR_INVALID, "NULL argument");
+    if (batch < 0 || batch > (1LL << 30)) return fail(QMOE_ERR_INVALID, "batch %lld", (long long)batch);
+    *bytes = batch * (t->k_pad + (int64_t)sizeof(float));
+    return QMOE_OK;
+}
+
+int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t batch, int64_t row_stride,
+                      const void *residual, void *y, void *workspace, int64_t workspace_bytes) {
+    if (!t) return fail(QMOE_ERR_INVALID, "tensor is NULL");
+    QTRY(check_dtype(dtype));
+    int64_t need = 0;
+    QTRY(qmoe_int8_workspace(t, batch, &need));
+    if (batch == 0) return QMOE_OK;
+    if (!x || !y || !workspace) return fail(QMOE_ERR_INVALID, "NULL argument");
+    if (batch > 1 && row_stride < t->in_f)
+        return fail(QMOE_ERR_INVALID, "row_stride %lld < in_features %lld", (long long)row_stride, (long long)t->in_f);
+    if (workspace_bytes < need)
+        return fail(QMOE_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                    (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 127u)
+        return fail(QMOE_ERR_INVALID, "workspace must be 128-byte aligned");
+    DeviceGuard g(t->ctx->device);
+    cudaStream_t st = t->ctx->stream;
+    int8_t *codes = static_cast<int8_t *>(workspace);
+    float *sx = reinterpret_cast<float *>(codes + batch * t->k_pad);
+    CUtensorMap tm_x;
+    if (!make_tmap_u8(&tm_x, codes, (uint64_t)t->k_pad, (uint64_t)batch, 128, (uint32_t)int8_token_tile(batch),
+                      CU_TENSOR_MAP_SWIZZLE_128B))
+        return fail(QMOE_ERR_CUDA, "tensor map encoding failed");
+    Int8RowsParams q{x, dtype, batch, row_stride, (int)t->in_f, (int)t->k_pad, codes, sx};
+    QTRY_CUDA(launch_quant_rows(q, st));
+    Int8GemmParams p{batch, t->out_f, (int)t->in_f, dtype, sx, t->s, residual, y, error_flag()};
+    QTRY_CUDA(launch_int8_gemm(t->tm, tm_x, p, st));
+    return QMOE_OK;
+}
+
+int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
+                 int32_t block_size, const int32_t *free_blocks, int64_t n_free, int64_t num_blocks,
+                 int32_t *block_table, int64_t max_blocks, int64_t capacity, int32_t *q_start, int32_t *kv_lens,
+                 int32_t *slots, int32_t *positions, int32_t *taken, int32_t *scratch) {
+    if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
+    if (block_size < 16 || block_size > 256 || block_size % 16)
+        return fail(QMOE_ERR_INVALID, "block_size %d must be a multiple of 16, at most 256", block_size);
+    if (requests < 0 || requests > (1 << 24) || n_free < 0 || n_free > INT32_MAX || num_blocks < 0 ||
+        max_blocks < 0 || capacity < 0 || capacity > INT32_MAX)
+        return fail(QMOE_ERR_INVALID, "requests %lld, n_free %lld, num_blocks %lld, max_blocks %lld, capacity %lld",
+                    (long long)requests, (long long)n_free, (long long)num_blocks, (long long)max_blocks,
+                    (long long)capacity);
+    if (num_blocks >= (1LL << 31) / block_size || max_blocks >= (1LL << 31) / block_size)
+        return fail(QMOE_ERR_INVALID, "num_blocks and max_blocks times block_size must be below 2^31");
+    if (!q_start || !taken || (requests > 0 && (!cached_lens || !new_lens || !kv_lens || !scratch)) ||
+        (requests > 0 && max_blocks > 0 && !block_table) || (n_free > 0 && !free_blocks) ||
+        (capacity > 0 && (!slots || !positions)))
+        return fail(QMOE_ERR_INVALID, "NULL argument");
+    DeviceGuard g(ctx->device);
+    KvPlanParams p{cached_lens, new_lens, requests, block_size, free_blocks, n_free, num_blocks, block_table,
+                   max_blocks, capacity, q_start, kv_lens, slots, positions, taken, scratch};
+    QTRY_CUDA(launch_kv_plan(p, ctx->stream));
+    return QMOE_OK;
+}
+
+static int check_cache(const qmoe_kv_cache *c, KvCacheDev &d) {
+    if (!c) return fail(QMOE_ERR_INVALID, "cache is NULL");
+    if (c->block_size < 16 || c->block_size > 256 || c->block_size % 16)
+        return fail(QMOE_ERR_INVALID, "block_size %d must be a multiple of 16, at most 256", c->block_size);
+    if (c->num_blocks < 0 || c->num_blocks >= (1LL << 31) / c->block_size)
+        return fail(QMOE_ERR_INVALID, "num_blocks %lld times block_size must be below 2^31", (long long)c->num_blocks);
+    if (c->kv_heads < 1 || c->kv_heads > 4096) return fail(QMOE_ERR_INVALID, "kv_heads %d", c->kv_heads);
+    if (!((c->k_dim == 64 && c->v_dim == 64) || (c->k_dim == 128 && c->v_dim == 128) ||
+          (c->k_dim == 192 && c->v_dim == 128)))
+        return fail(QMOE_ERR_UNSUPPORTED, "head dims (%d, %d): (64, 64), (128, 128) and (192, 128) are supported",
+                    c->k_dim, c->v_dim);
+    if (c->num_blocks > 0 && (!c->k || !c->v || !c->k_range || !c->v_range))
+        return fail(QMOE_ERR_INVALID, "NULL argument");
+    QTRY(check_align(c->k, QMOE_PTR_DEVICE, "k"));
+    QTRY(check_align(c->v, QMOE_PTR_DEVICE, "v"));
+    d = KvCacheDev{c->k, c->v, c->k_range, c->v_range, c->num_blocks, c->block_size, c->kv_heads, c->k_dim, c->v_dim};
+    return QMOE_OK;
+}
+
+int qmoe_kv_append(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *k, const void *v, int dtype, int64_t T,
+                   int64_t k_stride, int64_t v_stride, const int32_t *slots) {
+    if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
+    KvAppendParams p{};
+    QTRY(check_cache(cache, p.c));
+    QTRY(check_dtype(dtype));
+    if (T < 0 || T > (1 << 30)) return fail(QMOE_ERR_INVALID, "T %lld", (long long)T);
+    if (T == 0 || p.c.num_blocks == 0) return QMOE_OK;
+    if (!k || !v || !slots) return fail(QMOE_ERR_INVALID, "NULL argument");
+    if (T > 1 && (k_stride < (int64_t)p.c.heads * p.c.k_dim || v_stride < (int64_t)p.c.heads * p.c.v_dim))
+        return fail(QMOE_ERR_INVALID, "token strides (%lld, %lld) below the rows' widths", (long long)k_stride,
+                    (long long)v_stride);
+    const uintptr_t es = dtype_size(dtype);
+    p.k = k;
+    p.v = v;
+    p.dtype = dtype;
+    p.T = T;
+    p.ldk = k_stride;
+    p.ldv = v_stride;
+    p.vec_k = reinterpret_cast<uintptr_t>(k) % (4 * es) == 0 && k_stride % 4 == 0;
+    p.vec_v = reinterpret_cast<uintptr_t>(v) % (4 * es) == 0 && v_stride % 4 == 0;
+    p.slots = slots;
+    DeviceGuard g(ctx->device);
+    QTRY_CUDA(launch_kv_append(p, ctx->stream));
+    return QMOE_OK;
+}
+
+static int check_attend(const qmoe_kv_cache *cache, KvCacheDev &c, int64_t T, int64_t requests, int32_t heads,
+                        int64_t max_blocks, int64_t &max_kv) {
+    QTRY(check_cache(cache, c));
+    if (T < 0 || T > (1 << 24) || requests < 0 || requests > (1 << 24))
+        return fail(QMOE_ERR_INVALID, "T %lld, requests %lld (at most 2^24)", (long long)T, (long long)requests);
+    if (heads < 1 || heads > 65535 || heads % c.heads)
+        return fail(QMOE_ERR_INVALID, "heads %d must be a multiple of kv_heads %d", heads, c.heads);
+    if (max_blocks < 0 || max_blocks >= (1LL << 31) / c.block)
+        return fail(QMOE_ERR_INVALID, "max_blocks %lld times block_size must be below 2^31", (long long)max_blocks);
+    if (max_kv <= 0 || max_kv > max_blocks * c.block) max_kv = max_blocks * c.block;
+    return QMOE_OK;
+}
+
+int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int64_t T, int64_t requests, int32_t heads,
+                             int64_t max_blocks, int64_t max_kv, int64_t *bytes) {
+    if (!bytes) return fail(QMOE_ERR_INVALID, "NULL argument");
+    KvCacheDev c{};
+    QTRY(check_attend(cache, c, T, requests, heads, max_blocks, max_kv));
+    *bytes = (int64_t)(sizeof(float) *
+                       attend_workspace_floats(T, heads, c.v_dim, attend_splits(T, requests, heads, c.heads, max_kv)));
+    return QMOE_OK;
+}
+
+int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int dtype, int64_t T, int64_t q_stride,
+                   int32_t heads, const int32_t *q_start, const int32_t *kv_lens, int64_t requests,
+                   const int32_t *block_table, int64_t max_blocks, int64_t max_kv, float scale, void *out,
+                   int64_t out_stride, void *workspace, int64_t workspace_bytes) {
+    if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
+    QTRY(check_dtype(dtype));
+    AttendParams p{};
+    QTRY(check_attend(cache, p.c, T, requests, heads, max_blocks, max_kv));
+    if (T == 0 || requests == 0) return QMOE_OK;
+    if (!q || !out || !q_start || !kv_lens || (max_blocks > 0 && !block_table))
+        return fail(QMOE_ERR_INVALID, "NULL argument");
+    if (T > 1 && (q_stride < (int64_t)heads * p.c.k_dim || out_stride < (int64_t)heads * p.c.v_dim))
+        return fail(QMOE_ERR_INVALID, "token strides (%lld, %lld) below the rows' widths", (long long)q_stride,
+                    (long long)out_stride);
+    if (!(scale == scale) || scale - scale != 0.0f) return fail(QMOE_ERR_INVALID, "scale must be finite");
+    DeviceGuard g(ctx->device);
+    p.splits = attend_splits(T, requests, heads, p.c.heads, max_kv);
+    const int64_t need = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, p.c.v_dim, p.splits));
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(QMOE_ERR_INVALID, "workspace of %lld bytes (16-byte aligned), %lld needed",
+                    (long long)workspace_bytes, (long long)need);
+    p.q = q;
+    p.dtype = dtype;
+    p.T = T;
+    p.ldq = q_stride;
+    p.heads = heads;
+    p.q_start = q_start;
+    p.kv_lens = kv_lens;
+    p.table = block_table;
+    p.R = requests;
+    p.max_blocks = max_blocks;
+    p.scale = scale;
+    p.out = out;
+    p.ldo = out_stride;
+    p.ws = static_cast<float *>(workspace);
+    QTRY_CUDA(launch_attend(p, ctx->stream));
+    return QMOE_OK;
+}
+
+int qmoe_layer_norm(qmoe_ctx *ctx, const void *x, int dtype, int64_t T, int64_t hidden_dim, const float *weight,
+                    const float *bias, float eps, void *out) {
+    if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
+    QTRY(check_dtype(dtype));
+    if (T < 0 || T > INT32_MAX || hidden_dim <= 0 || hidden_dim % 64 || hidden_dim > (1 << 18))
+        return fail(QMOE_ERR_INVALID, "T %lld, hidden_dim %lld (a multiple of 64)", (long long)T,
+                    (long long)hidden_dim);
+    if (T == 0) return QMOE_OK;
+    if (!x || !weight || !bias || !out) return fail(QMOE_ERR_INVALID, "NULL argument");
+    QTRY(check_align(x, QMOE_PTR_DEVICE, "x"));
+    QTRY(check_align(out, QMOE_PTR_DEVICE, "out"));
+    QTRY(check_align(weight, QMOE_PTR_DEVICE, "weight"));
+    QTRY(check_align(bias, QMOE_PTR_DEVICE, "bias"));
+    DeviceGuard g(ctx->device);
+    NormParams n{x, dtype, T, (int)hidden_dim, weight, bias, eps, out};
+    QTRY_CUDA(launch_layernorm(n, ctx->stream));
+    return QMOE_OK;
+}
+
 }  // extern "C"
 
 namespace qmoe {

@@ -1,0 +1,43 @@
+// code8.cuh -- the 8-bit code of a value on a symmetric range, shared by the
+// row quantiser (int8.cu) and the append to the 8-bit cache (kv.cu).
+//
+//   r     = max(max |x|, 127 * 2^-64), NaN when an element is not finite
+//   code  = 127 x / r rounded to the nearest whole number, ties to even
+//   value = code * (r / 127)
+//
+// The rounding is that of the real quotient, not of a rounded one: the f32
+// estimate decides unless it lies within 2^-14 of a border between two codes
+// (its error is below 2^-16: two roundings of a value of at most 127), and
+// the f64 quotient decides there.  The f64 products a * m are exact (24 + 24
+// bits), and a quotient of 24-bit numbers that is not on a border is further
+// from it than f64's rounding, so a code is the same whatever computes it.
+#pragma once
+
+#include "common.cuh"
+
+namespace qmoe {
+
+constexpr float kRangeFloor = 127.0f * 5.42101086242752217e-20f;   // a scale of 2^-64
+
+// a * m / r as a code, |a * m| <= 127 r; mi = m / r in f32.
+QMOE_DEV int code8(float a, float m, float r, float mi) {
+    const float q = __fmul_rn(a, mi);
+    const float c = rintf(q);
+    if (fabsf(fabsf(__fsub_rn(q, c)) - 0.5f) < 6.103515625e-05f)
+        return (int)rint((double)a * (double)m / (double)r);
+    return (int)c;                                                 // NaN gives 0
+}
+
+// The range of values whose largest magnitude is `m`, when `finite`.
+QMOE_DEV float range8(float m, bool finite) {
+    return finite ? fmaxf(m, kRangeFloor) : __int_as_float(0x7fc00000);
+}
+
+QMOE_DEV float max_abs(float m, float v) { return fmaxf(m, fabsf(v)); }   // NaN is looked for apart
+
+// Four codes as bytes, the first in the lowest.
+QMOE_DEV uint32_t pack4(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+}
+
+}  // namespace qmoe

@@ -349,5 +349,79 @@ cudaError_t launch_combine_rows(const void *rows, int dtype, int64_t H, const in
 
 // ---- combine -----------------------------------------------------------
 
+// ---- 8-bit integer product (int8.cu) -------------------------------------
+struct Int8RowsParams {
+    const void *x;          // [T, K] f32 or bf16, rows ldx apart
+    int dtype;
+    int64_t T, ldx;
+    int K, ldc;             // ldc: K rounded up to 128; the codes past K are 0
+    int8_t *codes;          // [T, ldc]
+    float *scales;          // [T]
+};
+struct Int8GemmParams {
+    int64_t T, N;
+    int K;
+    int dtype;              // of residual and y
+    const float *sx, *sw;   // [T], [N]
+    const void *residual;   // [T, N] or nullptr
+    void *y;                // [T, N]
+    int *err;               // device error word
+};
+cudaError_t launch_quant_rows(const Int8RowsParams &p, cudaStream_t s);
+// Rows of the activation map's box for T tokens.
+int int8_token_tile(int64_t T);
+cudaError_t launch_int8_gemm(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const Int8GemmParams &p,
+                             cudaStream_t s);
+
+// ---- 8-bit paged cache (kv.cu, attend.cu) ----------------------------------
+struct KvCacheDev {
+    int8_t *k;              // [num_blocks, heads, k_dim / 64, block, 64]
+    int8_t *v;              // [num_blocks, heads, block / 16, v_dim, 16]
+    float *k_range, *v_range;   // [num_blocks, heads]
+    int64_t num_blocks;
+    int block, heads, k_dim, v_dim;
+};
+struct KvPlanParams {
+    const int32_t *cached, *fresh;   // [R]
+    int64_t R;
+    int block;
+    const int32_t *free_blocks;      // [n_free]
+    int64_t n_free, num_blocks;
+    int32_t *table;                  // [R, max_blocks]
+    int64_t max_blocks, capacity;    // capacity: rows of slots and positions
+    int32_t *q_start, *kv_lens;      // [R + 1], [R]
+    int32_t *slots, *positions;      // [capacity]
+    int32_t *taken;                  // [1]
+    int32_t *first;                  // [R] scratch: first place in the free list
+};
+struct KvAppendParams {
+    KvCacheDev c;
+    const void *k, *v;      // [T, heads, k_dim] / [T, heads, v_dim], tokens ldk / ldv apart
+    int dtype;
+    int64_t T, ldk, ldv;
+    bool vec_k, vec_v;      // four elements may be loaded at once
+    const int32_t *slots;   // [T]
+};
+struct AttendParams {
+    KvCacheDev c;
+    const void *q;          // [T, heads, k_dim], tokens ldq apart
+    int dtype;
+    int64_t T, ldq;
+    int heads;              // query heads
+    const int32_t *q_start, *kv_lens, *table;   // [R + 1], [R], [R, max_blocks]
+    int64_t R, max_blocks;
+    float scale;
+    void *out;              // [T, heads, v_dim], tokens ldo apart
+    int64_t ldo;
+    int splits;             // pieces of the keys; > 1 joins through ws
+    float *ws;              // attend_workspace_floats floats
+};
+cudaError_t launch_kv_plan(const KvPlanParams &p, cudaStream_t s);
+cudaError_t launch_kv_append(const KvAppendParams &p, cudaStream_t s);
+// Pieces that the keys of a request are cut into, for a batch whose longest
+// request holds max_kv tokens.
+int attend_splits(int64_t T, int64_t R, int heads, int kv_heads, int64_t max_kv);
+size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits);
+cudaError_t launch_attend(const AttendParams &p, cudaStream_t s);
 
 }  // namespace qmoe

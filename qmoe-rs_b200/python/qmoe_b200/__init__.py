@@ -8,8 +8,10 @@ from .capi import QmoeError
 from .layer import (BlockChain, Context, MoEConfig, PackedExpert, PackedQMoETensor, QMoELayer,
                     default_context)
 from . import quantize
+from .attention import AttentionBlock, Int8Tensor, KVCache, PagePlan, layer_norm, plan_pages, quantize_int8
 from .ep import ExpertParallelMoE, TorchComm
 
 __all__ = ["capi", "QmoeError", "BlockChain", "Context", "MoEConfig", "PackedExpert",
            "PackedQMoETensor", "QMoELayer", "default_context", "quantize",
-           "ExpertParallelMoE", "TorchComm"]
+           "AttentionBlock", "Int8Tensor", "KVCache", "PagePlan", "layer_norm", "plan_pages",
+           "quantize_int8", "ExpertParallelMoE", "TorchComm"]

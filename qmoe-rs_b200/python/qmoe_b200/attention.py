@@ -1,0 +1,350 @@
+"""The attention half of a decoder layer in 8 bits, over the C ABI.
+
+  Int8Tensor      a weight matrix in 8 bits; forward quantises the tokens
+  plan_pages      block table and slot map of a step, from request lengths
+  KVCache         paged keys and values in 8 bits: append, attend
+  AttentionBlock  x + out(attention(qkv(LN(x)))), the half in front of
+                  QMoELayer.forward_block (qmoe-rs src/model.rs:372-413);
+                  BlockChain runs both halves of every layer
+
+Activations are CUDA torch tensors, float32 or bfloat16.  Calls are
+asynchronous on the current torch stream, and workspaces come from torch's
+allocator in each call, so any of them may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Callable, Optional, Tuple
+
+import torch
+
+from . import capi
+from .layer import Context, _dtype_code, _ptr, default_context
+
+_I64 = ctypes.c_int64
+
+
+def _on(ctx: Context, **tensors) -> None:
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        if t.device.index != ctx.device:
+            raise ValueError(f"{name} is on cuda:{t.device.index}, the context on cuda:{ctx.device}")
+
+
+def _context_of(x, ctx: Optional[Context]) -> Context:
+    if ctx is not None:
+        return ctx
+    return default_context(x.device.index if isinstance(x, torch.Tensor) and x.is_cuda else 0)
+
+
+def _i32(t, name: str, shape) -> int:
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
+
+
+def quantize_int8(x, ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes int8 [rows, cols], scales f32 [rows]) of x [rows, cols]: with r
+    the row's largest magnitude, code = round(127 x / r) and scale = r / 127."""
+    ctx = _context_of(x, ctx)
+    _on(ctx, x=x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
+    dt = _dtype_code(x)
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    ctx.use_current_torch_stream()
+    capi.call("qmoe_quantize_int8", ctx.handle, x.data_ptr(), dt, x.shape[0], x.shape[1],
+              max(x.stride(0), x.shape[1]), codes.data_ptr(), scales.data_ptr())
+    return codes, scales
+
+
+class Int8Tensor:
+    """Device-resident 8-bit weight matrix with a scale per output channel,
+    the 8-bit counterpart of PackedQMoETensor (qmoe-rs src/tensor.rs:16-121)."""
+
+    def __init__(self, handle, ctx: Context, shape, scales):
+        self._h = handle
+        self.ctx = ctx
+        self.shape = tuple(int(v) for v in shape)
+        self.scales = scales
+        n = _I64()
+        capi.call("qmoe_int8_workspace", handle, 1, ctypes.byref(n))
+        self._row_bytes = int(n.value)
+
+    @classmethod
+    def from_bytes(cls, codes, shape: Tuple[int, int], scales, ctx: Optional[Context] = None) -> "Int8Tensor":
+        """codes int8 [out, in] and scales f32 [out], both host or both device memory."""
+        ctx = _context_of(codes, ctx)
+        out_f, in_f = (int(v) for v in shape)
+        for name, a, kind, n in (("codes", codes, "int8", out_f * in_f), ("scales", scales, "float32", out_f)):
+            have = a.numel() if isinstance(a, torch.Tensor) else a.size
+            if str(a.dtype).replace("torch.", "") != kind or have != n:
+                raise ValueError(f"{name} must hold {n} {kind} values, got {have} of {a.dtype}")
+        cp, kind, keep1 = _ptr(codes)
+        sp, kind2, keep2 = _ptr(scales)
+        if kind != kind2:
+            raise ValueError("codes and scales must both be host or both device memory")
+        if kind == capi.QMOE_PTR_DEVICE:
+            _on(ctx, codes=codes, scales=scales)
+        ctx.use_current_torch_stream()
+        h = ctypes.c_void_p()
+        capi.call("qmoe_int8_create", ctx.handle, cp, sp, out_f, in_f, kind, ctypes.byref(h))
+        return cls(h, ctx, shape, scales)
+
+    @classmethod
+    def from_float(cls, weight, ctx: Optional[Context] = None) -> "Int8Tensor":
+        """A CUDA weight [out, in] in float32 or bfloat16, quantised by output channel."""
+        codes, scales = quantize_int8(weight, ctx)
+        return cls.from_bytes(codes, tuple(weight.shape), scales, ctx)
+
+    def forward(self, x, residual=None, out=None):
+        """y [..., out] = x [..., in] times the weight (+ residual), x quantised by token.
+
+        `out` may be `residual` itself."""
+        out_f, in_f = self.shape
+        _on(self.ctx, x=x)
+        dt = _dtype_code(x)
+        if x.dim() < 1 or x.shape[-1] != in_f:
+            raise ValueError(f"x {list(x.shape)} does not end in in_features = {in_f}")
+        rows = x if x.dim() == 2 else x.reshape(-1, in_f)
+        if rows.stride(1) != 1 or rows.stride(0) < in_f:
+            rows = rows.contiguous()
+        batch = rows.shape[0]
+        shape = x.shape[:-1] + (out_f,)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        for name, a in (("residual", residual), ("out", out)):
+            if a is not None:
+                _on(self.ctx, **{name: a})
+                if a.shape != shape or a.dtype != x.dtype or not a.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous {x.dtype} {list(shape)}")
+        need = batch * self._row_bytes
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        self.ctx.use_current_torch_stream()
+        capi.call("qmoe_int8_forward", self._h, rows.data_ptr(), dt, batch, rows.stride(0),
+                  residual.data_ptr() if residual is not None else None, out.data_ptr(), ws.data_ptr(), need)
+        return out
+
+    def close(self):
+        if getattr(self, "_h", None):
+            capi.lib().qmoe_int8_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+@dataclass
+class PagePlan:
+    """A step's place in the cache (qmoe_kv_plan)."""
+
+    block_table: torch.Tensor   # [requests, max_blocks] int32, updated in place
+    q_start: torch.Tensor       # [requests + 1] first row of each request
+    kv_lens: torch.Tensor       # [requests] tokens held after the step, 0 for a denied request
+    slots: torch.Tensor         # [rows] block * block_size + offset, -1 for none
+    positions: torch.Tensor     # [rows] place in the request, -1 for none
+    taken: torch.Tensor         # [1] blocks taken from the front of the free list
+    max_kv: int = 0             # longest kv_lens if known on the host
+
+
+def plan_pages(cached_lens, new_lens, block_table, free_blocks, block_size: int, num_tokens: int,
+               num_blocks: int, max_kv: int = 0, ctx: Optional[Context] = None) -> PagePlan:
+    """Block table and slot map of a step: request r holds cached_lens[r] tokens
+    in the blocks of its row of block_table [requests, max_blocks] and gets
+    new_lens[r] more, taking what blocks it lacks from free_blocks in order.
+    num_tokens: rows of the step's token buffer; num_blocks: of the cache.  All
+    tensors int32 on the GPU; the host reads nothing.  A request that does not
+    fit is denied: kv_lens 0, slots and positions -1."""
+    ctx = _context_of(cached_lens, ctx)
+    _on(ctx, cached_lens=cached_lens, new_lens=new_lens, block_table=block_table, free_blocks=free_blocks)
+    if block_table.dim() != 2 or free_blocks.dim() != 1:
+        raise ValueError("block_table must be [requests, max_blocks] and free_blocks [n]")
+    R, width = block_table.shape
+    T = int(num_tokens)
+    if T < 0:
+        raise ValueError(f"num_tokens {T} < 0")
+    args = (_i32(cached_lens, "cached_lens", (R,)), _i32(new_lens, "new_lens", (R,)),
+            _i32(free_blocks, "free_blocks", free_blocks.shape), _i32(block_table, "block_table", (R, width)))
+    buf = torch.empty(3 * R + 2 + 2 * T, dtype=torch.int32, device=block_table.device)
+    kv, scratch, q_start, taken, slots, positions = buf.split([R, R, R + 1, 1, T, T])
+    at = buf.data_ptr()
+    ctx.use_current_torch_stream()
+    capi.call("qmoe_kv_plan", ctx.handle, args[0], args[1], R, int(block_size), args[2], free_blocks.shape[0],
+              int(num_blocks), args[3], width, T, at + 8 * R, at, at + 12 * R + 8, at + 12 * R + 8 + 4 * T,
+              at + 12 * R + 4, at + 4 * R)
+    return PagePlan(block_table, q_start, kv, slots, positions, taken, int(max_kv))
+
+
+class KVCache:
+    """Keys and values in 8 bits, in blocks of block_size tokens with one range
+    per block and head (qmoe_kv_cache):
+
+      k        int8 [num_blocks, kv_heads, k_dim / 64, block_size, 64]
+      v        int8 [num_blocks, kv_heads, block_size / 16, v_dim, 16]
+      k_range, v_range  f32 [num_blocks, kv_heads]; code c stands for c * range / 127
+    """
+
+    def __init__(self, num_blocks: int, block_size: int, kv_heads: int, k_dim: int, v_dim: Optional[int] = None,
+                 ctx: Optional[Context] = None):
+        ctx = ctx or default_context()
+        v_dim = k_dim if v_dim is None else v_dim
+        if k_dim % 64 or block_size % 16:
+            raise ValueError(f"k_dim {k_dim} must be a multiple of 64 and block_size {block_size} of 16")
+        dev = torch.device("cuda", ctx.device)
+        z = lambda *s, dtype: torch.zeros(s, dtype=dtype, device=dev)  # noqa: E731
+        self._set(z(num_blocks, kv_heads, k_dim // 64, block_size, 64, dtype=torch.int8),
+                  z(num_blocks, kv_heads, block_size // 16, v_dim, 16, dtype=torch.int8),
+                  z(num_blocks, kv_heads, dtype=torch.float32), z(num_blocks, kv_heads, dtype=torch.float32), ctx)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_range, v_range, ctx: Optional[Context] = None) -> "KVCache":
+        """A cache in the caller's tensors (layouts above)."""
+        self = cls.__new__(cls)
+        self._set(k, v, k_range, v_range, _context_of(k, ctx))
+        return self
+
+    def _set(self, k, v, k_range, v_range, ctx: Context) -> None:
+        _on(ctx, k=k, v=v, k_range=k_range, v_range=v_range)
+        if k.dim() != 5 or v.dim() != 5:
+            raise ValueError("k and v must have 5 dimensions")
+        nb, heads, chunks, bs, w = k.shape
+        want = (nb, heads, bs // 16, v.shape[3], 16)
+        if w != 64 or tuple(v.shape) != want or tuple(k_range.shape) != (nb, heads) or k_range.shape != v_range.shape:
+            raise ValueError(f"shapes k {list(k.shape)}, v {list(v.shape)}, ranges {list(k_range.shape)}, "
+                             f"{list(v_range.shape)} do not make a cache")
+        if k.dtype != torch.int8 or v.dtype != torch.int8 or k_range.dtype != torch.float32 or v_range.dtype != torch.float32:
+            raise TypeError("codes must be int8 and ranges float32")
+        if not all(t.is_contiguous() for t in (k, v, k_range, v_range)):
+            raise ValueError("a cache's tensors must be contiguous")
+        self.ctx, self.k, self.v, self.k_range, self.v_range = ctx, k, v, k_range, v_range
+        self.num_blocks, self.block_size, self.kv_heads = nb, bs, heads
+        self.k_dim, self.v_dim = 64 * chunks, v.shape[3]
+        self._c = capi.KvCacheC(k.data_ptr(), v.data_ptr(), k_range.data_ptr(), v_range.data_ptr(), nb, bs, heads,
+                                self.k_dim, self.v_dim)
+        self._p = ctypes.pointer(self._c)
+        n = _I64()
+        capi.call("qmoe_kv_attend_workspace", self._p, 0, 0, heads, 0, 0, ctypes.byref(n))   # checks the shape
+
+    def _rows(self, x, name: str, heads: int, dim: int, dtype) -> Tuple[int, int]:
+        """(pointer, token stride) of [tokens, heads, dim] whose heads are packed."""
+        if x.dim() != 3 or tuple(x.shape[1:]) != (heads, dim):
+            raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {list(x.shape)}")
+        if x.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+        if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
+            raise ValueError(f"the heads of {name} must be packed")
+        if x.shape[0] > 1 and x.stride(0) < heads * dim:
+            raise ValueError(f"the tokens of {name} overlap")
+        return x.data_ptr(), max(x.stride(0), heads * dim)
+
+    def append(self, k, v, slots) -> None:
+        """Rows k [tokens, kv_heads, k_dim] and v [tokens, kv_heads, v_dim] (views
+        whose heads are packed, e.g. of one projection's rows) to slots [tokens]
+        (plan_pages); rows with slot -1 are skipped."""
+        _on(self.ctx, k=k, v=v, slots=slots)
+        dt = _dtype_code(k)
+        kp, ks = self._rows(k, "k", self.kv_heads, self.k_dim, k.dtype)
+        vp, vs = self._rows(v, "v", self.kv_heads, self.v_dim, k.dtype)
+        T = k.shape[0]
+        if v.shape[0] != T:
+            raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
+        sp = _i32(slots, "slots", (T,))
+        self.ctx.use_current_torch_stream()
+        capi.call("qmoe_kv_append", self.ctx.handle, self._p, kp, vp, dt, T, ks, vs, sp)
+
+    def attend(self, q, q_start, kv_lens, block_table, scale: Optional[float] = None, max_kv: int = 0, out=None):
+        """Causal attention of q [tokens, heads, k_dim] over the cache; rows
+        q_start[r] .. q_start[r + 1] are the last tokens of request r, whose
+        kv_lens[r] tokens are in the blocks of block_table[r].  -> [tokens, heads,
+        v_dim].  Rows that see nothing are zeros; rows past the last request are
+        left as `out` has them (zeros without one).  max_kv: the longest kv_lens
+        if the host knows it (for speed alone)."""
+        _on(self.ctx, q=q, q_start=q_start, kv_lens=kv_lens, block_table=block_table)
+        dt = _dtype_code(q)
+        if q.dim() != 3:
+            raise ValueError(f"q must be [tokens, heads, {self.k_dim}], got {list(q.shape)}")
+        T, heads, _ = q.shape
+        qp, qs = self._rows(q, "q", heads, self.k_dim, q.dtype)
+        if block_table.dim() != 2:
+            raise ValueError("block_table must be [requests, max_blocks]")
+        R, width = block_table.shape
+        sp, lp, tp = (_i32(q_start, "q_start", (R + 1,)), _i32(kv_lens, "kv_lens", (R,)),
+                      _i32(block_table, "block_table", (R, width)))
+        if out is None:
+            out = torch.zeros(T, heads, self.v_dim, dtype=q.dtype, device=q.device)
+        else:
+            _on(self.ctx, out=out)
+            if out.shape[0] != T:
+                raise ValueError(f"out has {out.shape[0]} tokens, q {T}")
+        op, os_ = self._rows(out, "out", heads, self.v_dim, q.dtype)
+        n = _I64()
+        capi.call("qmoe_kv_attend_workspace", self._p, T, R, heads, width, int(max_kv), ctypes.byref(n))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
+        self.ctx.use_current_torch_stream()
+        capi.call("qmoe_kv_attend", self.ctx.handle, self._p, qp, dt, T, qs, heads, sp, lp, R, tp, width,
+                  int(max_kv), float(self.k_dim ** -0.5 if scale is None else scale), op, os_,
+                  ws.data_ptr() if ws is not None else None, n.value)
+        return out
+
+
+def layer_norm(x, weight, bias, eps: float = 1e-6, ctx: Optional[Context] = None):
+    """The block's LayerNorm (qmoe-rs src/model.rs:366-367) of x [tokens, hidden_dim]."""
+    ctx = _context_of(x, ctx)
+    _on(ctx, x=x, weight=weight, bias=bias)
+    dt = _dtype_code(x)
+    if x.dim() != 2 or weight.shape != (x.shape[1],) or bias.shape != weight.shape:
+        raise ValueError(f"x {list(x.shape)}, weight {list(weight.shape)}, bias {list(bias.shape)}")
+    if weight.dtype != torch.float32 or bias.dtype != torch.float32:
+        raise TypeError("weight and bias must be float32")
+    x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
+    out = torch.empty_like(x)
+    ctx.use_current_torch_stream()
+    capi.call("qmoe_layer_norm", ctx.handle, x.data_ptr(), dt, x.shape[0], x.shape[1], weight.data_ptr(),
+              bias.data_ptr(), float(eps), out.data_ptr())
+    return out
+
+
+class AttentionBlock:
+    """The attention half of a decoder layer (qmoe-rs src/model.rs:372-378,
+    :394-400), with 8-bit projections and cache:
+
+        y = LN(x);  q, k, v = qkv(y);  append k, v;  x + out(attention(q))
+
+    qkv: Int8Tensor [heads * k_dim + kv_heads * (k_dim + v_dim), hidden], the
+    rows of q, k and v one after the other; out: Int8Tensor [hidden, heads *
+    v_dim]; norm: (weight, bias, eps) of the input LayerNorm.  `rotate(q, k,
+    positions) -> (q, k)`, where given, applies the model's position encoding
+    (torch work on the current stream) before the keys are cached."""
+
+    def __init__(self, cache: KVCache, qkv: Int8Tensor, out: Int8Tensor, heads: int, norm,
+                 scale: Optional[float] = None, rotate: Optional[Callable] = None):
+        c = cache
+        rows = heads * c.k_dim + c.kv_heads * (c.k_dim + c.v_dim)
+        if heads % c.kv_heads:
+            raise ValueError(f"heads {heads} must be a multiple of kv_heads {c.kv_heads}")
+        if qkv.shape[0] != rows or out.shape != (qkv.shape[1], heads * c.v_dim):
+            raise ValueError(f"qkv {list(qkv.shape)} must be [{rows}, hidden] and out {list(out.shape)} "
+                             f"[hidden, {heads * c.v_dim}]")
+        self.cache, self.qkv, self.out, self.heads = cache, qkv, out, heads
+        self.norm, self.scale, self.rotate = norm, scale, rotate
+
+    def forward(self, x, plan: PagePlan):
+        """x [tokens, hidden] -> x + attention half; plan: plan_pages of the step."""
+        c, H = self.cache, self.heads
+        weight, bias, eps = self.norm
+        y = self.qkv.forward(layer_norm(x, weight, bias, eps, c.ctx))
+        q, k, v = y.split([H * c.k_dim, c.kv_heads * c.k_dim, c.kv_heads * c.v_dim], dim=1)
+        q, k, v = q.unflatten(1, (H, c.k_dim)), k.unflatten(1, (c.kv_heads, c.k_dim)), v.unflatten(1, (c.kv_heads, c.v_dim))
+        if self.rotate is not None:
+            q, k = self.rotate(q, k, plan.positions)
+        c.append(k, v, plan.slots)
+        o = c.attend(q, plan.q_start, plan.kv_lens, plan.block_table, self.scale, plan.max_kv)
+        return self.out.forward(o.flatten(1), residual=x.contiguous())

@@ -32,6 +32,7 @@ QMOE_PATH_DECODE_SPLIT = 3
 QMOE_NOALLOC_MAX_BATCH = 16384
 QMOE_NOALLOC_MAX_IN_FEATURES = 8192
 QMOE_EP_HANDLE_BYTES = 64
+QMOE_INT8_MAX_IN_FEATURES = 131072
 
 
 class QmoeError(RuntimeError):
@@ -65,6 +66,20 @@ class ExpertWeightsC(ctypes.Structure):
         ("up_scales", ctypes.c_void_p),
         ("down_packed", ctypes.c_void_p),
         ("down_scales", ctypes.c_void_p),
+    ]
+
+
+class KvCacheC(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_range", ctypes.c_void_p),
+        ("v_range", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("k_dim", ctypes.c_int32),
+        ("v_dim", ctypes.c_int32),
     ]
 
 
@@ -117,6 +132,20 @@ SIGNATURES = {
     "qmoe_ep_dispatch": (_I, [_P, _P, _I64, _P, _P, _P]),
     "qmoe_ep_wait": (_I, [_P, _I]),
     "qmoe_ep_return": (_I, [_P, _P]),
+    "qmoe_quantize_int8": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P]),
+    "qmoe_int8_create": (_I, [_P, _P, _P, _I64, _I64, _I, _PP]),
+    "qmoe_int8_destroy": (_I, [_P]),
+    "qmoe_int8_shape": (_I, [_P, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
+    "qmoe_int8_workspace": (_I, [_P, _I64, ctypes.POINTER(_I64)]),
+    "qmoe_int8_forward": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _P, _I64]),
+    "qmoe_kv_plan": (_I, [_P, _P, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P,
+                          _P, _P]),
+    "qmoe_kv_append": (_I, [_P, ctypes.POINTER(KvCacheC), _P, _P, _I, _I64, _I64, _I64, _P]),
+    "qmoe_kv_attend_workspace": (_I, [ctypes.POINTER(KvCacheC), _I64, _I64, _I32, _I64, _I64,
+                                      ctypes.POINTER(_I64)]),
+    "qmoe_kv_attend": (_I, [_P, ctypes.POINTER(KvCacheC), _P, _I, _I64, _I64, _I32, _P, _P, _I64, _P,
+                            _I64, _I64, ctypes.c_float, _P, _I64, _P, _I64]),
+    "qmoe_layer_norm": (_I, [_P, _P, _I, _I64, _I64, _P, _P, ctypes.c_float, _P]),
     "qmoe_layer_set_profiling": (_I, [_P, _I]),
     "qmoe_layer_stage_times": (_I, [_P, ctypes.POINTER(ctypes.c_float), _I,
                                     ctypes.POINTER(ctypes.c_int)]),

@@ -450,24 +450,42 @@ class QMoELayer:
 
 class BlockChain:
     """The layer loop of DeepSeekCoderV2::forward_next (src/model.rs:481-489)
-    over the MoE halves of consecutive decoder layers (attention left out):
-    x -> block_0 -> block_1 -> ..., each block a QMoELayer with its
-    post-attention LayerNorm set.  Repeated calls with the same buffers replay
-    one captured CUDA graph of all the layers' launches."""
+    over consecutive decoder layers: x -> block_0 -> block_1 -> ..., each block
+    a QMoELayer with its post-attention LayerNorm set.
 
-    def __init__(self, layers: Sequence["QMoELayer"]):
+    Without `attention` it runs the MoE halves alone, and repeated calls with
+    the same buffers replay one captured CUDA graph of all the layers'
+    launches.  With `attention`, one AttentionBlock a layer, it runs whole
+    layers (attention half, then MoE half) and forward takes the step's plan
+    (plan_pages); its launches can be captured into the caller's graph once
+    the layers are reserved."""
+
+    def __init__(self, layers: Sequence["QMoELayer"], attention: Optional[Sequence] = None):
         if not layers:
             raise ValueError("a chain needs at least one layer")
         self.layers = list(layers)
+        self.attention = list(attention) if attention is not None else None
+        if self.attention is not None:
+            if len(self.attention) != len(self.layers):
+                raise ValueError(f"{len(self.attention)} attention halves for {len(self.layers)} layers")
+            for L, a in zip(self.layers, self.attention):
+                if a.qkv.shape[1] != L.config.hidden_dim:
+                    raise ValueError(f"attention of width {a.qkv.shape[1]} in a layer of {L.config.hidden_dim}")
         self.ctx = self.layers[0].ctx
         arr = (ctypes.c_void_p * len(self.layers))(*[L.handle.value for L in self.layers])
         h = ctypes.c_void_p()
         capi.call("qmoe_chain_create", arr, len(self.layers), ctypes.byref(h))
         self._h = h
 
-    def forward(self, xs, out=None):
+    def forward(self, xs, out=None, plan=None):
         T, H = xs.shape
         dt = _dtype_code(xs)
+        if (plan is None) != (self.attention is None):
+            raise ValueError("a chain with attention needs a plan, one without takes none")
+        if self.attention is not None:
+            for i, (a, L) in enumerate(zip(self.attention, self.layers)):
+                xs = L.forward_block(a.forward(xs, plan), out=out if i == len(self.layers) - 1 else None)
+            return xs
         if out is None:
             out = _empty_like_kind(xs, (T, H), dt)
         xp, kind, keep = _ptr(xs)
