@@ -562,8 +562,8 @@ QMOE_API int qmoe_kv_append(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const voi
  * heads is a multiple of kv_heads.  max_kv: the longest kv_lens if the caller
  * knows it, else 0 (max_blocks * block_size is taken); only the time depends
  * on it.  Repeated calls give the same bits. */
-QMOE_API int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int64_t T, int64_t requests, int32_t heads,
-                                      int64_t max_blocks, int64_t max_kv, int64_t *bytes);
+QMOE_API int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int dtype, int64_t T, int64_t requests,
+                                      int32_t heads, int64_t max_blocks, int64_t max_kv, int64_t *bytes);
 QMOE_API int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int dtype, int64_t T,
                             int64_t q_stride, int32_t heads, const int32_t *q_start, const int32_t *kv_lens,
                             int64_t requests, const int32_t *block_table, int64_t max_blocks, int64_t max_kv,

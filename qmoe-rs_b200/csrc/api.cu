@@ -2325,13 +2325,15 @@ static int check_attend(const qmoe_kv_cache *cache, KvCacheDev &c, int64_t T, in
     return QMOE_OK;
 }
 
-int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int64_t T, int64_t requests, int32_t heads,
+int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int dtype, int64_t T, int64_t requests, int32_t heads,
                              int64_t max_blocks, int64_t max_kv, int64_t *bytes) {
     if (!bytes) return fail(QMOE_ERR_INVALID, "NULL argument");
+    QTRY(check_dtype(dtype));
     KvCacheDev c{};
     QTRY(check_attend(cache, c, T, requests, heads, max_blocks, max_kv));
-    *bytes = (int64_t)(sizeof(float) *
-                       attend_workspace_floats(T, heads, c.v_dim, attend_splits(T, requests, heads, c.heads, max_kv)));
+    int splits, chunk;
+    attend_pieces(c, T, requests, heads, dtype, max_kv, splits, chunk);
+    *bytes = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, c.v_dim, splits));
     return QMOE_OK;
 }
 
@@ -2351,7 +2353,9 @@ int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int
                     (long long)out_stride);
     if (!(scale == scale) || scale - scale != 0.0f) return fail(QMOE_ERR_INVALID, "scale must be finite");
     DeviceGuard g(ctx->device);
-    p.splits = attend_splits(T, requests, heads, p.c.heads, max_kv);
+    attend_pieces(p.c, T, requests, heads, dtype, max_kv, p.splits, p.chunk);
+    p.vec_q = reinterpret_cast<uintptr_t>(q) % (4 * dtype_size(dtype)) == 0 && q_stride % 4 == 0;
+    p.err = error_flag();
     const int64_t need = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, p.c.v_dim, p.splits));
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
         return fail(QMOE_ERR_INVALID, "workspace of %lld bytes (16-byte aligned), %lld needed",

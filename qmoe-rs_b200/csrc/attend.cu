@@ -14,13 +14,19 @@
 // with f32 activations q and P are the sums of two fp16 terms (22 bits).  The
 // 64-token sums of P cv are added to the running ones in f32.
 //
-// The layout of the cache is the operands': within 64 tokens, lane 4 g + c of
-// a warp takes the 16 bytes of K that are dims 16 c .. 16 c + 15 of a token and
-// the 16 bytes of V that are tokens 16 c .. 16 c + 15 of a dim, and each 4 bytes
-// of them are one B fragment of mma.m16n8k16.  Column 2 c + i of score tile j
-// is token 16 c + 2 j + i, so a lane's scores all lie in one block.
+// The tensor cores form S^T = K q^T and O^T = V^T P^T (mma.m16n8k16): tokens,
+// then dims, are the 16 rows, query rows (tokens x heads that share a kv head)
+// the 8 columns, so that a single token with a few heads wastes little.  The
+// layout of the cache is the operands': of a 64-token tile, lane 4 g + c takes
+// the 16 bytes of K that are dims 16 c .. 16 c + 15 (of each 64) of its tokens
+// and the 16 bytes of V that are tokens 16 c .. 16 c + 15 of its dims, and every
+// 4 bytes of them are half of an A fragment.  Row r of token tile u is token
+// 16 ((r % 8) / 2) + 4 u + 2 (r / 8) + r % 2: transposed eight by eight
+// (movmatrix), the scores' fragments are then P^T's for those bytes of V, and a
+// lane's scores all lie in one group of 16 tokens, hence in one block.
 #include "code8.cuh"
 #include "kernels.h"
+#include "sm100.cuh"
 
 #include <cuda_fp16.h>
 
@@ -56,12 +62,22 @@ QMOE_DEV void codes_to_half(uint32_t v, uint32_t &lo, uint32_t &hi) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
 }
 
+// Four codes as 1152 + c.
+QMOE_DEV void codes_biased(uint32_t v, uint32_t &lo, uint32_t &hi) {
+    v ^= 0x80808080u;
+    lo = __byte_perm(v, 0x64646464u, 0x4140);
+    hi = __byte_perm(v, 0x64646464u, 0x4342);
+}
+
 QMOE_DEV void mma_f16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+
+// 32-bit word t of v (t a constant after unrolling).
+QMOE_DEV uint32_t word_of(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
 
 // The largest r in [0, R) with start[r] / tq + r <= slot.  Tiles of request r
 // take the slots from there on; start never falls, so neither does that.  A
@@ -81,17 +97,27 @@ QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int
     return lo;
 }
 
-struct Rows {                                    // of one CTA: up to 16 rows of one request and kv head
+// tok / block for a multiple of 16: per_block = ceil(2^36 / (block / 16)); exact
+// below 2^31, since the error of the product is below 2^27 * 16 < 2^36 / 16.
+QMOE_DEV int block_index(const AttendParams &p, int tok) {
+    return (int)(((uint64_t)(uint32_t)(tok >> 4) * p.per_block) >> 36);
+}
+
+struct Rows {                                    // of one CTA: rows of one request and kv head
     int64_t t0;                                  // token of row 0
-    int tokens, gq, head0;                       // row i * gq + g: token t0 + i, head head0 + g
+    int tokens, head0;                           // row i * gq + g: token t0 + i, head head0 + g
     int pos0;                                    // last key of token t0 (may be negative)
     int keys;                                    // keys of the last token
     int64_t request;
 };
 
-QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, int gq, int hg, Rows &w) {
+// Which requests a launch serves.
+enum Serve { kAll = 0, kSingle = 1, kSeveral = 2 };
+
+QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, int serve, Rows &w) {
     const int64_t r = find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
+    if (serve == kSingle ? n != 1 : serve == kSeveral && n == 1) return false;
     const int64_t i0 = (slot - (s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
@@ -104,26 +130,51 @@ QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, int gq, int
     const int64_t keys = pos0 + cnt;             // one past the last token's last key
     w.request = r;
     w.tokens = (int)cnt;
-    w.gq = gq;
     w.pos0 = (int)(pos0 < -(1 << 30) ? -(1 << 30) : pos0);
     w.keys = (int)(keys < 0 ? 0 : keys > most ? most : keys);
     return true;
 }
 
-template <int DK, int DV, bool BF16>
+// Every warp keeps a ring of its own in shared memory: halves of a tile (the K
+// of 64 tokens, then their V), fetched by bulk copies a 16-token group each,
+// the next ones in flight while one is worked on.  16 tokens of V start 32
+// bytes off a multiple of 128 from the ones before, so the lanes of a quarter
+// warp (two dims, four groups) read 128 bytes of distinct banks.
+constexpr int kSlots = 3;
+
+template <int DK, int DV, int NT>
 struct Shared {
-    static constexpr int kTerms = BF16 ? 1 : 2;
-    uint4 q[kTerms][DK / 16][32];                // A fragments of q
-    float back[16];                              // 2^-k of the row's scaling
-    float m[kWarps][16], l[kWarps][16];
-    float o[kWarps][16][DV];
+    static constexpr int kVGroup = DV * 16 + 32;
+    static constexpr int kSlot = (64 * DK > 4 * kVGroup ? 64 * DK : 4 * kVGroup);
+    union {
+        uint8_t ring[kWarps][kSlots][kSlot];
+        float o[kWarps][8 * NT][DV + 4];         // once the ring is done with
+    };
+    float m[kWarps][8 * NT], l[kWarps][8 * NT];
+    uint64_t full[kWarps][kSlots];
+    int abort;
 };
 
-template <int DK, int DV, bool BF16>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p, int tq, int gq, int hgroups) {
+QMOE_DEV void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     sm100::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+
+// Eight by eight 16-bit values, transposed.
+QMOE_DEV uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// NT * 8 query rows, gq heads by tq tokens of them in use.
+template <int DK, int DV, bool BF16, int NT>
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p, int tq, int gq, int hgroups, int serve) {
     constexpr int kTerms = BF16 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    using Sm = Shared<DK, DV, BF16>;
+    using Sm = Shared<DK, DV, NT>;
     Sm &S = *reinterpret_cast<Sm *>(smem_raw);
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
@@ -131,182 +182,332 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p, 
     const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups, split = blockIdx.z;
     const int G = p.heads / p.c.heads;
     Rows w;
-    if (!find_rows(p, blockIdx.x, tq, gq, hg, w)) return;        // the whole CTA alike
-    w.head0 = h * G + hg * 16;
-    const int heads_here = G - hg * 16 < gq ? G - hg * 16 : gq;
+    if (!find_rows(p, blockIdx.x, tq, serve, w)) return;                // the whole CTA alike
+    w.head0 = h * G + hg * gq;
+    const int heads_here = G - hg * gq < gq ? G - hg * gq : gq;
     const int bs = p.c.block;
 
-    // ---- q: scale rows by a power of two, lay out the A fragments
-    for (int row = warp; row < 16; row += kWarps) {
-        const int i = row / gq, gg = row - i * gq;
+    const int tiles = (w.keys + 63) / 64;
+    // pieces of p.chunk tiles, larger where the request is longer than the host was told
+    const int even = (tiles + p.splits - 1) / p.splits, chunk = p.chunk > even ? p.chunk : even;
+    const int t_lo = split * chunk, t_hi = t_lo + chunk < tiles ? t_lo + chunk : tiles;
+    const int mine = t_hi > t_lo + warp ? (t_hi - t_lo - warp + kWarps - 1) / kWarps : 0;   // tiles of this warp
+    const int32_t *row_table = p.table + w.request * p.max_blocks;
+    const int grp = g >> 1;                       // this lane's group of 16 tokens in a tile
+    // the block and head of this lane's group of the warp's k-th tile, -1 past
+    // the keys and where the table's entry is none
+    auto block_of = [&](int k) -> int64_t {
+        if (k >= mine) return -1;
+        const int tok = (t_lo + warp + k * kWarps) * 64 + 16 * grp;
+        if (tok >= w.keys) return -1;
+        const int64_t b = row_table[block_index(p, tok)];
+        return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
+    };
+    // copies of item n (K of tile n / 2, or its V) into slot n % kSlots: an even
+    // lane g a piece of 64 dims each of K, or c = 0 its group of V
+    auto fetch = [&](int n, int64_t bh) {
+        if (n >= 2 * mine) return;
+        const int tok = (t_lo + warp + (n >> 1) * kWarps) * 64 + 16 * grp, off = tok - block_index(p, tok) * bs;
+        uint8_t *dst = S.ring[warp][n % kSlots];
+        uint64_t *bar = &S.full[warp][n % kSlots];
+        const bool is_v = n & 1;
+        const bool copy = bh >= 0 && (g & 1) == 0 && c < (is_v ? 1 : DK / 64);
+        const uint32_t bytes = is_v ? DV * 16 : 1024;
+        const uint32_t count = __popc(__ballot_sync(0xffffffffu, copy));
+        if (lane == 0) sm100::mbar_arrive_expect_tx(bar, count * bytes);
+        __syncwarp();
+        if (copy) {
+            if (is_v)
+                bulk_load(dst + grp * Sm::kVGroup, p.c.v + (bh * (bs / 16) + off / 16) * (DV * 16), bytes, bar);
+            else
+                bulk_load(dst + c * 4096 + grp * 1024, p.c.k + ((bh * (DK / 64) + c) * bs + off) * 64, bytes, bar);
+        }
+    };
+
+    int64_t blk = block_of(0), blk1 = block_of(1), blk2 = block_of(2);
+    if (tid == 0) {
+        for (int i = 0; i < kWarps * kSlots; ++i) sm100::mbar_init(&S.full[0][0] + i, 1);
+        S.abort = 0;
+        sm100::fence_mbar_init();
+    }
+    __syncthreads();
+    fetch(0, blk);
+    fetch(1, blk);
+    fetch(2, blk1);
+    float kr = blk >= 0 ? p.c.k_range[blk] : 0.0f, vr = blk >= 0 ? p.c.v_range[blk] : 127.0f;
+
+    // ---- q: rows brought to fp16 by a power of two, as B fragments: lane 4 g + c
+    // has dims 64 J + 16 c + 4 t + {0, 1 | 2, 3} of row 8 x + g for step 4 J + t
+    uint32_t qf[kTerms][NT][DK / 16][2];
+    float back[NT][2], bias[NT][2];               // of this lane's columns 2 c, 2 c + 1
+    int last[NT][2];                              // their last keys
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int row = 8 * x + g, i = row / gq, gg = row - i * gq;
         const bool live = i < w.tokens && gg < heads_here;
+        const int64_t at = live ? (w.t0 + i) * p.ldq + (int64_t)(w.head0 + gg) * DK + 16 * c : 0;
+        float v[DK / 64][16];
         float m = 0.0f;
-        const int64_t at = live ? (w.t0 + i) * p.ldq + (int64_t)(w.head0 + gg) * DK : 0;
-        if (live)
-            for (int d = lane; d < DK; d += 32) m = fmaxf(m, fabsf(load_act(p.q, p.dtype, at + d)));
-        m = warp_max(m);
+#pragma unroll
+        for (int J = 0; J < DK / 64; ++J)
+#pragma unroll
+            for (int d = 0; d < 16; d += 4) {
+                const float4 f = !live ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                       : p.vec_q ? load_act4(p.q, p.dtype, at + 64 * J + d)
+                                                 : make_float4(load_act(p.q, p.dtype, at + 64 * J + d),
+                                                               load_act(p.q, p.dtype, at + 64 * J + d + 1),
+                                                               load_act(p.q, p.dtype, at + 64 * J + d + 2),
+                                                               load_act(p.q, p.dtype, at + 64 * J + d + 3));
+                v[J][d] = f.x;
+                v[J][d + 1] = f.y;
+                v[J][d + 2] = f.z;
+                v[J][d + 3] = f.w;
+                m = max_abs(max_abs(max_abs(max_abs(m, f.x), f.y), f.z), f.w);
+            }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
         int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
         e = e < -100 ? -100 : e > 100 ? 100 : e;
         const float up = pow2i(14 - e);
-        if (lane == 0) S.back[row] = pow2i(e - 14);
-        for (int d = 4 * lane; d < DK; d += 128) {
-            float v[4];
+        float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = live ? __fmul_rn(load_act(p.q, p.dtype, at + d + j), up) : 0.0f;
-            // dims 64 J + 16 c + 4 t + {0,1 | 2,3} are k = {2c, 2c+1 | 2c+8, 2c+9} of step 4 J + t
-            const int step = (d >> 6) * 4 + ((d >> 2) & 3), cc = (d >> 4) & 3;
-            uint32_t lo = h2(v[0], v[1]), hi = h2(v[2], v[3]);
+        for (int J = 0; J < DK / 64; ++J)
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term) {
-                uint32_t *f = reinterpret_cast<uint32_t *>(&S.q[term][step][4 * (row & 7) + cc]) + (row >> 3);
-                f[0] = lo;
-                f[2] = hi;
-                if (kTerms == 2) {
-                    lo = h2(__fsub_rn(v[0], h_lo(lo)), __fsub_rn(v[1], h_hi(lo)));
-                    hi = h2(__fsub_rn(v[2], h_lo(hi)), __fsub_rn(v[3], h_hi(hi)));
-                }
+            for (int t = 0; t < 8; ++t) {
+                const float a = __fmul_rn(v[J][2 * t], up), b = __fmul_rn(v[J][2 * t + 1], up);
+                const uint32_t hi = h2(a, b);
+                sum += h_lo(hi) + h_hi(hi);
+                qf[0][x][4 * J + t / 2][t & 1] = hi;
+                if (kTerms == 2)
+                    qf[kTerms - 1][x][4 * J + t / 2][t & 1] = h2(__fsub_rn(a, h_lo(hi)), __fsub_rn(b, h_hi(hi)));
             }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float down = pow2i(e - 14);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {             // row g's lanes 4 g .. have it: fetch those of the columns
+            back[x][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + i));
+            bias[x][i] = -1152.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * c + i));
+            last[x][i] = w.pos0 + (8 * x + 2 * c + i) / gq;
         }
     }
-    __syncthreads();
 
-    float acc[DV / 8][4];
+    float acc[DV / 16][NT][4];
 #pragma unroll
-    for (int t = 0; t < DV / 8; ++t)
+    for (int t = 0; t < DV / 16; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][j] = 0.0f;
-    float mx[2] = {neg_inf(), neg_inf()}, sum[2] = {0.0f, 0.0f};
-    const float back[2] = {S.back[g], S.back[g + 8]};
-    int last[2];                                  // last key of rows g, g + 8
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-    for (int a = 0; a < 2; ++a) last[a] = w.pos0 + (g + 8 * a) / gq;
+            for (int i = 0; i < 4; ++i) acc[t][x][i] = 0.0f;
+    float mx[NT][2], sum[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mx[x][i] = neg_inf();
+            sum[x][i] = 0.0f;
+        }
 
-    const int tiles = (w.keys + 63) / 64, per = (tiles + p.splits - 1) / p.splits;
-    const int t_lo = split * per, t_hi = t_lo + per < tiles ? t_lo + per : tiles;
-    const int32_t *row_table = p.table + w.request * p.max_blocks;
-    // the block of 16 tokens from `tok` on, -1 past the keys and where the entry is none
-    auto block_of = [&](int tok) -> int64_t {
-        if (tok >= w.keys) return -1;
-        const int64_t b = row_table[tok / bs];
-        return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
-    };
-    for (int tile = t_lo + warp; tile < t_hi; tile += kWarps) {
-        const int tk = tile * 64 + 16 * (g >> 1), tv = tile * 64 + 16 * c;
-        const int64_t bk = block_of(tk), bv = block_of(tv);
-        // ---- scores
-        float s[8][4];
+    bool ok = true;
+    int n = 0;                                    // items worked on
+    for (int k = 0; k < mine; ++k) {
+        const int tg = (t_lo + warp + k * kWarps) * 64 + 16 * grp + (g & 1);   // token of row g, tile u: tg + 4 u
+        const float kr1 = blk1 >= 0 ? p.c.k_range[blk1] : 0.0f, vr1 = blk1 >= 0 ? p.c.v_range[blk1] : 127.0f;
+        const int64_t blk3 = block_of(k + 3);
+        // ---- scores.  One term: the codes as 1152 + c, the sum of q taken off at
+        // the start (its rounding, 2^-24 of 1152 sum q, is small beside bf16's);
+        // two terms: the codes themselves, the small term first and each 64 dims
+        // in sums of their own, added in f32.
+        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][n % kSlots], (n / kSlots) & 1, &S.abort, p.err))) break;
+        const uint8_t *slot = S.ring[warp][n % kSlots] + (16 * grp + (g & 1)) * 64 + c * 16;
+        float s[4][NT][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = 0.0f;
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u][x][i] = kTerms == 1 ? bias[x][i & 1] : 0.0f;
 #pragma unroll
         for (int J = 0; J < DK / 64; ++J) {
             uint4 kc[8];
-            const int8_t *src = p.c.k + ((bk * (DK / 64) + J) * bs + tk % bs + (g & 1)) * 64 + c * 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                kc[j] = bk >= 0 ? *reinterpret_cast<const uint4 *>(src + j * 128) : make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < 8; ++j) kc[j] = *reinterpret_cast<const uint4 *>(slot + J * 4096 + j * 128);
+            if (kTerms == 1) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const uint4 a0 = S.q[0][4 * J + t][lane];
-                const uint4 a1 = kTerms == 2 ? S.q[kTerms - 1][4 * J + t][lane] : a0;
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t word = t == 0 ? kc[j].x : t == 1 ? kc[j].y : t == 2 ? kc[j].z : kc[j].w;
-                    uint32_t b0, b1;
-                    codes_to_half(word, b0, b1);
-                    mma_f16(s[j], a0, b0, b1);
-                    if (kTerms == 2) mma_f16(s[j], a1, b0, b1);
+                    for (int u = 0; u < 4; ++u) {
+                        uint4 a;
+                        codes_biased(word_of(kc[2 * u], t), a.x, a.z);
+                        codes_biased(word_of(kc[2 * u + 1], t), a.y, a.w);
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) mma_f16(s[u][x], a, qf[0][x][4 * J + t][0], qf[0][x][4 * J + t][1]);
+                    }
+            } else {
+                float part[4][NT][4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) part[u][x][i] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint4 a;
+                        codes_to_half(word_of(kc[2 * u], t & 3), a.x, a.z);
+                        codes_to_half(word_of(kc[2 * u + 1], t & 3), a.y, a.w);
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) {
+                            const uint32_t(&b)[2] = qf[t < 4 ? kTerms - 1 : 0][x][4 * J + (t & 3)];
+                            mma_f16(part[u][x], a, b[0], b[1]);
+                        }
+                    }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[u][x][i] += part[u][x][i];
+            }
+        }
+        __syncwarp();
+        fetch(n + 3, blk1);                       // V of the next tile
+        ++n;
+        // ---- softmax
+        vr = vr < kRangeFloor ? kRangeFloor : vr; // a block of zeros of another writer; NaN stays
+        const float ks = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
+        const float lv = log2f(__fdiv_rn(vr, 127.0f)), iv = __fdiv_rn(127.0f, vr);
+        // a tile that every row sees whole needs no mask
+        const bool whole = __all_sync(0xffffffffu, blk >= 0 && tg + 15 < w.keys && tg + 15 <= w.pos0);
+        float fix[NT][2];
+        uint32_t pb[kTerms][NT][4][2];            // P^T: row 8 x + g, tokens 16 c + 4 u + {0, 1 | 2, 3}
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            float top[2] = {neg_inf(), neg_inf()};
+            const float f[2] = {ks * back[x][0], ks * back[x][1]};
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u][x][i] = __fmaf_rn(s[u][x][i], f[i & 1], lv);
+            if (!whole) {
+                int see[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    see[i] = blk >= 0 ? (last[x][i] < w.keys - 1 ? last[x][i] : w.keys - 1) - tg : -1;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * u + (i & 2) > see[i & 1]) s[u][x][i] = neg_inf();
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], s[u][x][i]);
+            float base[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+                const float m = fmaxf(mx[x][i], top[i]);
+                fix[x][i] = m == neg_inf() ? 1.0f : ex2(mx[x][i] - m);
+                base[i] = m == neg_inf() ? 0.0f : m - kPShift;
+                mx[x][i] = m;
+                sum[x][i] *= fix[x][i];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[u][x][i] = ex2(s[u][x][i] - base[i & 1]);
+                    sum[x][i & 1] = __fmaf_rn(s[u][x][i], iv, sum[x][i & 1]);
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float a = s[u][x][2 * half], b = s[u][x][2 * half + 1];
+                    const uint32_t hi = h2(a, b);
+                    pb[0][x][u][half] = transpose8(hi);
+                    if (kTerms == 2) pb[kTerms - 1][x][u][half] = transpose8(h2(a - h_lo(hi), b - h_hi(hi)));
                 }
             }
         }
-        // ---- softmax
-        const float kr = bv >= 0 ? p.c.k_range[bv] : 0.0f;
-        float vr = bv >= 0 ? p.c.v_range[bv] : 127.0f;
-        vr = vr < kRangeFloor ? kRangeFloor : vr;              // a block of zeros of another writer; NaN stays
-        const float ks = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
-        const float lv = log2f(__fdiv_rn(vr, 127.0f)), iv = __fdiv_rn(127.0f, vr);
-        float top[2] = {neg_inf(), neg_inf()};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int a = i >> 1, tok = tv + 2 * j + (i & 1);
-                const float v = __fmaf_rn(s[j][i], ks * back[a], lv);
-                s[j][i] = bv >= 0 && tok < w.keys && tok <= last[a] ? v : neg_inf();
-                top[a] = fmaxf(top[a], s[j][i]);
-            }
-        float fix[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            top[a] = fmaxf(top[a], __shfl_xor_sync(0xffffffffu, top[a], 1));
-            top[a] = fmaxf(top[a], __shfl_xor_sync(0xffffffffu, top[a], 2));
-            const float m = fmaxf(mx[a], top[a]);
-            fix[a] = m == neg_inf() ? 1.0f : ex2(mx[a] - m);
-            mx[a] = m;
-            sum[a] *= fix[a];
-        }
-        const float base[2] = {mx[0] == neg_inf() ? 0.0f : mx[0] - kPShift, mx[1] == neg_inf() ? 0.0f : mx[1] - kPShift};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int a = i >> 1;
-                s[j][i] = ex2(s[j][i] - base[a]);
-                sum[a] = __fmaf_rn(s[j][i], iv, sum[a]);
-            }
         // ---- P V
-        uint4 pa[kTerms][4];
+        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][n % kSlots], (n / kSlots) & 1, &S.abort, p.err))) break;
+        slot = S.ring[warp][n % kSlots] + c * Sm::kVGroup + g * 16;
+        constexpr int kSide = NT >= 4 ? 2 : 4;    // 16-dim tiles side by side
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            pa[0][u] = make_uint4(h2(s[2 * u][0], s[2 * u][1]), h2(s[2 * u][2], s[2 * u][3]),
-                                  h2(s[2 * u + 1][0], s[2 * u + 1][1]), h2(s[2 * u + 1][2], s[2 * u + 1][3]));
-            if (kTerms == 2) {
-                const uint4 a = pa[0][u];
-                pa[kTerms - 1][u] =
-                    make_uint4(h2(s[2 * u][0] - h_lo(a.x), s[2 * u][1] - h_hi(a.x)),
-                               h2(s[2 * u][2] - h_lo(a.y), s[2 * u][3] - h_hi(a.y)),
-                               h2(s[2 * u + 1][0] - h_lo(a.z), s[2 * u + 1][1] - h_hi(a.z)),
-                               h2(s[2 * u + 1][2] - h_lo(a.w), s[2 * u + 1][3] - h_hi(a.w)));
-            }
-        }
-        const int8_t *src = p.c.v + (bv * (bs / 16) + (tv % bs) / 16) * (DV * 16) + g * 16;
+        for (int t0 = 0; t0 < DV / 16; t0 += kSide) {
+            uint4 va[kSide], vb[kSide];
+            float o[kSide][NT][4];
 #pragma unroll
-        for (int t = 0; t < DV / 8; ++t) {
-            const uint4 vc = bv >= 0 ? *reinterpret_cast<const uint4 *>(src + t * 128) : make_uint4(0, 0, 0, 0);
-            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < kSide; ++t) {
+                va[t] = *reinterpret_cast<const uint4 *>(slot + (t0 + t) * 256);
+                vb[t] = *reinterpret_cast<const uint4 *>(slot + (t0 + t) * 256 + 128);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint32_t word = u == 0 ? vc.x : u == 1 ? vc.y : u == 2 ? vc.z : vc.w;
-                uint32_t b0, b1;
-                codes_to_half(word, b0, b1);
-                mma_f16(o, pa[0][u], b0, b1);
-                if (kTerms == 2) mma_f16(o, pa[kTerms - 1][u], b0, b1);
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[t][x][i] = 0.0f;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = __fmaf_rn(acc[t][i], fix[i >> 1], o[i]);
+            for (int u = 0; u < 4 * kTerms; ++u)
+#pragma unroll
+                for (int t = 0; t < kSide; ++t) {
+                    uint4 a;
+                    codes_to_half(word_of(va[t], u & 3), a.x, a.z);
+                    codes_to_half(word_of(vb[t], u & 3), a.y, a.w);
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        const uint32_t(&b)[2] = pb[u < 4 ? kTerms - 1 : 0][x][u & 3];
+                        mma_f16(o[t][x], a, b[0], b[1]);
+                    }
+                }
+#pragma unroll
+            for (int t = 0; t < kSide; ++t)
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[t0 + t][x][i] = __fmaf_rn(acc[t0 + t][x][i], fix[x][i & 1], o[t][x][i]);
         }
+        __syncwarp();
+        fetch(n + 3, blk2);                       // K of the tile after the next
+        ++n;
+        blk = blk1;
+        blk1 = blk2;
+        blk2 = blk3;
+        kr = kr1;
+        vr = vr1;
     }
+    if (!ok) {                                    // let the copies already issued land before the CTA exits
+        for (int i = n; i < n + kSlots && i < 2 * mine; ++i)
+            for (uint32_t tries = 0; tries < sm100::kMaxWaitProbes; ++tries)
+                if (sm100::mbar_try_wait(&S.full[warp][i % kSlots], (i / kSlots) & 1)) break;
+    }
+    __syncthreads();                              // the ring is free
 
     // ---- join the warps
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-        sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 1);
-        sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 2);
-        if (c == 0) {
-            S.m[warp][g + 8 * a] = mx[a];
-            S.l[warp][g + 8 * a] = sum[a];
-        }
-    }
+    for (int x = 0; x < NT; ++x) {
 #pragma unroll
-    for (int t = 0; t < DV / 8; ++t) {
-        *reinterpret_cast<float2 *>(&S.o[warp][g][8 * t + 2 * c]) = make_float2(acc[t][0], acc[t][1]);
-        *reinterpret_cast<float2 *>(&S.o[warp][g + 8][8 * t + 2 * c]) = make_float2(acc[t][2], acc[t][3]);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum[x][i] += __shfl_xor_sync(0xffffffffu, sum[x][i], o);
+            if (g == 0) {
+                S.m[warp][8 * x + 2 * c + i] = mx[x][i];
+                S.l[warp][8 * x + 2 * c + i] = sum[x][i];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < DV / 16; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S.o[warp][8 * x + 2 * c + (i & 1)][16 * t + g + 4 * (i & 2)] = acc[t][x][i];
     }
     __syncthreads();
-    for (int row = warp; row < 16; row += kWarps) {
+    for (int row = warp; row < w.tokens * gq; row += kWarps) {
         const int i = row / gq, gg = row - i * gq;
-        if (i >= w.tokens || gg >= heads_here) continue;
+        if (gg >= heads_here) continue;
         float m = neg_inf(), f[kWarps], l = 0.0f;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) m = fmaxf(m, S.m[k][row]);
@@ -329,7 +530,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p, 
             } else {
                 const int64_t at = (t * p.heads + head) * p.splits + split;
                 float *ml = p.ws + at * 2;
-                if (d == lane && lane == 0) {
+                if (d == 0) {
                     ml[0] = m;
                     ml[1] = l;
                 }
@@ -370,48 +571,89 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p) 
     }
 }
 
-// Rows of a CTA: gq heads of a kv head by tq tokens.
-void row_shape(int G, int &gq, int &tq, int &hgroups) {
-    gq = G < 16 ? G : 16;
-    tq = 16 / gq;
-    hgroups = (G + 15) / 16;
+// Rows of a CTA: nt * 8 of them, gq heads of a kv head by tq tokens.  For a
+// request's single token as few as the heads need, for several as many as the
+// registers hold (bf16 32, f32 16), which read the keys less often.
+struct RowShape {
+    int nt, gq, tq, hgroups;
+};
+RowShape row_shape(bool single, int G, int dtype) {
+    const int most = dtype ? 4 : 2;
+    RowShape r;
+    r.nt = !single ? most : G <= 8 ? 1 : G <= 16 || most == 2 ? 2 : 4;
+    r.gq = G < 8 * r.nt ? G : 8 * r.nt;
+    r.tq = single ? 1 : 8 * r.nt / r.gq;
+    r.hgroups = (G + r.gq - 1) / r.gq;
+    return r;
+}
+
+template <int DK, int DV, bool BF16, int NT>
+cudaError_t launch_nt(const AttendParams &p, const RowShape &r, int serve, cudaStream_t s) {
+    const size_t smem = sizeof(Shared<DK, DV, NT>);
+    auto kernel = attend_kernel<DK, DV, BF16, NT>;
+    cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)(p.T / r.tq + p.R), (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
+                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups, serve);
 }
 
 template <int DK, int DV, bool BF16>
 cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
-    int gq, tq, hgroups;
-    row_shape(p.heads / p.c.heads, gq, tq, hgroups);
-    const size_t smem = sizeof(Shared<DK, DV, BF16>);
-    auto kernel = attend_kernel<DK, DV, BF16>;
-    cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
+    const int G = p.heads / p.c.heads;
+    const bool several = p.T > p.R;               // a request may have more than one token
+    cudaError_t e = cudaSuccess;
+    if (several) e = launch_nt<DK, DV, BF16, BF16 ? 4 : 2>(p, row_shape(false, G, p.dtype), kSeveral, s);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(kernel, dim3((unsigned)(p.T / tq + p.R), (unsigned)(p.c.heads * hgroups), (unsigned)p.splits),
-                   dim3(kThreads), smem, s, p, tq, gq, hgroups);
+    const RowShape r = row_shape(true, G, p.dtype);
+    const int serve = several ? kSingle : kAll;
+    if (r.nt == 1) e = launch_nt<DK, DV, BF16, 1>(p, r, serve, s);
+    else if (r.nt == 2) e = launch_nt<DK, DV, BF16, 2>(p, r, serve, s);
+    else e = launch_nt<DK, DV, BF16, BF16 ? 4 : 2>(p, r, serve, s);
     if (e != cudaSuccess || p.splits == 1) return e;
     return launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)((p.T * p.heads + 7) / 8)), dim3(256), 0, s, p);
 }
 
+// CTAs of the single-token kernel that an SM holds.
+int resident(int k_dim, int v_dim) {
+    const size_t smem = k_dim == 64    ? sizeof(Shared<64, 64, 1>)
+                        : k_dim == 128 ? sizeof(Shared<128, 128, 1>)
+                                       : sizeof(Shared<192, 128, 1>);
+    return 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
+}
+
 }  // namespace
 
-int attend_splits(int64_t T, int64_t R, int heads, int kv_heads, int64_t max_kv) {
-    int gq, tq, hgroups;
-    row_shape(heads / kv_heads, gq, tq, hgroups);
-    const int64_t rows = (T + tq - 1) / tq > R ? (T + tq - 1) / tq : R;
-    const int64_t ctas = (rows < 1 ? 1 : rows) * kv_heads * hgroups;
-    const int64_t tiles = (max_kv + 63) / 64;
-    int64_t s = (4 * (int64_t)device_sm_count() + ctas - 1) / ctas;
-    const int64_t most = (tiles + kWarps - 1) / kWarps;
-    if (s > most) s = most;
-    if (s > 64) s = 64;
-    return s < 1 ? 1 : (int)s;
+// A batch of few CTAs is cut so that they fill the device once (a request of
+// the longest length each); one of many into pieces of a quarter of that, since
+// its requests may be of any length.
+void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
+                   int &chunk) {
+    const RowShape r = row_shape(T <= R, heads / c.heads, dtype);
+    const int64_t rows = T <= R ? R : (T + r.tq - 1) / r.tq > R ? (T + r.tq - 1) / r.tq : R;
+    const int64_t ctas = (rows < 1 ? 1 : rows) * c.heads * r.hgroups;
+    const int64_t fill = (int64_t)device_sm_count() * resident(c.k_dim, c.v_dim);
+    const int64_t tiles = max_kv < 1 ? 1 : (max_kv + 63) / 64;
+    int64_t s = 4 * ctas <= fill ? fill / ctas : (4 * fill + ctas - 1) / ctas;
+    int64_t ch = (tiles + s - 1) / s;
+    ch = ch < 2 * kWarps ? 2 * kWarps : (ch + kWarps - 1) / kWarps * kWarps;
+    s = (tiles + ch - 1) / ch;
+    if (s > 256) {
+        s = 256;
+        ch = (tiles + s - 1) / s;
+    }
+    chunk = (int)ch;
+    splits = (int)s;
 }
 
 size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits) {
     return splits <= 1 ? 0 : (size_t)T * heads * splits * (v_dim + 2);
 }
 
-cudaError_t launch_attend(const AttendParams &p, cudaStream_t s) {
-    if (p.T == 0 || p.R == 0) return cudaSuccess;
+cudaError_t launch_attend(const AttendParams &params, cudaStream_t s) {
+    if (params.T == 0 || params.R == 0) return cudaSuccess;
+    AttendParams p = params;
+    const uint64_t d = (uint64_t)p.c.block / 16;
+    p.per_block = ((1ull << 36) + d - 1) / d;
     const bool bf = p.dtype != 0;
     if (p.c.k_dim == 64 && p.c.v_dim == 64) return bf ? launch_dims<64, 64, true>(p, s) : launch_dims<64, 64, false>(p, s);
     if (p.c.k_dim == 128 && p.c.v_dim == 128)

@@ -406,6 +406,7 @@ struct AttendParams {
     KvCacheDev c;
     const void *q;          // [T, heads, k_dim], tokens ldq apart
     int dtype;
+    bool vec_q;             // four elements may be loaded at once
     int64_t T, ldq;
     int heads;              // query heads
     const int32_t *q_start, *kv_lens, *table;   // [R + 1], [R], [R, max_blocks]
@@ -413,14 +414,17 @@ struct AttendParams {
     float scale;
     void *out;              // [T, heads, v_dim], tokens ldo apart
     int64_t ldo;
-    int splits;             // pieces of the keys; > 1 joins through ws
+    int splits, chunk;      // pieces of the keys (64 chunk tokens each); > 1 joins through ws
+    int *err;               // device error word
     float *ws;              // attend_workspace_floats floats
+    uint64_t per_block;     // set by launch_attend
 };
 cudaError_t launch_kv_plan(const KvPlanParams &p, cudaStream_t s);
 cudaError_t launch_kv_append(const KvAppendParams &p, cudaStream_t s);
 // Pieces that the keys of a request are cut into, for a batch whose longest
 // request holds max_kv tokens.
-int attend_splits(int64_t T, int64_t R, int heads, int kv_heads, int64_t max_kv);
+void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
+                   int &chunk);
 size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits);
 cudaError_t launch_attend(const AttendParams &p, cudaStream_t s);
 

@@ -231,7 +231,7 @@ class KVCache:
                                 self.k_dim, self.v_dim)
         self._p = ctypes.pointer(self._c)
         n = _I64()
-        capi.call("qmoe_kv_attend_workspace", self._p, 0, 0, heads, 0, 0, ctypes.byref(n))   # checks the shape
+        capi.call("qmoe_kv_attend_workspace", self._p, 0, 0, 0, heads, 0, 0, ctypes.byref(n))   # checks the shape
 
     def _rows(self, x, name: str, heads: int, dim: int, dtype) -> Tuple[int, int]:
         """(pointer, token stride) of [tokens, heads, dim] whose heads are packed."""
@@ -286,7 +286,7 @@ class KVCache:
                 raise ValueError(f"out has {out.shape[0]} tokens, q {T}")
         op, os_ = self._rows(out, "out", heads, self.v_dim, q.dtype)
         n = _I64()
-        capi.call("qmoe_kv_attend_workspace", self._p, T, R, heads, width, int(max_kv), ctypes.byref(n))
+        capi.call("qmoe_kv_attend_workspace", self._p, dt, T, R, heads, width, int(max_kv), ctypes.byref(n))
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
         self.ctx.use_current_torch_stream()
         capi.call("qmoe_kv_attend", self.ctx.handle, self._p, qp, dt, T, qs, heads, sp, lp, R, tp, width,

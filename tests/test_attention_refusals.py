@@ -38,7 +38,7 @@ BAD_CACHES = [(dict(block_size=8), capi.QMOE_ERR_INVALID), (dict(block_size=24),
 @pytest.mark.parametrize("change,code", BAD_CACHES, ids=lambda v: str(v))
 def test_caches(ctx, change, code):
     n = ctypes.c_int64()
-    got, msg = rc("qmoe_kv_attend_workspace", cache(**change), 1, 1, 2, 4, 0, ctypes.byref(n))
+    got, msg = rc("qmoe_kv_attend_workspace", cache(**change), 0, 1, 1, 2, 4, 0, ctypes.byref(n))
     assert got == code and msg
     got, _ = rc("qmoe_kv_append", ctx, cache(**change), 4096, 4096, 0, 1, 128, 128, 4096)
     assert got == code
