@@ -111,13 +111,9 @@ struct Rows {                                    // of one CTA: rows of one requ
     int64_t request;
 };
 
-// Which requests a launch serves.
-enum Serve { kAll = 0, kSingle = 1, kSeveral = 2 };
-
-QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, int serve, Rows &w) {
+QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Rows &w) {
     const int64_t r = find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    if (serve == kSingle ? n != 1 : serve == kSeveral && n == 1) return false;
     const int64_t i0 = (slot - (s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
@@ -169,22 +165,14 @@ QMOE_DEV uint32_t transpose8(uint32_t v) {
     return r;
 }
 
-// NT * 8 query rows, gq heads by tq tokens of them in use.
+// A CTA's rows on NT * 8 columns: row i * gq + g of w.
 template <int DK, int DV, bool BF16, int NT>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p, int tq, int gq, int hgroups, int serve) {
+QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split, int gq, int heads_here,
+                          uint8_t *smem_raw) {
     constexpr int kTerms = BF16 ? 1 : 2;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
     using Sm = Shared<DK, DV, NT>;
     Sm &S = *reinterpret_cast<Sm *>(smem_raw);
-    QMOE_PDL_WAIT();
-    QMOE_PDL_TRIGGER();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups, split = blockIdx.z;
-    const int G = p.heads / p.c.heads;
-    Rows w;
-    if (!find_rows(p, blockIdx.x, tq, serve, w)) return;                // the whole CTA alike
-    w.head0 = h * G + hg * gq;
-    const int heads_here = G - hg * gq < gq ? G - hg * gq : gq;
     const int bs = p.c.block;
 
     const int tiles = (w.keys + 63) / 64;
@@ -540,6 +528,31 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     }
 }
 
+// Columns of a request's several tokens, as many as the registers hold: the
+// more, the less often the keys are read.
+__host__ __device__ constexpr int most_columns(bool bf16) { return bf16 ? 4 : 2; }
+
+// Up to tq tokens of a request by gq heads of a kv head.  One token (its heads
+// on N1 * 8 columns) and several may meet in a batch; SEVERAL says whether they
+// can.
+template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p, int tq, int gq, int hgroups) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    QMOE_PDL_WAIT();
+    QMOE_PDL_TRIGGER();
+    const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups;
+    const int G = p.heads / p.c.heads;
+    Rows w;
+    if (!find_rows(p, blockIdx.x, tq, w)) return;                // the whole CTA alike
+    w.head0 = h * G + hg * gq;
+    const int heads_here = G - hg * gq < gq ? G - hg * gq : gq;
+    constexpr int kMost = most_columns(BF16);
+    if (SEVERAL && N1 != kMost && w.tokens > 1)
+        attend_rows<DK, DV, BF16, kMost>(p, w, h, blockIdx.z, gq, heads_here, smem_raw);
+    else
+        attend_rows<DK, DV, BF16, N1>(p, w, h, blockIdx.z, gq, heads_here, smem_raw);
+}
+
 // Joins the pieces: one warp per (token, head).
 template <int DV, bool BF16>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p) {
@@ -571,44 +584,40 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p) 
     }
 }
 
-// Rows of a CTA: nt * 8 of them, gq heads of a kv head by tq tokens.  For a
-// request's single token as few as the heads need, for several as many as the
-// registers hold (bf16 32, f32 16), which read the keys less often.
 struct RowShape {
-    int nt, gq, tq, hgroups;
+    int n1;                                       // columns / 8 of a single token
+    int gq, tq, hgroups;
+    bool several;                                 // a request may have more than one token
 };
-RowShape row_shape(bool single, int G, int dtype) {
-    const int most = dtype ? 4 : 2;
+RowShape row_shape(int64_t T, int64_t R, int G, int dtype) {
+    const int most = most_columns(dtype != 0);
     RowShape r;
-    r.nt = !single ? most : G <= 8 ? 1 : G <= 16 || most == 2 ? 2 : 4;
-    r.gq = G < 8 * r.nt ? G : 8 * r.nt;
-    r.tq = single ? 1 : 8 * r.nt / r.gq;
+    r.several = T > R;
+    r.gq = G < 8 * most ? G : 8 * most;
+    r.n1 = r.gq <= 8 ? 1 : r.gq <= 16 ? 2 : 4;
+    r.tq = r.several ? 8 * most / r.gq : 1;
     r.hgroups = (G + r.gq - 1) / r.gq;
     return r;
 }
 
-template <int DK, int DV, bool BF16, int NT>
-cudaError_t launch_nt(const AttendParams &p, const RowShape &r, int serve, cudaStream_t s) {
-    const size_t smem = sizeof(Shared<DK, DV, NT>);
-    auto kernel = attend_kernel<DK, DV, BF16, NT>;
+template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
+cudaError_t launch_n1(const AttendParams &p, const RowShape &r, cudaStream_t s) {
+    const size_t smem = sizeof(Shared<DK, DV, SEVERAL ? most_columns(BF16) : N1>);
+    auto kernel = attend_kernel<DK, DV, BF16, N1, SEVERAL>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)(p.T / r.tq + p.R), (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
-                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups, serve);
+                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups);
 }
 
 template <int DK, int DV, bool BF16>
 cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
-    const int G = p.heads / p.c.heads;
-    const bool several = p.T > p.R;               // a request may have more than one token
-    cudaError_t e = cudaSuccess;
-    if (several) e = launch_nt<DK, DV, BF16, BF16 ? 4 : 2>(p, row_shape(false, G, p.dtype), kSeveral, s);
-    if (e != cudaSuccess) return e;
-    const RowShape r = row_shape(true, G, p.dtype);
-    const int serve = several ? kSingle : kAll;
-    if (r.nt == 1) e = launch_nt<DK, DV, BF16, 1>(p, r, serve, s);
-    else if (r.nt == 2) e = launch_nt<DK, DV, BF16, 2>(p, r, serve, s);
-    else e = launch_nt<DK, DV, BF16, BF16 ? 4 : 2>(p, r, serve, s);
+    const RowShape r = row_shape(p.T, p.R, p.heads / p.c.heads, p.dtype);
+    constexpr int kMost = most_columns(BF16);
+    cudaError_t e;
+    if (r.n1 == 1) e = r.several ? launch_n1<DK, DV, BF16, 1, true>(p, r, s) : launch_n1<DK, DV, BF16, 1, false>(p, r, s);
+    else if (r.n1 == 2) e = r.several ? launch_n1<DK, DV, BF16, 2, true>(p, r, s) : launch_n1<DK, DV, BF16, 2, false>(p, r, s);
+    else e = launch_n1<DK, DV, BF16, kMost, false>(p, r, s);
     if (e != cudaSuccess || p.splits == 1) return e;
     return launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)((p.T * p.heads + 7) / 8)), dim3(256), 0, s, p);
 }
@@ -628,8 +637,8 @@ int resident(int k_dim, int v_dim) {
 // its requests may be of any length.
 void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
                    int &chunk) {
-    const RowShape r = row_shape(T <= R, heads / c.heads, dtype);
-    const int64_t rows = T <= R ? R : (T + r.tq - 1) / r.tq > R ? (T + r.tq - 1) / r.tq : R;
+    const RowShape r = row_shape(T, R, heads / c.heads, dtype);
+    const int64_t rows = (T + r.tq - 1) / r.tq > R ? (T + r.tq - 1) / r.tq : R;
     const int64_t ctas = (rows < 1 ? 1 : rows) * c.heads * r.hgroups;
     const int64_t fill = (int64_t)device_sm_count() * resident(c.k_dim, c.v_dim);
     const int64_t tiles = max_kv < 1 ? 1 : (max_kv + 63) / 64;
