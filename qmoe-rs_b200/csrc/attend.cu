@@ -79,16 +79,20 @@ QMOE_DEV void mma_f16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
 // 32-bit word t of v (t a constant after unrolling).
 QMOE_DEV uint32_t word_of(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
 
-// The largest r in [0, R) with start[r] / tq + r <= slot.  Tiles of request r
-// take the slots from there on; start never falls, so neither does that.  A
-// warp looks at 32 places at a time.
+// The request whose tiles of tq tokens hold slot `slot`.  With one token a tile
+// the slots are the tokens: the last request that starts at or before it.  Else
+// the tiles of request r start at start[r] / tq + r, which leaves each request
+// room for a part of a tile more.  Both never fall with r; a warp looks at 32
+// places at a time.
+QMOE_DEV int64_t first_slot(const int32_t *start, int64_t r, int tq) { return tq == 1 ? start[r] : start[r] / tq + r; }
+
 QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int tq) {
     const int lane = threadIdx.x & 31;
     int64_t lo = 0, n = R;                       // the answer is in [lo, lo + n)
     while (n > 1) {
         const int64_t step = (n + 31) / 32;
         const int64_t i = lo + lane * step;
-        const bool le = lane == 0 || (i < lo + n && start[i] / tq + i <= slot);
+        const bool le = lane == 0 || (i < lo + n && first_slot(start, i, tq) <= slot);
         const int last = 31 - __clz(__ballot_sync(0xffffffffu, le));
         const int64_t at = lo + last * step;
         n = lo + n - at < step ? lo + n - at : step;
@@ -114,7 +118,7 @@ struct Rows {                                    // of one CTA: rows of one requ
 QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Rows &w) {
     const int64_t r = find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    const int64_t i0 = (slot - (s0 / tq + r)) * tq;
+    const int64_t i0 = (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
     w.t0 = s0 + i0;
@@ -536,7 +540,7 @@ __host__ __device__ constexpr int most_columns(bool bf16) { return bf16 ? 4 : 2;
 // on N1 * 8 columns) and several may meet in a batch; SEVERAL says whether they
 // can.
 template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p, int tq, int gq, int hgroups) {
+__global__ void __launch_bounds__(kThreads, 8 / kWarps) attend_kernel(const AttendParams p, int tq, int gq, int hgroups) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
@@ -553,34 +557,73 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
         attend_rows<DK, DV, BF16, N1>(p, w, h, blockIdx.z, gq, heads_here, smem_raw);
 }
 
-// Joins the pieces: one warp per (token, head).
+// Joins the pieces, one CTA per (token, head): thread s weighs piece s, the
+// warps share the pieces' sums out.
+constexpr int kJoinWarps = 4;
+constexpr int kMaxSplits = 256;
+
 template <int DV, bool BF16>
-__global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p) {
+    constexpr int kPer = DV / 32;
+    __shared__ float weight[kMaxSplits];
+    __shared__ float red[kJoinWarps], part_sum[kJoinWarps][DV];
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t t = w / p.heads;
-    if (t >= p.T || t >= p.q_start[p.R]) return;
-    const float *ml = p.ws + w * p.splits * 2;
-    const float *part = p.ws + p.T * p.heads * p.splits * 2 + w * p.splits * DV;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.x;
+    const int64_t t = row / p.heads;
+    if (t >= p.q_start[p.R]) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + row * p.splits;
+    const float *part = p.ws + p.T * p.heads * p.splits * 2 + row * p.splits * DV;
+    float2 v[kMaxSplits / (kJoinWarps * 32)];
     float m = neg_inf();
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
-    float l = 0.0f, o[DV / 32];
 #pragma unroll
-    for (int j = 0; j < DV / 32; ++j) o[j] = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = m == neg_inf() ? 1.0f : ex2(ml[2 * s] - m);
-        l = __fmaf_rn(ml[2 * s + 1], f, l);
-#pragma unroll
-        for (int j = 0; j < DV / 32; ++j) o[j] = __fmaf_rn(part[(int64_t)s * DV + 32 * j + lane], f, o[j]);
+    for (int k = 0; k < kMaxSplits / (kJoinWarps * 32); ++k) {
+        const int s = k * kJoinWarps * 32 + tid;
+        v[k] = s < p.splits ? ml[s] : make_float2(neg_inf(), 0.0f);
+        m = fmaxf(m, v[k].x);
     }
-    const int64_t at = t * p.ldo + (w - t * p.heads) * DV + lane;
+    m = warp_max(m);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < DV / 32; ++j) {
-        const float y = l == 0.0f ? 0.0f : __fdiv_rn(o[j], l);
-        if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.out)[at + 32 * j] = __float2bfloat16_rn(y);
-        else reinterpret_cast<float *>(p.out)[at + 32 * j] = y;
+    for (int k = 0; k < kJoinWarps; ++k) m = fmaxf(m, red[k]);
+    __syncthreads();
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMaxSplits / (kJoinWarps * 32); ++k) {
+        const int s = k * kJoinWarps * 32 + tid;
+        const float f = m == neg_inf() ? 1.0f : ex2(v[k].x - m);
+        if (s < p.splits) weight[s] = f;
+        l = __fmaf_rn(v[k].y, f, l);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) red[warp] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinWarps; ++k) l += red[k];
+    float o[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
+#pragma unroll 4
+    for (int s = warp; s < p.splits; s += kJoinWarps) {
+        const float f = weight[s];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) o[j] = __fmaf_rn(part[(int64_t)s * DV + 32 * j + lane], f, o[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) part_sum[warp][32 * j + lane] = o[j];
+    __syncthreads();
+    const int64_t at = t * p.ldo + (row - t * p.heads) * DV;
+    for (int d = tid; d < DV; d += kJoinWarps * 32) {
+        float y = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinWarps; ++k) y += part_sum[k][d];
+        y = l == 0.0f ? 0.0f : __fdiv_rn(y, l);
+        if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.out)[at + d] = __float2bfloat16_rn(y);
+        else reinterpret_cast<float *>(p.out)[at + d] = y;
     }
 }
 
@@ -606,7 +649,8 @@ cudaError_t launch_n1(const AttendParams &p, const RowShape &r, cudaStream_t s) 
     auto kernel = attend_kernel<DK, DV, BF16, N1, SEVERAL>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)(p.T / r.tq + p.R), (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
+    const int64_t slots = r.tq == 1 ? p.T : p.T / r.tq + p.R;
+    return launch_pdl(kernel, dim3((unsigned)slots, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
                       dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups);
 }
 
@@ -619,7 +663,8 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     else if (r.n1 == 2) e = r.several ? launch_n1<DK, DV, BF16, 2, true>(p, r, s) : launch_n1<DK, DV, BF16, 2, false>(p, r, s);
     else e = launch_n1<DK, DV, BF16, kMost, false>(p, r, s);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)((p.T * p.heads + 7) / 8)), dim3(256), 0, s, p);
+    return launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(p.T * p.heads)),
+                      dim3(kJoinWarps * 32), 0, s, p);
 }
 
 // CTAs of the single-token kernel that an SM holds.
@@ -627,7 +672,8 @@ int resident(int k_dim, int v_dim) {
     const size_t smem = k_dim == 64    ? sizeof(Shared<64, 64, 1>)
                         : k_dim == 128 ? sizeof(Shared<128, 128, 1>)
                                        : sizeof(Shared<192, 128, 1>);
-    return 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
+    const int most = 8 / kWarps, fit = (int)(228 * 1024 / (smem + 1024));
+    return fit < most ? fit : most;
 }
 
 }  // namespace
@@ -646,8 +692,8 @@ void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dty
     int64_t ch = (tiles + s - 1) / s;
     ch = ch < 2 * kWarps ? 2 * kWarps : (ch + kWarps - 1) / kWarps * kWarps;
     s = (tiles + ch - 1) / ch;
-    if (s > 256) {
-        s = 256;
+    if (s > kMaxSplits) {
+        s = kMaxSplits;
         ch = (tiles + s - 1) / s;
     }
     chunk = (int)ch;
