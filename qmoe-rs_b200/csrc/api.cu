@@ -2231,8 +2231,7 @@ int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t batch, int
     int8_t *codes = static_cast<int8_t *>(workspace);
     float *sx = reinterpret_cast<float *>(codes + batch * t->k_pad);
     CUtensorMap tm_x;
-    if (!make_tmap_u8(&tm_x, codes, (uint64_t)t->k_pad, (uint64_t)batch, 128, (uint32_t)int8_token_tile(batch),
-                      CU_TENSOR_MAP_SWIZZLE_128B))
+    if (!make_tmap_u8(&tm_x, codes, (uint64_t)t->k_pad, (uint64_t)batch, 128, (uint32_t)int8_token_tile(batch, t->out_f, (int)t->in_f), CU_TENSOR_MAP_SWIZZLE_128B))
         return fail(QMOE_ERR_CUDA, "tensor map encoding failed");
     Int8RowsParams q{x, dtype, batch, row_stride, (int)t->in_f, (int)t->k_pad, codes, sx};
     QTRY_CUDA(launch_quant_rows(q, st));

@@ -18,51 +18,101 @@ using namespace sm100;
 
 // ---- rows to codes ---------------------------------------------------------
 
-constexpr int kRowThreads = 256;
-
 template <bool BF16>
 QMOE_DEV float load1(const void *x, int64_t i) {
     return BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(x)[i])
                 : reinterpret_cast<const float *>(x)[i];
 }
 
-// One CTA per row: its largest magnitude, then its codes (the row comes from
-// L1 / L2 the second time).
+// Eight elements from a 16-byte aligned address.
 template <bool BF16>
-__global__ void __launch_bounds__(kRowThreads)
+QMOE_DEV void load8(const void *x, int64_t i, float (&v)[8]) {
+    const float4 a = load_act4(x, BF16 ? 1 : 0, i), b = load_act4(x, BF16 ? 1 : 0, i + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// THREADS per row, each 8 * GROUPS elements of it in registers (GROUPS 0: any
+// length or alignment, read twice).  A row is one load latency and one
+// reduction, so short rows share a CTA (a warp each) and long ones take 1024
+// threads: 4096 rows of 7168 bf16 are read once and written once.
+template <bool BF16, int THREADS, int GROUPS>
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS)
 quant_rows_kernel(const Int8RowsParams p) {
-    __shared__ float wmax[kRowThreads / 32];
-    __shared__ int wbad[kRowThreads / 32];
+    constexpr int kRows = THREADS < 128 ? 128 / THREADS : 1;
+    constexpr int kW = THREADS / 32;              // warps of a row
+    __shared__ float wmax[kW];
+    __shared__ int wbad[kW];
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
-    const int64_t t = blockIdx.x;
+    const int tid = threadIdx.x % THREADS;
+    const int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
+    if (t >= p.T) return;                         // kRows > 1: whole warps, no CTA barrier follows
     const int64_t base = t * p.ldx;
-    const int tid = threadIdx.x;
+    float v[GROUPS ? GROUPS : 1][8];
     float m = 0.0f;
     bool bad = false;
-    for (int k = tid; k < p.K; k += kRowThreads) {
-        const float v = load1<BF16>(p.x, base + k);
-        m = max_abs(m, v);
-        bad |= !(fabsf(v) < __int_as_float(0x7f800000));
+    if constexpr (GROUPS > 0) {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+            const int k = (q * THREADS + tid) * 8;
+            if (k < p.K) {
+                load8<BF16>(p.x, base + k, v[q]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[q][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                m = max_abs(m, v[q][j]);
+                bad |= !(fabsf(v[q][j]) < __int_as_float(0x7f800000));
+            }
+    } else {
+        for (int k = tid; k < p.K; k += THREADS) {
+            const float x = load1<BF16>(p.x, base + k);
+            m = max_abs(m, x);
+            bad |= !(fabsf(x) < __int_as_float(0x7f800000));
+        }
     }
     m = warp_max(m);
     bad = __any_sync(0xffffffffu, bad);
-    if ((tid & 31) == 0) {
-        wmax[tid >> 5] = m;
-        wbad[tid >> 5] = bad;
+    if constexpr (kW > 1) {
+        if ((tid & 31) == 0) {
+            wmax[tid >> 5] = m;
+            wbad[tid >> 5] = bad;
+        }
+        __syncthreads();
+        const int i = tid & 31;
+        m = warp_max(i < kW ? wmax[i] : 0.0f);
+        bad = __any_sync(0xffffffffu, i < kW && wbad[i]);
     }
-    __syncthreads();
-    int any = 0;
-#pragma unroll
-    for (int w = 0; w < kRowThreads / 32; ++w) {
-        m = fmaxf(m, wmax[w]);
-        any |= wbad[w];
-    }
-    const float r = range8(m, !any), mi = __fdiv_rn(127.0f, r);
+    const float r = range8(m, !bad), mi = __fdiv_rn(127.0f, r);
     int8_t *o = p.codes + t * p.ldc;
-    for (int k = tid; k < p.ldc; k += kRowThreads)
-        o[k] = (int8_t)(k < p.K ? code8(load1<BF16>(p.x, base + k), 127.0f, r, mi) : 0);
+    if constexpr (GROUPS > 0) {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+            const int k = (q * THREADS + tid) * 8;
+            if (k >= p.ldc) continue;
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = code8(v[q][j], 127.0f, r, mi);
+            *reinterpret_cast<uint2 *>(o + k) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+        }
+    } else {
+        for (int k = tid; k < p.ldc; k += THREADS)
+            o[k] = (int8_t)(k < p.K ? code8(load1<BF16>(p.x, base + k), 127.0f, r, mi) : 0);
+    }
     if (tid == 0) p.scales[t] = __fdiv_rn(r, 127.0f);
+}
+
+template <int THREADS, int GROUPS>
+cudaError_t launch_rows(const Int8RowsParams &p, cudaStream_t s) {
+    constexpr int kRows = THREADS < 128 ? 128 / THREADS : 1;
+    return launch_pdl(p.dtype ? quant_rows_kernel<true, THREADS, GROUPS> : quant_rows_kernel<false, THREADS, GROUPS>,
+                      dim3((unsigned)((p.T + kRows - 1) / kRows)), dim3(THREADS < 128 ? 128 : THREADS), 0, s, p);
 }
 
 // ---- the product -------------------------------------------------------------
@@ -73,19 +123,31 @@ quant_rows_kernel(const Int8RowsParams p) {
 // TMA in 128-byte K blocks (128-byte swizzle), rows and K past the end filled
 // with zeros, and the accumulator is double-buffered in tensor memory.
 //
-// Persistent grid, eight warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner,
-// 4-7 epilogue (one TMEM lane quarter each).  Every wait is bounded; on a
-// time-out the kernel flags the device error word, drains its copies and MMAs
-// (again bounded), frees TMEM and returns.
+// Eight warps: 0 TMA producer, 1 MMA issuer, 2 TMEM owner, 4-7 epilogue (one
+// TMEM lane quarter each).  With tiles enough for the device the grid is
+// persistent and a tile's epilogue runs under the next one's MMAs.  With fewer,
+// a cluster of CTAs takes the K blocks of one tile in parts: each leaves its
+// 32-bit sums in its shared memory, and after a cluster barrier each adds its
+// share of the tokens from all of them (integers, so the parts' order does not
+// matter).  The first weight blocks are asked for before the row quantiser in
+// front has finished.
+//
+// Every wait is bounded; on a time-out the kernel flags the device error word,
+// drains its copies and MMAs (again bounded), frees TMEM and returns.
 
 constexpr int kThreads = 256;
 constexpr int kABytes = 128 * 128;
 
+// Up to 64 tokens two CTAs share an SM, so that one streams while the other
+// starts or ends.
 template <int BN>
 struct Tile {
     static constexpr int stage = kABytes + BN * 128;
-    static constexpr int stages = 200 * 1024 / stage > 8 ? 8 : 200 * 1024 / stage;
+    static constexpr int stages = (BN <= 64 ? 100 : 200) * 1024 / stage;
+    static constexpr int ctas = BN <= 64 ? 2 : 1;
     static constexpr uint32_t cols = 2 * BN < 32 ? 32 : 2 * BN;
+    static_assert(stages * stage >= BN * 512, "the sums of a tile do not fit the ring");
+    static_assert(ctas * cols <= 512, "tensor memory");
 };
 
 constexpr int kMaxStages = 8;
@@ -95,6 +157,7 @@ struct Smem {
     uint64_t dfull[2], dempty[2], drain;
     uint32_t tmem_base;
     int abort;
+    float sx[4][256];                             // each epilogue warp's copy of a tile's token scales
 };
 
 QMOE_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -105,20 +168,45 @@ QMOE_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint3
         : "memory");
 }
 
+template <bool BF16>
+QMOE_DEV void finish(const Int8GemmParams &p, int64_t t, int n, int sum, float sx, float sw, float res) {
+    const int64_t at = t * p.N + n;
+    float y = __fmul_rn(__fmul_rn((float)sum, sx), sw);
+    if (p.residual) y = __fadd_rn(y, res);
+    if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(y);
+    else reinterpret_cast<float *>(p.y)[at] = y;
+}
+
+QMOE_DEV void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The int at this CTA's shared address, in CTA `rank` of the cluster.
+QMOE_DEV int load_cluster(const int *at, int rank) {
+    uint32_t remote;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+    return v;
+}
+
 template <int BN, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Tile<BN>::ctas)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                 const Int8GemmParams p) {
+                 const Int8GemmParams p, const int parts) {
     using Cfg = Tile<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Smem *S = reinterpret_cast<Smem *>(ring + Cfg::stages * Cfg::stage);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int tiles_t = (int)((p.T + BN - 1) / BN), tiles_n = (int)((p.N + 127) / 128);
-    const int total = tiles_t * tiles_n;            // at least the grid
+    const int total = tiles_t * tiles_n;
     const int nkb = (p.K + 127) / 128;
+    // the tiles of this CTA (parts > 1: one), and its K blocks of them
+    const int rank = parts > 1 ? blockIdx.x % parts : 0;
+    const int tile0 = parts > 1 ? blockIdx.x / parts : blockIdx.x, step = parts > 1 ? total : gridDim.x;
+    const int kb0 = nkb * rank / parts, kb1 = nkb * (rank + 1) / parts;
 
     if (tid == 0) {
         for (int i = 0; i < Cfg::stages; ++i) {
@@ -145,15 +233,25 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t u = 0;
+            uint32_t u = 0, early = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
+            {   // weights of the first blocks: nothing in front of this kernel writes them
+                const int n0 = (tile0 / tiles_t) * 128;
+                for (; (int)early < kb1 - kb0 && early < Cfg::stages; ++early) {
+                    mbar_arrive_expect_tx(&S->full[early], Cfg::stage);
+                    tma_load_2d(ring + early * Cfg::stage, &tm_w, &S->full[early], (kb0 + (int)early) * 128, n0);
+                }
+            }
+            QMOE_PDL_WAIT();
+            for (int tile = tile0; ok && tile < total; tile += step) {
                 const int t0 = (tile % tiles_t) * BN, n0 = (tile / tiles_t) * 128;
-                for (int kb = 0; kb < nkb; ++kb, ++u) {
+                for (int kb = kb0; kb < kb1; ++kb, ++u) {
                     const uint32_t s = u % Cfg::stages;
-                    if (!(ok = mbar_wait(&S->empty[s], ((u / Cfg::stages) & 1) ^ 1, abort, p.err))) break;
-                    mbar_arrive_expect_tx(&S->full[s], Cfg::stage);
-                    tma_load_2d(ring + s * Cfg::stage, &tm_w, &S->full[s], kb * 128, n0);
+                    if (u >= early) {
+                        if (!(ok = mbar_wait(&S->empty[s], ((u / Cfg::stages) & 1) ^ 1, abort, p.err))) break;
+                        mbar_arrive_expect_tx(&S->full[s], Cfg::stage);
+                        tma_load_2d(ring + s * Cfg::stage, &tm_w, &S->full[s], kb * 128, n0);
+                    }
                     tma_load_2d(ring + s * Cfg::stage + kABytes, &tm_x, &S->full[s], kb * 128, t0);
                 }
             }
@@ -162,25 +260,27 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
                     for (uint32_t n = 0; n < kMaxWaitProbes; ++n)
                         if (mbar_try_wait(&S->full[v % Cfg::stages], (v / Cfg::stages) & 1)) break;
         }
+        __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
             uint32_t u = 0, i = 0;
             bool ok = true, issued = false;
             const uint64_t d0 = smem_desc(smem_u32(ring), 16, 1024, 2);
-            for (int tile = blockIdx.x; ok && tile < total; tile += gridDim.x, ++i) {
+            for (int tile = tile0; ok && tile < total; tile += step, ++i) {
                 const int64_t left = p.T - (int64_t)(tile % tiles_t) * BN;
                 const int N = left >= BN ? BN : (int)(left + 15) / 16 * 16;
                 const uint32_t idesc = idesc_i8(128, N, true, true);
                 const uint32_t d = tmem + (i & 1) * BN;
                 if (!(ok = mbar_wait(&S->dempty[i & 1], ((i >> 1) & 1) ^ 1, abort, p.err))) break;
                 tc_fence_after();
-                for (int kb = 0; kb < nkb; ++kb, ++u) {
+                for (int kb = kb0; kb < kb1; ++kb, ++u) {
                     const uint32_t s = u % Cfg::stages;
                     if (!(ok = mbar_wait(&S->full[s], (u / Cfg::stages) & 1, abort, p.err))) break;
                     tc_fence_after();
                     const uint64_t a = d0 + ((s * Cfg::stage) >> 4), b = a + (kABytes >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) mma_i8_ss(d, a + 2 * kk, b + 2 * kk, idesc, (kb | kk) != 0);
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_i8_ss(d, a + 2 * kk, b + 2 * kk, idesc, (kb != kb0) | (kk != 0));
                     issued = true;
                     mma_commit(&S->empty[s]);
                 }
@@ -194,20 +294,38 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
                     if (mbar_try_wait(&S->drain, 0)) break;
             }
         }
+        __syncwarp();
     } else if (warp >= 4) {
         constexpr int CH = BN < 32 ? 16 : 32;
         const int q = warp & 3;
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
         uint32_t i = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < total; tile += gridDim.x, ++i) {
+        QMOE_PDL_WAIT();
+        for (int tile = tile0; ok && tile < total; tile += step, ++i) {
             const int64_t t0 = (int64_t)(tile % tiles_t) * BN;
             const int n = (tile / tiles_t) * 128 + q * 32 + lane;
-            const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
             const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
+            const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
+            float *sx = S->sx[q];
+            __syncwarp();
+            for (int j = lane; j < count; j += 32) sx[j] = p.sx[t0 + j];
+            __syncwarp();
             if (!(ok = mbar_wait_warp(&S->dfull[i & 1], (i >> 1) & 1, abort, p.err))) break;
             tc_fence_after();
+            // rolled: a tile's code stays small beside the other warps'
+#pragma unroll 1
             for (int c = 0; c < count; c += CH) {
+                float res[CH];
+                if (parts == 1 && p.residual) {   // all in flight at once; rows and channels past the end read the last
+                    const int64_t nn = n < p.N ? n : p.N - 1;
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        res[j] = load1<BF16>(p.residual, (t0 + (c + j < count ? c + j : count - 1)) * p.N + nn);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) res[j] = 0.0f;
+                }
                 uint32_t v[CH];
                 if constexpr (CH == 32) tmem_ld_x32(tmem + lane_addr + (i & 1) * BN + c, v);
                 else tmem_ld_x16(tmem + lane_addr + (i & 1) * BN + c, v);
@@ -217,14 +335,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S->dempty[i & 1]);
                 }
+                if (parts > 1) {                  // every MMA has read its operands: the ring is free
+                    int *sums = reinterpret_cast<int *>(ring);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) {
-                    if (c + j >= count || n >= p.N) continue;
-                    const int64_t t = t0 + c + j, at = t * p.N + n;
-                    float y = __fmul_rn(__fmul_rn((float)(int)v[j], __ldg(p.sx + t)), sw);
-                    if (p.residual) y = __fadd_rn(y, load1<BF16>(p.residual, at));
-                    if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(y);
-                    else reinterpret_cast<float *>(p.y)[at] = y;
+                    for (int j = 0; j < CH; ++j) sums[(c + j) * 128 + q * 32 + lane] = (int)v[j];
+                } else if (n < p.N) {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (c + j < count) finish<BF16>(p, t0 + c + j, n, (int)v[j], sx[c + j], sw, res[j]);
                 }
                 __syncwarp();
             }
@@ -236,39 +354,100 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::cols);
+        __syncwarp();
+    }
+    if (parts > 1) {
+        QMOE_PDL_WAIT();
+        cluster_barrier();
+        const int64_t t0 = (int64_t)(tile0 % tiles_t) * BN;
+        const int n = (tile0 / tiles_t) * 128 + (tid & 127);
+        const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
+        const int *sums = reinterpret_cast<const int *>(ring);
+        const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
+        for (int j = rank + parts * (tid >> 7); j < count; j += 2 * parts) {
+            int sum = 0;
+            for (int r = 0; r < parts; ++r) sum += load_cluster(sums + j * 128 + (tid & 127), r);
+            if (n < p.N)
+                finish<BF16>(p, t0 + j, n, sum, p.sx[t0 + j], sw,
+                             p.residual ? load1<BF16>(p.residual, (t0 + j) * p.N + n) : 0.0f);
+        }
+        cluster_barrier();                        // the others may still read this CTA's sums
     }
 }
 
+// How a product is cut.  Up to 64 tokens one tile holds them all (the weights
+// are read once); above, the widest tile of 256, 128 or 64 tokens that gives
+// every SM one.  Where the tiles are still too few, clusters of up to 8 CTAs
+// share a tile's K, with two K blocks each at least.
+struct Cut {
+    int bn, parts;
+};
+Cut cut_of(int64_t T, int64_t N, int K) {
+    const int64_t sms = device_sm_count(), tn = (N + 127) / 128, nkb = (K + 127) / 128;
+    Cut c;
+    c.bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    while (T > 64 && c.bn > 64 && tn * ((T + c.bn - 1) / c.bn) < sms) c.bn /= 2;
+    const int64_t tiles = tn * ((T + c.bn - 1) / c.bn), room = sms * (c.bn <= 64 ? 2 : 1);
+    int64_t parts = room / tiles;
+    if (parts > nkb / 2) parts = nkb / 2;
+    c.parts = parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
+    return c;
+}
+
 template <int BN>
-cudaError_t launch_bn(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const Int8GemmParams &p, cudaStream_t s) {
+cudaError_t launch_bn(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const Int8GemmParams &p, int parts,
+                      cudaStream_t s) {
     using Cfg = Tile<BN>;
     const size_t smem = 1024 + (size_t)Cfg::stages * Cfg::stage + sizeof(Smem);
     auto kernel = p.dtype ? int8_gemm_kernel<BN, true> : int8_gemm_kernel<BN, false>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    const int64_t total = ((p.T + BN - 1) / BN) * ((p.N + 127) / 128);
-    const int64_t sms = device_sm_count();
-    return launch_pdl(kernel, dim3((unsigned)(total < sms ? total : sms)), dim3(kThreads), smem, s, tm_w, tm_x, p);
+    const int64_t total = ((p.T + BN - 1) / BN) * ((p.N + 127) / 128), room = (int64_t)device_sm_count() * Cfg::ctas;
+    const int64_t grid = parts > 1 ? total * parts : total < room ? total : room;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)parts;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_x, p, parts);
 }
 
 }  // namespace
 
-int int8_token_tile(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256; }
+int int8_token_tile(int64_t T, int64_t N, int K) { return cut_of(T, N, K).bn; }
 
 cudaError_t launch_quant_rows(const Int8RowsParams &p, cudaStream_t s) {
     if (p.T == 0) return cudaSuccess;
-    return launch_pdl(p.dtype ? quant_rows_kernel<true> : quant_rows_kernel<false>, dim3((unsigned)p.T),
-                      dim3(kRowThreads), 0, s, p);
+    // whole groups of eight elements and codes, aligned
+    const uintptr_t es = p.dtype ? 2 : 4;
+    const bool vec = p.K % 8 == 0 && p.ldc % 8 == 0 && p.ldx % (16 / es) == 0 &&
+                     reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.codes) % 8 == 0;
+    if (!vec) return p.ldc <= 1024 ? launch_rows<32, 0>(p, s) : launch_rows<256, 0>(p, s);
+    if (p.ldc <= 512) return launch_rows<32, 2>(p, s);
+    if (p.ldc <= 2048) return launch_rows<128, 2>(p, s);
+    if (p.ldc <= 8192) return launch_rows<512, 2>(p, s);
+    if (p.ldc <= 16384) return launch_rows<1024, 2>(p, s);
+    return launch_rows<1024, 0>(p, s);
 }
 
 cudaError_t launch_int8_gemm(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const Int8GemmParams &p,
                              cudaStream_t s) {
-    switch (int8_token_tile(p.T)) {
-        case 16: return launch_bn<16>(tm_w, tm_x, p, s);
-        case 32: return launch_bn<32>(tm_w, tm_x, p, s);
-        case 64: return launch_bn<64>(tm_w, tm_x, p, s);
-        case 128: return launch_bn<128>(tm_w, tm_x, p, s);
-        default: return launch_bn<256>(tm_w, tm_x, p, s);
+    const Cut c = cut_of(p.T, p.N, p.K);
+    switch (c.bn) {
+        case 16: return launch_bn<16>(tm_w, tm_x, p, c.parts, s);
+        case 32: return launch_bn<32>(tm_w, tm_x, p, c.parts, s);
+        case 64: return launch_bn<64>(tm_w, tm_x, p, c.parts, s);
+        case 128: return launch_bn<128>(tm_w, tm_x, p, c.parts, s);
+        default: return launch_bn<256>(tm_w, tm_x, p, c.parts, s);
     }
 }
 

@@ -368,8 +368,8 @@ struct Int8GemmParams {
     int *err;               // device error word
 };
 cudaError_t launch_quant_rows(const Int8RowsParams &p, cudaStream_t s);
-// Rows of the activation map's box for T tokens.
-int int8_token_tile(int64_t T);
+// Rows of the activation map's box.
+int int8_token_tile(int64_t T, int64_t N, int K);
 cudaError_t launch_int8_gemm(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const Int8GemmParams &p,
                              cudaStream_t s);
 
