@@ -2354,6 +2354,7 @@ int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int
     DeviceGuard g(ctx->device);
     attend_pieces(p.c, T, requests, heads, dtype, max_kv, p.splits, p.chunk);
     p.vec_q = reinterpret_cast<uintptr_t>(q) % (4 * dtype_size(dtype)) == 0 && q_stride % 4 == 0;
+    p.vec_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_stride % 8 == 0;
     p.err = error_flag();
     const int64_t need = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, p.c.v_dim, p.splits));
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))

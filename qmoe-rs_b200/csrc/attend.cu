@@ -24,50 +24,16 @@
 // 16 ((r % 8) / 2) + 4 u + 2 (r / 8) + r % 2: transposed eight by eight
 // (movmatrix), the scores' fragments are then P^T's for those bytes of V, and a
 // lane's scores all lie in one group of 16 tokens, hence in one block.
-#include "code8.cuh"
+#include "attend.cuh"
 #include "kernels.h"
 #include "sm100.cuh"
-
-#include <cuda_fp16.h>
 
 namespace qmoe {
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kPShift = 14.0f;              // P up to 2^14: fp16 keeps 2^-38 of the largest
-
-QMOE_DEV float neg_inf() { return __int_as_float(0xff800000); }
-
-QMOE_DEV float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-QMOE_DEV uint32_t h2(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-
-QMOE_DEV float h_lo(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xffff))); }
-QMOE_DEV float h_hi(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
-
-// Four codes -> two fp16 pairs: 0x6400 | (c + 128) is 1152 + c, exactly.
-QMOE_DEV void codes_to_half(uint32_t v, uint32_t &lo, uint32_t &hi) {
-    v ^= 0x80808080u;
-    const uint32_t a = __byte_perm(v, 0x64646464u, 0x4140), b = __byte_perm(v, 0x64646464u, 0x4342);
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
-}
-
-// Four codes as 1152 + c.
-QMOE_DEV void codes_biased(uint32_t v, uint32_t &lo, uint32_t &hi) {
-    v ^= 0x80808080u;
-    lo = __byte_perm(v, 0x64646464u, 0x4140);
-    hi = __byte_perm(v, 0x64646464u, 0x4342);
-}
 
 QMOE_DEV void mma_f16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm(
@@ -101,12 +67,6 @@ QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int
     return lo;
 }
 
-// tok / block for a multiple of 16: per_block = ceil(2^36 / (block / 16)); exact
-// below 2^31, since the error of the product is below 2^27 * 16 < 2^36 / 16.
-QMOE_DEV int block_index(const AttendParams &p, int tok) {
-    return (int)(((uint64_t)(uint32_t)(tok >> 4) * p.per_block) >> 36);
-}
-
 struct Rows {                                    // of one CTA: rows of one request and kv head
     int64_t t0;                                  // token of row 0
     int tokens, head0;                           // row i * gq + g: token t0 + i, head head0 + g
@@ -115,10 +75,12 @@ struct Rows {                                    // of one CTA: rows of one requ
     int64_t request;
 };
 
-QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Rows &w) {
-    const int64_t r = find_request(p.q_start, p.R, slot, tq);
+// by_request: slot r is request r, if it has up to tq tokens.
+QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, bool by_request, Rows &w) {
+    const int64_t r = by_request ? slot : find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    const int64_t i0 = (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
+    if (by_request && n > tq) return false;
+    const int64_t i0 = by_request ? 0 : (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
     w.t0 = s0 + i0;
@@ -244,12 +206,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         for (int J = 0; J < DK / 64; ++J)
 #pragma unroll
             for (int d = 0; d < 16; d += 4) {
-                const float4 f = !live ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                       : p.vec_q ? load_act4(p.q, p.dtype, at + 64 * J + d)
-                                                 : make_float4(load_act(p.q, p.dtype, at + 64 * J + d),
-                                                               load_act(p.q, p.dtype, at + 64 * J + d + 1),
-                                                               load_act(p.q, p.dtype, at + 64 * J + d + 2),
-                                                               load_act(p.q, p.dtype, at + 64 * J + d + 3));
+                const float4 f = live ? load_q4(p, at + 64 * J + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 v[J][d] = f.x;
                 v[J][d + 1] = f.y;
                 v[J][d + 2] = f.z;
@@ -258,8 +215,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
             }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        const int e = q_exponent(m);
         const float up = pow2i(14 - e);
         float sum = 0.0f;
 #pragma unroll
@@ -540,14 +496,14 @@ __host__ __device__ constexpr int most_columns(bool bf16) { return bf16 ? 4 : 2;
 // on N1 * 8 columns) and several may meet in a batch; SEVERAL says whether they
 // can.
 template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
-__global__ void __launch_bounds__(kThreads, 8 / kWarps) attend_kernel(const AttendParams p, int tq, int gq, int hgroups) {
+__global__ void __launch_bounds__(kThreads, 8 / kWarps) attend_kernel(const AttendParams p, int tq, int gq, int hgroups, bool by_request) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups;
     const int G = p.heads / p.c.heads;
     Rows w;
-    if (!find_rows(p, blockIdx.x, tq, w)) return;                // the whole CTA alike
+    if (!find_rows(p, blockIdx.x, tq, by_request, w)) return;                // the whole CTA alike
     w.head0 = h * G + hg * gq;
     const int heads_here = G - hg * gq < gq ? G - hg * gq : gq;
     constexpr int kMost = most_columns(BF16);
@@ -563,16 +519,25 @@ constexpr int kJoinWarps = 4;
 constexpr int kMaxSplits = 256;
 
 template <int DV, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p, int tq,
+                                                                       bool by_request) {
     constexpr int kPer = DV / 32;
     __shared__ float weight[kMaxSplits];
     __shared__ float red[kJoinWarps], part_sum[kJoinWarps][DV];
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x;
-    const int64_t t = row / p.heads;
-    if (t >= p.q_start[p.R]) return;
+    // the tokens of request blockIdx.x, or token blockIdx.x
+    int64_t t = blockIdx.x, t_hi = t + 1;
+    if (by_request) {
+        t = p.q_start[blockIdx.x];
+        t_hi = p.q_start[blockIdx.x + 1];
+        if (t_hi - t > tq || t < 0) return;
+    }
+    const int64_t rows = p.q_start[p.R] < p.T ? p.q_start[p.R] : p.T;
+    t_hi = t_hi < rows ? t_hi : rows;
+    for (; t < t_hi; ++t) {
+    const int64_t row = t * p.heads + blockIdx.y;
     const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + row * p.splits;
     const float *part = p.ws + p.T * p.heads * p.splits * 2 + row * p.splits * DV;
     float2 v[kMaxSplits / (kJoinWarps * 32)];
@@ -616,7 +581,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
     for (int j = 0; j < kPer; ++j) part_sum[warp][32 * j + lane] = o[j];
     __syncthreads();
-    const int64_t at = t * p.ldo + (row - t * p.heads) * DV;
+    const int64_t at = t * p.ldo + (int64_t)blockIdx.y * DV;
     for (int d = tid; d < DV; d += kJoinWarps * 32) {
         float y = 0.0f;
 #pragma unroll
@@ -625,12 +590,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
         if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.out)[at + d] = __float2bfloat16_rn(y);
         else reinterpret_cast<float *>(p.out)[at + d] = y;
     }
+    __syncthreads();
+    }
 }
 
 struct RowShape {
     int n1;                                       // columns / 8 of a single token
     int gq, tq, hgroups;
     bool several;                                 // a request may have more than one token
+    bool by_request;                              // requests of more than tq tokens are the prompt kernel's
 };
 RowShape row_shape(int64_t T, int64_t R, int G, int dtype) {
     const int most = most_columns(dtype != 0);
@@ -640,6 +608,7 @@ RowShape row_shape(int64_t T, int64_t R, int G, int dtype) {
     r.n1 = r.gq <= 8 ? 1 : r.gq <= 16 ? 2 : 4;
     r.tq = r.several ? 8 * most / r.gq : 1;
     r.hgroups = (G + r.gq - 1) / r.gq;
+    r.by_request = r.several && dtype != 0;
     return r;
 }
 
@@ -649,9 +618,9 @@ cudaError_t launch_n1(const AttendParams &p, const RowShape &r, cudaStream_t s) 
     auto kernel = attend_kernel<DK, DV, BF16, N1, SEVERAL>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    const int64_t slots = r.tq == 1 ? p.T : p.T / r.tq + p.R;
+    const int64_t slots = r.by_request ? p.R : r.tq == 1 ? p.T : p.T / r.tq + p.R;
     return launch_pdl(kernel, dim3((unsigned)slots, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
-                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups);
+                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups, r.by_request);
 }
 
 template <int DK, int DV, bool BF16>
@@ -662,9 +631,11 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     if (r.n1 == 1) e = r.several ? launch_n1<DK, DV, BF16, 1, true>(p, r, s) : launch_n1<DK, DV, BF16, 1, false>(p, r, s);
     else if (r.n1 == 2) e = r.several ? launch_n1<DK, DV, BF16, 2, true>(p, r, s) : launch_n1<DK, DV, BF16, 2, false>(p, r, s);
     else e = launch_n1<DK, DV, BF16, kMost, false>(p, r, s);
-    if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(p.T * p.heads)),
-                      dim3(kJoinWarps * 32), 0, s, p);
+    if (e == cudaSuccess && p.splits > 1)
+        e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(r.by_request ? p.R : p.T), (unsigned)p.heads),
+                       dim3(kJoinWarps * 32), 0, s, p, r.tq, r.by_request);
+    if (e == cudaSuccess && r.by_request) e = launch_attend_prompt(p, r.tq, s);
+    return e;
 }
 
 // CTAs of the single-token kernel that an SM holds.
@@ -684,7 +655,7 @@ int resident(int k_dim, int v_dim) {
 void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
                    int &chunk) {
     const RowShape r = row_shape(T, R, heads / c.heads, dtype);
-    const int64_t rows = (T + r.tq - 1) / r.tq > R ? (T + r.tq - 1) / r.tq : R;
+    const int64_t rows = r.by_request || (T + r.tq - 1) / r.tq < R ? R : (T + r.tq - 1) / r.tq;
     const int64_t ctas = (rows < 1 ? 1 : rows) * c.heads * r.hgroups;
     const int64_t fill = (int64_t)device_sm_count() * resident(c.k_dim, c.v_dim);
     const int64_t tiles = max_kv < 1 ? 1 : (max_kv + 63) / 64;

@@ -407,6 +407,7 @@ struct AttendParams {
     const void *q;          // [T, heads, k_dim], tokens ldq apart
     int dtype;
     bool vec_q;             // four elements may be loaded at once
+    bool vec_out;           // eight bf16 may be stored at once
     int64_t T, ldq;
     int heads;              // query heads
     const int32_t *q_start, *kv_lens, *table;   // [R + 1], [R], [R, max_blocks]
@@ -427,5 +428,7 @@ void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dty
                    int &chunk);
 size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits);
 cudaError_t launch_attend(const AttendParams &p, cudaStream_t s);
+// The requests of more than `few` tokens (bf16), after launch_attend's own.
+cudaError_t launch_attend_prompt(const AttendParams &p, int few, cudaStream_t s);
 
 }  // namespace qmoe

@@ -109,6 +109,27 @@ def attend(q, kf, kr, vf, vr, q_start, kv_lens, table, bs, scale, out):
     return out
 
 
+def attend_dense(q, kf, kr, vf, vr, q_start, kv_lens, table, bs, scale, out):
+    """attend() for tables without holes, a request and head at a time."""
+    heads, H = q.shape[1], kf.shape[1]
+    for r, kv in enumerate(kv_lens):
+        a, b = q_start[r], q_start[r + 1]
+        if a == b:
+            continue
+        if kv == 0:
+            out[a:b] = 0.0
+            continue
+        pages = torch.tensor(table[r][:-(-kv // bs)])
+        hidden = torch.arange(kv)[None] > torch.arange(kv - (b - a), kv)[:, None]
+        for h in range(heads):
+            kh = h // (heads // H)
+            k = (kf[pages, kh].to(D) * (kr[pages, kh].to(D) / 127.0)[:, None, None]).flatten(0, 1)[:kv]
+            v = (vf[pages, kh].to(D) * (vr[pages, kh].to(D) / 127.0)[:, None, None]).flatten(0, 1)[:kv]
+            s = (q[a:b, h].to(D) @ k.T * scale).masked_fill(hidden, -math.inf)
+            out[a:b, h] = torch.softmax(s, 1) @ v
+    return out
+
+
 def attend_bound(dtype):
     """Largest |error| of an attention output relative to the largest |v| of its head.
 

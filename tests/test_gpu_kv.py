@@ -231,6 +231,27 @@ def test_attend(dtype, lens, shape):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(16, 1, 1, 64, 64), (48, 1, 2, 192, 128), (32, 1, 7, 128, 128), (128, 2, 2, 128, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("lens", [[(257, 257), (1, 1), (130, 129)], [(900, 300), (0, 40), (64, 64), (333, 33)],
+                                  [(1, 1)] * 40 + [(600, 70)] + [(20, 20)] * 9])
+def test_attend_prompts(dtype, shape, lens):
+    """Prompts and chunks over several tiles of keys and rows, single tokens between them."""
+    bs, H, G, dk, dv = shape
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, lens, 5, pad=3, spread=1.5)
+    q[starts[-1]:] = float("nan")
+    scale = ref.new_scale(dk)
+    out = torch.full((q.shape[0], H * G, dv), 0.25, dtype=q.dtype, device="cuda")
+    got = cache.attend(q.cuda(), i32(starts), i32(kv), i32([x for r in table for x in r], len(table), len(table[0])), out=out)
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, scale, torch.full(out.shape, 0.25, dtype=torch.float64))
+    check_attend(got, want, flat[3], dtype)
+    assert (got[starts[-1]:] == 0.25).all()
+    for _ in range(2):
+        assert torch.equal(cache.attend(q.cuda(), i32(starts), i32(kv), i32([x for r in table for x in r], len(table),
+                                                                           len(table[0])), out=out.clone()), got)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_bad_pages_views_and_empty_blocks(dtype):
     bs, H, G, dk, dv = 16, 2, 4, 128, 128
     cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, [(100, 1), (40, 9), (7, 1)], 8, holes=True)
