@@ -34,7 +34,11 @@ using namespace sm100;
 constexpr int kSoftWarps = 8;
 constexpr int kCodeWarp0 = 8, kCodeWarps = 4;
 constexpr int kMmaWarp = 12;
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;             // warps 13-15 only give their registers up
+// Registers a thread: the softmax holds a row's scores of a tile.  Of the 128 a
+// thread that the CTA is launched with, 2 * 168 + 112 + 64 = 4 * 128.
+constexpr int kSoftRegs = 168, kCodeRegs = 112, kMmaRegs = 64;
+static_assert(2 * kSoftRegs + kCodeRegs + kMmaRegs <= 512, "registers of the CTA");
 constexpr float kGrow = 8.0f;                 // log2 of how far a maximum may outgrow the scaling
 constexpr float kShift = 6.0f;                // P = 2^6 at the scaling's maximum
 constexpr int kScaleRing = 4;                 // tiles whose scales are kept: the codes run at most
@@ -60,17 +64,24 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-QMOE_DEV void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem]^T; a descriptor's halves apart, so that a step
+// is one 32-bit addition.
+QMOE_DEV void mma_f16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                         uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "{\n .reg .pred p;\n .reg .b64 ad, bd;\n setp.ne.b32 p, %5, 0;\n mov.b64 ad, {%1, %3};\n mov.b64 bd, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, {%6, %6, %6, %6}, p;\n}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T.
-QMOE_DEV void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    mma_bf16_ts(d_tmem, a_tmem, b_desc, idesc, accumulate);   // kind::f16; idesc says which type
+template <int N>
+QMOE_DEV void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+QMOE_DEV void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 QMOE_DEV uint4 ldg_code(const int8_t *at) { return __ldg(reinterpret_cast<const uint4 *>(at)); }
@@ -182,7 +193,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             mbar_init(&S.v_full[i], kCodeWarps);
             mbar_init(&S.v_empty[i], 1);
         }
-        for (int i = 0; i < kScaleRing; ++i) mbar_init(&S.scale_full[i], 1);
+        for (int i = 0; i < kScaleRing; ++i) mbar_init(&S.scale_full[i], kCodeWarps);
         mbar_init(&S.drain, 1);
         S.abort = 0;
         fence_mbar_init();
@@ -205,6 +216,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
 
     if (warp < kSoftWarps) {
         // ---------------------------------------------------------- softmax
+        more_registers<kSoftRegs>();
         const int m = warp >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const uint32_t s_at = tmem + lanes + m * kSCol, o_at = tmem + lanes + kOCol + m * 128;
@@ -216,33 +228,49 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             const int64_t tok = (int64_t)it.t0 + m * tq + i;
             const int64_t out_at = tok * p.ldo + (int64_t)(head0 + gg) * DV;
             if (nt == 0 || cnt <= 0) {
-                if (live)
-                    for (int d = 0; d < DV; ++d) reinterpret_cast<__nv_bfloat16 *>(p.out)[out_at + d] = __float2bfloat16_rn(0.0f);
+                // nothing to see: zeros, a row a warp at a time
+                for (int x = 0; x < 32 && cnt > 0; ++x) {
+                    const int64_t at = __shfl_sync(0xffffffffu, live ? out_at : -1, x);
+                    if (at >= 0)
+                        for (int d = lane; d < DV; d += 32) reinterpret_cast<__nv_bfloat16 *>(p.out)[at + d] = __float2bfloat16_rn(0.0f);
+                }
                 u += nt;
                 continue;
             }
-            // q: the row by a power of two, as fp16, 64 dims a 128-byte row
-            float back;
-            {
-                const int64_t at = live ? tok * p.ldq + (int64_t)(head0 + gg) * DK : 0;
-                float mx = 0.0f;
-                if (live)
-                    for (int d = 0; d < DK; d += 4) {
-                        const float4 v = load_q4(p, at + d);
-                        mx = max_abs(max_abs(max_abs(max_abs(mx, v.x), v.y), v.z), v.w);
+            // q: rows by a power of two, as fp16, 64 dims a 128-byte row; four of the
+            // warp's rows at a time, four dims a lane
+            float back = 0.0f;
+            constexpr int kRep = (DK + 127) / 128;
+#pragma unroll 1
+            for (int x = 0; x < 32; x += 4) {
+                float4 v[4][kRep];
+                const int64_t mine = live ? tok * p.ldq + (int64_t)(head0 + gg) * DK : -1;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int64_t at = __shfl_sync(0xffffffffu, mine, x + y);
+#pragma unroll
+                    for (int z = 0; z < kRep; ++z) {
+                        const int d = 4 * lane + 128 * z;
+                        v[y][z] = at >= 0 && d < DK ? load_q4(p, at + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
-                const int e = q_exponent(mx);
-                const float up = pow2i(14 - e);
-                back = pow2i(e - 14);
-                for (int d = 0; d < DK; d += 8) {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        const float4 a = load_q4(p, at + d), b = load_q4(p, at + d + 4);
-                        w = make_uint4(h2(a.x * up, a.y * up), h2(a.z * up, a.w * up), h2(b.x * up, b.y * up),
-                                       h2(b.z * up, b.w * up));
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    float mx = 0.0f;
+#pragma unroll
+                    for (int z = 0; z < kRep; ++z)
+                        mx = max_abs(max_abs(max_abs(max_abs(mx, v[y][z].x), v[y][z].y), v[y][z].z), v[y][z].w);
+                    const int e = q_exponent(warp_max(mx)), at = q * 32 + x + y;
+                    const float up = pow2i(14 - e);
+                    if (lane == x + y) back = pow2i(e - 14);
+#pragma unroll
+                    for (int z = 0; z < kRep; ++z) {
+                        const int d = 4 * lane + 128 * z;
+                        if (d < DK)
+                            *reinterpret_cast<uint2 *>(S.q[m] + (d >> 6) * (128 * 128) + at * 128 +
+                                                       ((((d >> 3) & 7) ^ (at & 7)) << 4) + 2 * (d & 4)) =
+                                make_uint2(h2(v[y][z].x * up, v[y][z].y * up), h2(v[y][z].z * up, v[y][z].w * up));
                     }
-                    *reinterpret_cast<uint4 *>(S.q[m] + (d >> 6) * (128 * 128) + row * 128 +
-                                               ((((d >> 3) & 7) ^ (row & 7)) << 4)) = w;
                 }
             }
             fence_proxy_async_smem();
@@ -259,71 +287,65 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 const float *f = S.f[u % kScaleRing], *lv = S.lv[u % kScaleRing], *iv = S.iv[u % kScaleRing];
                 const int see = last - j * KT;                               // columns 0 .. see are visible
                 const bool whole = j * KT + KT - 1 <= first_last && j * KT + KT <= it.keys;
-                float top = neg_inf();
+                uint32_t t[KT / 32][32];
 #pragma unroll
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld_x32(s_at + c, v);
-                    tmem_wait_ld();
+                for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(s_at + 32 * c, t[c]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float a = f[c / 16 + half] * back, b = lv[c / 16 + half];
-                        if (whole) {
+                        const float a = f[2 * c + half] * back, b = lv[2 * c + half];
 #pragma unroll
-                            for (int x = 0; x < 16; ++x)
-                                top = fmaxf(top, __fmaf_rn(__uint_as_float(v[16 * half + x]), a, b));
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < 16; ++x) {
-                                const float t = __fmaf_rn(__uint_as_float(v[16 * half + x]), a, b);
-                                top = c + 16 * half + x <= see ? fmaxf(top, t) : top;
-                            }
-                        }
+                        for (int x = 16 * half; x < 16 * half + 16; ++x)
+                            t[c][x] = __float_as_uint(__fmaf_rn(__uint_as_float(t[c][x]), a, b));
                     }
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (32 * c + x > see) t[c][x] = 0xff800000u;     // -inf
                 }
+                float tops[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) tops[x & 3] = fmaxf(tops[x & 3], __uint_as_float(t[c][x]));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 if (__any_sync(0xffffffffu, top > mx + kGrow)) {             // also the first tile: mx is -inf
                     const float to = top > mx ? top : mx;
                     const float by = to == neg_inf() ? 1.0f : ex2(mx - to);
                     mx = to;
                     sum *= by;
                     if (j > 0) {
-#pragma unroll
-                        for (int c = 0; c < DV; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld_x32(o_at + c, o);
+#pragma unroll 1
+                        for (int c = 0; c < DV; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld_x16(o_at + c, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * by);
-                            tmem_st_x32(o_at + c, o);
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * by);
+                            tmem_st_x16(o_at + c, o);
                         }
                     }
                 }
                 const float base = mx == neg_inf() ? 0.0f : mx - kShift;
 #pragma unroll
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t v[32], w[16];
-                    tmem_ld_x32(s_at + c, v);
-                    tmem_wait_ld();
+                for (int c = 0; c < KT / 32; ++c) {
+                    uint32_t w[16];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float a = f[c / 16 + half] * back, b = lv[c / 16 + half] - base;
                         float part = 0.0f;
 #pragma unroll
-                        for (int x = 0; x < 16; x += 2) {
-                            float t0 = __fmaf_rn(__uint_as_float(v[16 * half + x]), a, b);
-                            float t1 = __fmaf_rn(__uint_as_float(v[16 * half + x + 1]), a, b);
-                            if (!whole) {
-                                t0 = c + 16 * half + x <= see ? t0 : neg_inf();
-                                t1 = c + 16 * half + x + 1 <= see ? t1 : neg_inf();
-                            }
-                            t0 = ex2(t0);
-                            t1 = ex2(t1);
+                        for (int x = 16 * half; x < 16 * half + 16; x += 2) {
+                            const float t0 = ex2(__uint_as_float(t[c][x]) - base), t1 = ex2(__uint_as_float(t[c][x + 1]) - base);
                             part += t0 + t1;
-                            w[8 * half + x / 2] = h2(t0, t1);
+                            w[x / 2] = h2(t0, t1);
                         }
-                        sum = __fmaf_rn(part, iv[c / 16 + half], sum);
+                        sum = __fmaf_rn(part, iv[2 * c + half], sum);
                     }
-                    tmem_st_x16(s_at + c / 2, w);
+                    tmem_st_x16(s_at + 16 * c, w);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -368,90 +390,129 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         }
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------- codes to operands
-        constexpr int kKLoads = KT / 8 / kCodeWarps * (DK / 64);   // 8 tokens by 64 dims a load of the warp
-        constexpr int kVLoads = KT / 16 * (DV / 32) / kCodeWarps;  // 32 dims of a group of 16 tokens
+        fewer_registers<kCodeRegs>();
+        // Warp w has groups kOwn w .. of 16 tokens: of each the loads are 8 tokens by 64
+        // dims of K, 32 dims of V.  K of the next tile is loaded while V of this one is
+        // converted, and V while K is; the blocks are looked up two tiles ahead.
+        constexpr int kOwn = KT / 16 / kCodeWarps, kKLoads = 2 * (DK / 64), kVLoads = DV / 32;
         const int w = warp - kCodeWarp0, g = lane >> 2, c = lane & 3;
+        const int bs = p.c.block;
         while (ok && next_item(p, lo, span, few, r, it)) {
             const int nt = (it.keys + KT - 1) / KT;
             const int32_t *table = p.table + it.request * p.max_blocks;
-            auto block_of = [&](int tok) -> int64_t {
+            // the block and head of this warp's group x of tile j
+            auto block_of = [&](int j, int x) -> int64_t {
+                const int tok = j * KT + (w * kOwn + x) * 16;
                 if (tok >= it.keys) return -1;
                 const int64_t b = table[block_index(p, tok)];
                 return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
             };
-            // lane x's group x of a tile: its block, one tile ahead
-            int64_t ahead = lane < KT / 16 ? block_of(16 * lane) : -1;
+            auto off_of = [&](int j, int x) {
+                const int tok = j * KT + (w * kOwn + x) * 16;
+                return tok - block_index(p, tok) * bs;
+            };
+            uint4 kc[kOwn][kKLoads], vc[kOwn][kVLoads];
+            auto load_k = [&](int j, const int64_t (&bh)[kOwn]) {
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) {
+                    const int8_t *at = p.c.k + (bh[x] * (DK / 64) * bs + off_of(j, x) + g) * 64 + c * 16;
+#pragma unroll
+                    for (int y = 0; y < kKLoads; ++y)
+                        kc[x][y] = bh[x] >= 0 ? ldg_code(at + (y >> 1) * bs * 64 + (y & 1) * 512) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            auto load_v = [&](int j, const int64_t (&bh)[kOwn]) {
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) {
+                    const int8_t *at = p.c.v + ((bh[x] * (bs / 16) + off_of(j, x) / 16) * DV + lane) * 16;
+#pragma unroll
+                    for (int y = 0; y < kVLoads; ++y)
+                        vc[x][y] = bh[x] >= 0 ? ldg_code(at + y * 512) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            int64_t b0[kOwn], b1[kOwn], b2[kOwn];                    // of this tile, the next, the one after
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x) {
+                b0[x] = block_of(0, x);
+                b1[x] = block_of(1, x);
+            }
+            float kr = 0.0f, vr = 127.0f;                           // ranges of group `lane` of the warp's
+            auto load_ranges = [&](const int64_t (&bh)[kOwn]) {
+                int64_t mine = -1;
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) mine = lane == x ? bh[x] : mine;
+                kr = mine >= 0 ? p.c.k_range[mine] : 0.0f;
+                vr = mine >= 0 ? p.c.v_range[mine] : -1.0f;          // none
+            };
+            if (nt > 0) {
+                load_k(0, b0);
+                load_v(0, b0);
+                load_ranges(b0);
+            }
             for (int j = 0; j < nt; ++j, ++u) {
-                const int64_t mine = ahead;
-                ahead = lane < KT / 16 && j + 1 < nt ? block_of((j + 1) * KT + 16 * lane) : -1;
-                uint4 kc[kKLoads], vc[kVLoads];
+                const uint32_t st = u & 1;
 #pragma unroll
-                for (int x = 0; x < kKLoads; ++x) {
-                    const int J = x % (DK / 64), t = (w + kCodeWarps * (x / (DK / 64))) * 8 + g;   // dims 64 J, token t
-                    const int64_t bh = __shfl_sync(0xffffffffu, mine, t >> 4);
-                    const int tok = j * KT + t, off = tok - block_index(p, tok) * p.c.block;
-                    kc[x] = bh >= 0 ? ldg_code(p.c.k + ((bh * (DK / 64) + J) * p.c.block + off) * 64 + c * 16)
-                                    : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int x = 0; x < kVLoads; ++x) {
-                    const int grp = w + kCodeWarps * (x / (DV / 32)), d = (x % (DV / 32)) * 32 + lane;
-                    const int64_t bh = __shfl_sync(0xffffffffu, mine, grp);
-                    const int tok = j * KT + 16 * grp, off = tok - block_index(p, tok) * p.c.block;
-                    vc[x] = bh >= 0 ? ldg_code(p.c.v + ((bh * (p.c.block / 16) + off / 16) * DV + d) * 16)
-                                    : make_uint4(0, 0, 0, 0);
-                }
+                for (int x = 0; x < kOwn; ++x) b2[x] = block_of(j + 2, x);
                 // The groups' scales.  Their slot was the tile's four back: the softmax is done
                 // with it, since this warp has seen the scores of the tile three back finished
                 // (the last wait for an empty K), and those wait for that tile's P.
-                if (w == 0) {
-                    float kr = 0.0f, vr = 127.0f;
-                    if (mine >= 0) {
-                        kr = p.c.k_range[mine];
-                        vr = p.c.v_range[mine];
-                    }
-                    vr = vr < kRangeFloor ? kRangeFloor : vr;
-                    if (lane < KT / 16) {
-                        S.f[u % kScaleRing][lane] = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
-                        S.lv[u % kScaleRing][lane] = mine >= 0 ? log2f(__fdiv_rn(vr, 127.0f)) : neg_inf();
-                        S.iv[u % kScaleRing][lane] = mine >= 0 ? __fdiv_rn(127.0f, vr) : 0.0f;
-                    }
-                    __syncwarp();
+                if (lane < kOwn) {
+                    const bool none = vr == -1.0f;
+                    const float v1 = vr < kRangeFloor ? kRangeFloor : vr;
+                    S.f[u % kScaleRing][w * kOwn + lane] = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
+                    S.lv[u % kScaleRing][w * kOwn + lane] = none ? neg_inf() : log2f(__fdiv_rn(v1, 127.0f));
+                    S.iv[u % kScaleRing][w * kOwn + lane] = none ? 0.0f : __fdiv_rn(127.0f, v1);
                 }
-                const uint32_t st = u & 1;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.scale_full[u % kScaleRing]);
                 if (!(ok = mbar_wait_warp(&S.k_empty[st], ((u >> 1) & 1) ^ 1, abort, p.err))) break;
-                if (w == 0 && lane == 0) mbar_arrive(&S.scale_full[u % kScaleRing]);
 #pragma unroll
-                for (int x = 0; x < kKLoads; ++x) {
-                    const int J = x % (DK / 64), t = (w + kCodeWarps * (x / (DK / 64))) * 8 + g;
-                    store_codes(S.k[st] + J * (KT * 128) + t * 128, 2 * c, t, kc[x]);
-                }
+                for (int x = 0; x < kOwn; ++x)
+#pragma unroll
+                    for (int y = 0; y < kKLoads; ++y) {
+                        const int t = (w * kOwn + x) * 16 + (y & 1) * 8 + g;
+                        store_codes(S.k[st] + (y >> 1) * (KT * 128) + t * 128, 2 * c, g, kc[x][y]);
+                    }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.k_full[st]);
+                if (j + 1 < nt) {
+                    load_k(j + 1, b1);
+                    load_ranges(b1);
+                }
                 if (!(ok = mbar_wait_warp(&S.v_empty[st], ((u >> 1) & 1) ^ 1, abort, p.err))) break;
 #pragma unroll
-                for (int x = 0; x < kVLoads; ++x) {
-                    const int grp = w + kCodeWarps * (x / (DV / 32)), d = (x % (DV / 32)) * 32 + lane;
-                    store_codes(S.v[st] + (grp >> 2) * (DV * 128) + d * 128, 2 * (grp & 3), d, vc[x]);
-                }
+                for (int x = 0; x < kOwn; ++x)
+#pragma unroll
+                    for (int y = 0; y < kVLoads; ++y) {
+                        const int grp = w * kOwn + x, d = 32 * y + lane;
+                        store_codes(S.v[st] + (grp >> 2) * (DV * 128) + d * 128, 2 * (grp & 3), lane, vc[x][y]);
+                    }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.v_full[st]);
+                if (j + 1 < nt) load_v(j + 1, b1);
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) {
+                    b0[x] = b1[x];
+                    b1[x] = b2[x];
+                }
             }
         }
-    } else {
+    } else if (fewer_registers<kMmaRegs>(), warp == kMmaWarp) {
         // ---------------------------------------------------------- MMA
         const uint32_t is = idesc_f16(128, KT), io = idesc_f16(128, DV);
-        const uint64_t q0 = smem_desc(smem_u32(S.q[0]), 16, 1024, 2), k0 = smem_desc(smem_u32(S.k[0]), 16, 1024, 2),
-                       v0 = smem_desc(smem_u32(S.v[0]), 16, 1024, 2);
+        const uint64_t q0 = smem_desc(smem_u32(S.q[0]), 16, 1024, 2);
+        const uint32_t desc_hi = (uint32_t)(q0 >> 32), q_lo = (uint32_t)q0,
+                       k_lo = q_lo + (uint32_t)((S.k[0] - S.q[0]) >> 4), v_lo = q_lo + (uint32_t)((S.v[0] - S.q[0]) >> 4);
         bool issued = false;
         auto scores = [&](int m, uint32_t st) {
             if (lane == 0) {
+                const uint32_t d = tmem + m * kSCol, a = q_lo + ((m * Sm::kQ) >> 4), b = k_lo + ((st * Sm::kK) >> 4);
 #pragma unroll
                 for (int x = 0; x < DK / 16; ++x)
-                    mma_f16_ss(tmem + m * kSCol, q0 + ((m * Sm::kQ + (x >> 2) * (128 * 128)) >> 4) + 2 * (x & 3),
-                               k0 + ((st * Sm::kK + (x >> 2) * (KT * 128)) >> 4) + 2 * (x & 3), is, x != 0);
+                    mma_f16_ss(d, a + ((x >> 2) * (128 * 128) >> 4) + 2 * (x & 3),
+                               b + ((x >> 2) * (KT * 128) >> 4) + 2 * (x & 3), desc_hi, is, x != 0);
                 mma_commit(&S.s_full[m]);
             }
             issued = true;
@@ -476,11 +537,13 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     if (!(ok = mbar_wait_warp(&S.p_full[m], tiles[m] & 1, abort, p.err))) break;
                     ++tiles[m];
                     tc_fence_after();
-                    if (lane == 0)
+                    if (lane == 0) {
+                        const uint32_t d = tmem + kOCol + m * 128, a = tmem + m * kSCol, b = v_lo + ((st * Sm::kV) >> 4);
 #pragma unroll
-                        for (int x = 0; x < KT / 16; ++x)
-                            mma_f16_ts(tmem + kOCol + m * 128, tmem + m * kSCol + 8 * x,
-                                       v0 + ((st * Sm::kV + (x >> 2) * (DV * 128)) >> 4) + 2 * (x & 3), io, (j | x) != 0);
+                        for (int x = 0; x < KT / 16; ++x)          // kind::f16: the descriptor says which type
+                            mma_bf16_ts_lohi(d, a + 8 * x, b + ((x >> 2) * (DV * 128) >> 4) + 2 * (x & 3), desc_hi, io,
+                                             (j | x) != 0);
+                    }
                     if (j + 1 < nt) {
                         if (m == 0 && !(ok = mbar_wait_warp(&S.k_full[st1], ((u + 1) >> 1) & 1, abort, p.err))) break;
                         tc_fence_after();
