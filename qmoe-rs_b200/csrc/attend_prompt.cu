@@ -24,7 +24,7 @@
 // by 128 keys of 128 dims.
 #include "attend.cuh"
 #include "kernels.h"
-#include "sm100.cuh"
+#include "mma_warp.cuh"
 
 namespace qmoe {
 namespace {
@@ -62,17 +62,6 @@ struct Shared {
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
     return (1u << 4)          // D = f32; A, B = f16 (format 0)
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// D[tmem] (+)= A[smem] * B[smem]^T; a descriptor's halves apart, so that a step
-// is one 32-bit addition.
-QMOE_DEV void mma_f16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
-                         uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n .reg .b64 ad, bd;\n setp.ne.b32 p, %5, 0;\n mov.b64 ad, {%1, %3};\n mov.b64 bd, {%2, %3};\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, {%6, %6, %6, %6}, p;\n}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(0u)
-        : "memory");
 }
 
 template <int N>
@@ -507,14 +496,12 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                        k_lo = q_lo + (uint32_t)((S.k[0] - S.q[0]) >> 4), v_lo = q_lo + (uint32_t)((S.v[0] - S.q[0]) >> 4);
         bool issued = false;
         auto scores = [&](int m, uint32_t st) {
-            if (lane == 0) {
-                const uint32_t d = tmem + m * kSCol, a = q_lo + ((m * Sm::kQ) >> 4), b = k_lo + ((st * Sm::kK) >> 4);
+            const uint32_t d = tmem + m * kSCol, a = q_lo + ((m * Sm::kQ) >> 4), b = k_lo + ((st * Sm::kK) >> 4);
 #pragma unroll
-                for (int x = 0; x < DK / 16; ++x)
-                    mma_f16_ss(d, a + ((x >> 2) * (128 * 128) >> 4) + 2 * (x & 3),
-                               b + ((x >> 2) * (KT * 128) >> 4) + 2 * (x & 3), desc_hi, is, x != 0);
-                mma_commit(&S.s_full[m]);
-            }
+            for (int x = 0; x < DK / 16; ++x)
+                warp_mma_f16_ss(d, a + ((x >> 2) * (128 * 128) >> 4) + 2 * (x & 3),
+                                b + ((x >> 2) * (KT * 128) >> 4) + 2 * (x & 3), desc_hi, is, x != 0);
+            warp_commit(&S.s_full[m]);
             issued = true;
         };
         while (ok && next_item(p, lo, span, few, r, it)) {
@@ -530,39 +517,34 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                         scores(m, st);
                     }
                     if (!ok) break;
-                    if (lane == 0) mma_commit(&S.k_empty[st]);
+                    warp_commit(&S.k_empty[st]);
                 }
                 if (!(ok = mbar_wait_warp(&S.v_full[st], (u >> 1) & 1, abort, p.err))) break;
                 for (int m = 0; m < both; ++m) {
                     if (!(ok = mbar_wait_warp(&S.p_full[m], tiles[m] & 1, abort, p.err))) break;
                     ++tiles[m];
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t d = tmem + kOCol + m * 128, a = tmem + m * kSCol, b = v_lo + ((st * Sm::kV) >> 4);
+                    const uint32_t d = tmem + kOCol + m * 128, a = tmem + m * kSCol, b = v_lo + ((st * Sm::kV) >> 4);
 #pragma unroll
-                        for (int x = 0; x < KT / 16; ++x)          // kind::f16: the descriptor says which type
-                            mma_bf16_ts_lohi(d, a + 8 * x, b + ((x >> 2) * (DV * 128) >> 4) + 2 * (x & 3), desc_hi, io,
-                                             (j | x) != 0);
-                    }
+                    for (int x = 0; x < KT / 16; ++x)
+                        warp_mma_f16_ts(d, a + 8 * x, b + ((x >> 2) * (DV * 128) >> 4) + 2 * (x & 3), desc_hi, io, (j | x) != 0);
                     if (j + 1 < nt) {
                         if (m == 0 && !(ok = mbar_wait_warp(&S.k_full[st1], ((u + 1) >> 1) & 1, abort, p.err))) break;
                         tc_fence_after();
                         scores(m, st1);
                     } else {
-                        if (lane == 0) mma_commit(&S.o_full[m]);
+                        warp_commit(&S.o_full[m]);
                         ++items[m];
                     }
                 }
                 if (!ok) break;
-                if (lane == 0) {
-                    mma_commit(&S.v_empty[st]);
-                    if (j + 1 < nt) mma_commit(&S.k_empty[st1]);
-                }
+                warp_commit(&S.v_empty[st]);
+                if (j + 1 < nt) warp_commit(&S.k_empty[st1]);
             }
         }
         // every MMA issued so far completes before TMEM is freed
         if (issued) {
-            if (lane == 0) mma_commit(&S.drain);
+            warp_commit(&S.drain);
             __syncwarp();
             for (uint32_t n = 0; n < kMaxWaitProbes; ++n)
                 if (__all_sync(0xffffffffu, mbar_try_wait(&S.drain, 0))) break;

@@ -9,7 +9,7 @@
 // once to x's type.  A row of x with a non-finite element has the scale NaN.
 #include "code8.cuh"
 #include "kernels.h"
-#include "sm100.cuh"
+#include "mma_warp.cuh"
 
 namespace qmoe {
 namespace {
@@ -160,14 +160,6 @@ struct Smem {
     float sx[4][256];                             // each epilogue warp's copy of a tile's token scales
 };
 
-QMOE_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
-        : "memory");
-}
-
 template <bool BF16>
 QMOE_DEV void finish(const Int8GemmParams &p, int64_t t, int n, int sum, float sx, float sw, float res) {
     const int64_t at = t * p.N + n;
@@ -262,37 +254,36 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t u = 0, i = 0;
-            bool ok = true, issued = false;
-            const uint64_t d0 = smem_desc(smem_u32(ring), 16, 1024, 2);
-            for (int tile = tile0; ok && tile < total; tile += step, ++i) {
-                const int64_t left = p.T - (int64_t)(tile % tiles_t) * BN;
-                const int N = left >= BN ? BN : (int)(left + 15) / 16 * 16;
-                const uint32_t idesc = idesc_i8(128, N, true, true);
-                const uint32_t d = tmem + (i & 1) * BN;
-                if (!(ok = mbar_wait(&S->dempty[i & 1], ((i >> 1) & 1) ^ 1, abort, p.err))) break;
+        uint32_t u = 0, i = 0;
+        bool ok = true, issued = false;
+        const uint64_t d0 = smem_desc(smem_u32(ring), 16, 1024, 2);
+        const uint32_t lo = (uint32_t)d0, hi = (uint32_t)(d0 >> 32);
+        for (int tile = tile0; ok && tile < total; tile += step, ++i) {
+            const int64_t left = p.T - (int64_t)(tile % tiles_t) * BN;
+            const int N = left >= BN ? BN : (int)(left + 15) / 16 * 16;
+            const uint32_t idesc = idesc_i8(128, N, true, true);
+            const uint32_t d = tmem + (i & 1) * BN;
+            if (!(ok = mbar_wait_warp(&S->dempty[i & 1], ((i >> 1) & 1) ^ 1, abort, p.err))) break;
+            tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb, ++u) {
+                const uint32_t s = u % Cfg::stages;
+                if (!(ok = mbar_wait_warp(&S->full[s], (u / Cfg::stages) & 1, abort, p.err))) break;
                 tc_fence_after();
-                for (int kb = kb0; kb < kb1; ++kb, ++u) {
-                    const uint32_t s = u % Cfg::stages;
-                    if (!(ok = mbar_wait(&S->full[s], (u / Cfg::stages) & 1, abort, p.err))) break;
-                    tc_fence_after();
-                    const uint64_t a = d0 + ((s * Cfg::stage) >> 4), b = a + (kABytes >> 4);
+                const uint32_t a = lo + ((s * Cfg::stage) >> 4), b = a + (kABytes >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_i8_ss(d, a + 2 * kk, b + 2 * kk, idesc, (kb != kb0) | (kk != 0));
-                    issued = true;
-                    mma_commit(&S->empty[s]);
-                }
-                if (!ok) break;
-                mma_commit(&S->dfull[i & 1]);
+                for (int kk = 0; kk < 4; ++kk)
+                    warp_mma_i8_ss(d, a + 2 * kk, b + 2 * kk, hi, idesc, (kb != kb0) | (kk != 0));
+                issued = true;
+                warp_commit(&S->empty[s]);
             }
-            // every MMA issued so far completes before TMEM is freed
-            if (issued) {
-                mma_commit(&S->drain);
-                for (uint32_t n = 0; n < kMaxWaitProbes; ++n)
-                    if (mbar_try_wait(&S->drain, 0)) break;
-            }
+            if (!ok) break;
+            warp_commit(&S->dfull[i & 1]);
+        }
+        // every MMA issued so far completes before TMEM is freed
+        if (issued) {
+            warp_commit(&S->drain);
+            for (uint32_t n = 0; n < kMaxWaitProbes; ++n)
+                if (__all_sync(0xffffffffu, mbar_try_wait(&S->drain, 0))) break;
         }
         __syncwarp();
     } else if (warp >= 4) {
