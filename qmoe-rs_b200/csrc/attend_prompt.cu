@@ -5,23 +5,24 @@
 // blocks' scales folded into t = (q . ck) * f + log2(rv / 127), P = 2^(t - M) in
 // fp16, f32 sums.  What differs is where it runs.  A CTA takes 256 query rows
 // (two tiles of 128: tq tokens by the heads that share a kv head) and goes once
-// over their keys in tiles of KT tokens:
+// over their keys in tiles of 64 tokens:
 //
 //   warps 0-3, 4-7   one row of a query tile a thread: q to fp16 in shared
 //                    memory, then per key tile the scores from tensor memory,
 //                    the running maximum and sum, P back to tensor memory
-//   warps 8-11       codes from the cache to fp16 operands in shared memory
-//                    (K [token][dim], V [dim][token], 128-byte swizzle), the
-//                    16-token groups' scales beside them
-//   warp 12          tcgen05: S = q K^T (both operands in shared memory), then
-//                    O += P V (P from tensor memory), the two query tiles in
-//                    turn, so that one's softmax runs under the other's MMAs
+//   warps 8-11       K: codes from the cache to fp16 operands in shared memory
+//                    ([token][dim], 128-byte swizzle), a group of 16 tokens a
+//                    warp, and the groups' scales
+//   warps 12-15      V likewise ([dim][token])
+//   warp 16          tcgen05: S = q K^T (both operands in shared memory), then
+//                    O += P V (P from tensor memory)
 //
-// O stays in tensor memory.  It is rescaled only where a row's maximum has
-// grown by more than 2^8 since it was last scaled; until then P may reach
-// 2^(8 + 6), which fp16 holds.  Work is bound by the exponentials (a quarter of
-// an MMA's elements a cycle) and the MMAs alike: 2048 cycles each for 256 rows
-// by 128 keys of 128 dims.
+// Tensor memory holds two score tiles and O of each query tile.  The scores of
+// a tile are asked for two tiles ahead, so a softmax waits for no MMA, and the
+// two query tiles' softmaxes run side by side.  O is rescaled only where a row's
+// maximum has grown by more than 2^8 since it was last scaled; until then P may
+// reach 2^(8 + 6), which fp16 holds.  For 256 rows by 128 keys of 128 dims the
+// exponentials take 2048 cycles of an SM (16 a cycle) and the MMAs as many.
 #include "attend.cuh"
 #include "kernels.h"
 #include "mma_warp.cuh"
@@ -31,29 +32,27 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kSoftWarps = 8;
-constexpr int kCodeWarp0 = 8, kCodeWarps = 4;
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 16 * 32;             // warps 13-15 only give their registers up
-// Registers a thread: the softmax holds a row's scores of a tile.  Of the 128 a
-// thread that the CTA is launched with, 2 * 168 + 112 + 64 = 4 * 128.
-constexpr int kSoftRegs = 168, kCodeRegs = 112, kMmaRegs = 64;
-static_assert(2 * kSoftRegs + kCodeRegs + kMmaRegs <= 512, "registers of the CTA");
+constexpr int kSoftWarps = 8, kVWarp0 = 12, kMmaWarp = 16;
+constexpr int kThreads = 17 * 32;
+constexpr int KT = 64;                        // keys a tile: a group of 16 for each K and V warp
 constexpr float kGrow = 8.0f;                 // log2 of how far a maximum may outgrow the scaling
 constexpr float kShift = 6.0f;                // P = 2^6 at the scaling's maximum
-constexpr int kScaleRing = 4;                 // tiles whose scales are kept: the codes run at most
-                                              // two tiles ahead of the softmax
+// Tiles whose scales are kept.  A K warp writes those of tile u once the scores
+// of tile u - stages are done; these were asked for after P of tile u - stages -
+// 2, so the softmax is done with the slot's tile u - 8.
+constexpr int kScaleRing = 8;
 
-template <int DK, int DV, int KT>
+template <int DK, int DV>
 struct Shared {
+    static constexpr int kStages = DK > 128 ? 3 : 4;
     static constexpr int kQ = 128 * DK * 2, kK = KT * DK * 2, kV = DV * KT * 2;
+    static_assert(kStages + 2 <= kScaleRing, "scales");
     uint8_t q[2][kQ];
-    uint8_t k[2][kK];
-    uint8_t v[2][kV];
+    uint8_t k[kStages][kK];
+    uint8_t v[kStages][kV];
     float f[kScaleRing][KT / 16], lv[kScaleRing][KT / 16], iv[kScaleRing][KT / 16];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t scale_full[kScaleRing];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
+    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t drain;
     uint32_t tmem_base;
     int abort;
@@ -62,15 +61,6 @@ struct Shared {
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
     return (1u << 4)          // D = f32; A, B = f16 (format 0)
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-template <int N>
-QMOE_DEV void more_registers() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-QMOE_DEV void fewer_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 QMOE_DEV uint4 ldg_code(const int8_t *at) { return __ldg(reinterpret_cast<const uint4 *>(at)); }
@@ -152,19 +142,21 @@ QMOE_DEV int64_t first_request(const int32_t *start, int64_t R, int64_t lo) {
     return at;
 }
 
-template <int DK, int DV, int KT>
+template <int DK, int DV>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int hgroups, const int few) {
-    using Sm = Shared<DK, DV, KT>;
+    using Sm = Shared<DK, DV>;
+    constexpr int kStages = Sm::kStages;
     extern __shared__ uint8_t smem_raw[];
     Sm &S = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
-    // late windows first: their rows see the most keys
-    const int span = 2 * tq;
-    const int64_t lo = (int64_t)(gridDim.x - 1 - blockIdx.x) * span;
-    const int h = blockIdx.y / hgroups, hg = blockIdx.y - h * hgroups, G = p.heads / p.c.heads;
+    // late windows of all heads first: their rows see the most keys
+    const int span = 2 * tq, groups = p.c.heads * hgroups, windows = gridDim.x / groups;
+    const int window = blockIdx.x / groups, hh = blockIdx.x - window * groups;
+    const int64_t lo = (int64_t)(windows - 1 - window) * span;
+    const int h = hh / hgroups, hg = hh - h * hgroups, G = p.heads / p.c.heads;
     const int head0 = h * G + hg * gq, heads_here = G - hg * gq < gq ? G - hg * gq : gq;
     int64_t r = first_request(p.q_start, p.R, lo);
     const int64_t r0 = r;
@@ -174,15 +166,18 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&S.q_full[i], 4);
-            mbar_init(&S.s_full[i], 1);
-            mbar_init(&S.p_full[i], 4);
-            mbar_init(&S.o_full[i], 1);
-            mbar_init(&S.k_full[i], kCodeWarps);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&S.s_full[i][b], 2);        // the MMAs, and the warp that issued them
+                mbar_init(&S.p_full[i][b], 4);
+                mbar_init(&S.pv_done[i][b], 1);
+            }
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&S.k_full[i], 4);
             mbar_init(&S.k_empty[i], 1);
-            mbar_init(&S.v_full[i], kCodeWarps);
+            mbar_init(&S.v_full[i], 4);
             mbar_init(&S.v_empty[i], 1);
         }
-        for (int i = 0; i < kScaleRing; ++i) mbar_init(&S.scale_full[i], kCodeWarps);
         mbar_init(&S.drain, 1);
         S.abort = 0;
         fence_mbar_init();
@@ -195,20 +190,20 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem_base;
-    constexpr uint32_t kSCol = 128, kOCol = 256;      // S (and P in its first half) of tile m at 128 m, O at 256 + 128 m
+    // columns: scores (P in a tile's first half) of query tile m, buffer b at
+    // 128 m + 64 b; O of query tile m at 256 + 128 m
+    constexpr uint32_t kOCol = 256;
     volatile int *abort = &S.abort;
     bool ok = true;
-    uint32_t u = 0;                                   // key tiles so far
-    uint32_t items[2] = {0, 0};                       // items with query tile m so far
-    uint32_t tiles[2] = {0, 0};                       // key tiles with query tile m so far
     r = r0;
 
     if (warp < kSoftWarps) {
         // ---------------------------------------------------------- softmax
-        more_registers<kSoftRegs>();
         const int m = warp >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const uint32_t s_at = tmem + lanes + m * kSCol, o_at = tmem + lanes + kOCol + m * 128;
+        const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + kOCol + m * 128;
+        const float scale = fabsf(p.scale) * kLog2e, sign = p.scale < 0.0f ? -1.0f : 1.0f;
+        uint32_t u = 0, n = 0;                        // key tiles of the CTA, and those with this query tile, so far
         while (ok && next_item(p, lo, span, few, r, it)) {
             const int cnt = it.cnt - m * tq < tq ? it.cnt - m * tq : tq;      // tokens of this query tile
             const int nt = (it.keys + KT - 1) / KT;
@@ -226,16 +221,16 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 u += nt;
                 continue;
             }
-            // q: rows by a power of two, as fp16, 64 dims a 128-byte row; four of the
-            // warp's rows at a time, four dims a lane
+            // q: rows by a power of two (and the scale's sign), as fp16, 64 dims a
+            // 128-byte row; some of the warp's rows at a time, four dims a lane
             float back = 0.0f;
-            constexpr int kRep = (DK + 127) / 128;
+            constexpr int kRep = (DK + 127) / 128, kAtOnce = 8 / kRep;
 #pragma unroll 1
-            for (int x = 0; x < 32; x += 4) {
-                float4 v[4][kRep];
+            for (int x = 0; x < 32; x += kAtOnce) {
+                float4 v[kAtOnce][kRep];
                 const int64_t mine = live ? tok * p.ldq + (int64_t)(head0 + gg) * DK : -1;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < kAtOnce; ++y) {
                     const int64_t at = __shfl_sync(0xffffffffu, mine, x + y);
 #pragma unroll
                     for (int z = 0; z < kRep; ++z) {
@@ -244,13 +239,13 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     }
                 }
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < kAtOnce; ++y) {
                     float mx = 0.0f;
 #pragma unroll
                     for (int z = 0; z < kRep; ++z)
                         mx = max_abs(max_abs(max_abs(max_abs(mx, v[y][z].x), v[y][z].y), v[y][z].z), v[y][z].w);
                     const int e = q_exponent(warp_max(mx)), at = q * 32 + x + y;
-                    const float up = pow2i(14 - e);
+                    const float up = sign * pow2i(14 - e);
                     if (lane == x + y) back = pow2i(e - 14);
 #pragma unroll
                     for (int z = 0; z < kRep; ++z) {
@@ -265,49 +260,52 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.q_full[m]);
+            back *= scale;
             const int last = live ? it.pos0 + m * tq + i : -1;               // this row's last key
             const int first_last = it.pos0 + m * tq;                         // the first token's
             float mx = neg_inf(), sum = 0.0f;                                // mx: what O and sum are scaled to
-            for (int j = 0; j < nt; ++j, ++u, ++tiles[m]) {
-                if (!(ok = mbar_wait_warp(&S.s_full[m], tiles[m] & 1, abort, p.err))) break;
-                // complete by now (the codes came after it): the wait orders the reads behind it
-                if (!(ok = mbar_wait_warp(&S.scale_full[u % kScaleRing], (u / kScaleRing) & 1, abort, p.err))) break;
+            for (int j = 0; j < nt; ++j, ++u, ++n) {
+                const uint32_t at = s_at + 64 * (n & 1);
+                if (!(ok = mbar_wait_warp(&S.s_full[m][n & 1], (n >> 1) & 1, abort, p.err))) break;
                 tc_fence_after();
-                const float *f = S.f[u % kScaleRing], *lv = S.lv[u % kScaleRing], *iv = S.iv[u % kScaleRing];
+                uint32_t t[2][32];
+                tmem_ld_x32(at, t[0]);
+                tmem_ld_x32(at + 32, t[1]);
+                // the groups' factors: a > 0, so that a masked score of -inf stays one and
+                // the largest score is the largest t (a poisoned group's NaN is in lv)
+                float a[4], b[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    a[x] = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
+                    b[x] = S.lv[u % kScaleRing][x];
+                }
                 const int see = last - j * KT;                               // columns 0 .. see are visible
                 const bool whole = j * KT + KT - 1 <= first_last && j * KT + KT <= it.keys;
-                uint32_t t[KT / 32][32];
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(s_at + 32 * c, t[c]);
                 tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float a = f[2 * c + half] * back, b = lv[2 * c + half];
-#pragma unroll
-                        for (int x = 16 * half; x < 16 * half + 16; ++x)
-                            t[c][x] = __float_as_uint(__fmaf_rn(__uint_as_float(t[c][x]), a, b));
-                    }
                 if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (32 * c + x > see) t[c][x] = 0xff800000u;     // -inf
+                    for (int x = 0; x < 64; ++x)
+                        if (x > see) t[x >> 5][x & 31] = 0xff800000u;        // -inf
                 }
-                float tops[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+                float top = neg_inf();
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
+                for (int x = 0; x < 4; ++x) {
+                    float g0 = neg_inf(), g1 = neg_inf();
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) tops[x & 3] = fmaxf(tops[x & 3], __uint_as_float(t[c][x]));
-                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    for (int y = 0; y < 16; y += 2) {
+                        g0 = fmaxf(g0, __uint_as_float(t[x >> 1][16 * (x & 1) + y]));
+                        g1 = fmaxf(g1, __uint_as_float(t[x >> 1][16 * (x & 1) + y + 1]));
+                    }
+                    top = fmaxf(top, __fmaf_rn(fmaxf(g0, g1), a[x], b[x]));
+                }
                 if (__any_sync(0xffffffffu, top > mx + kGrow)) {             // also the first tile: mx is -inf
                     const float to = top > mx ? top : mx;
                     const float by = to == neg_inf() ? 1.0f : ex2(mx - to);
                     mx = to;
                     sum *= by;
-                    if (j > 0) {
+                    if (j > 0) {                                             // O is the last tile's product's until it is done
+                        if (!(ok = mbar_wait_warp(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DV; c += 16) {
                             uint32_t o[16];
@@ -321,33 +319,34 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 }
                 const float base = mx == neg_inf() ? 0.0f : mx - kShift;
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
+                        const float ga = a[2 * c + half], gb = b[2 * c + half] - base;
                         float part = 0.0f;
 #pragma unroll
                         for (int x = 16 * half; x < 16 * half + 16; x += 2) {
-                            const float t0 = ex2(__uint_as_float(t[c][x]) - base), t1 = ex2(__uint_as_float(t[c][x + 1]) - base);
+                            const float t0 = ex2(__fmaf_rn(__uint_as_float(t[c][x]), ga, gb));
+                            const float t1 = ex2(__fmaf_rn(__uint_as_float(t[c][x + 1]), ga, gb));
                             part += t0 + t1;
                             w[x / 2] = h2(t0, t1);
                         }
-                        sum = __fmaf_rn(part, iv[2 * c + half], sum);
+                        sum = __fmaf_rn(part, S.iv[u % kScaleRing][2 * c + half], sum);
                     }
-                    tmem_st_x16(s_at + 16 * c, w);
+                    tmem_st_x16(at + 16 * c, w);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.p_full[m]);
+                if (lane == 0) mbar_arrive(&S.p_full[m][n & 1]);
             }
             if (!ok) break;
-            if (!(ok = mbar_wait_warp(&S.o_full[m], items[m] & 1, abort, p.err))) break;
-            ++items[m];
+            if (!(ok = mbar_wait_warp(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
             tc_fence_after();
             const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
             const bool wide = p.vec_out;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < DV; c += 32) {
                 uint32_t o[32];
                 tmem_ld_x32(o_at + c, o);
@@ -359,10 +358,10 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                         uint32_t w[4];
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(
                                 sum == 0.0f ? 0.0f : __uint_as_float(o[x + 2 * y]) * inv,
                                 sum == 0.0f ? 0.0f : __uint_as_float(o[x + 2 * y + 1]) * inv);
-                            w[y] = *reinterpret_cast<const uint32_t *>(&b);
+                            w[y] = *reinterpret_cast<const uint32_t *>(&v);
                         }
                         if (wide) {
                             *reinterpret_cast<uint4 *>(to + x) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -379,173 +378,134 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         }
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------- codes to operands
-        fewer_registers<kCodeRegs>();
-        // Warp w has groups kOwn w .. of 16 tokens: of each the loads are 8 tokens by 64
-        // dims of K, 32 dims of V.  K of the next tile is loaded while V of this one is
-        // converted, and V while K is; the blocks are looked up two tiles ahead.
-        constexpr int kOwn = KT / 16 / kCodeWarps, kKLoads = 2 * (DK / 64), kVLoads = DV / 32;
-        const int w = warp - kCodeWarp0, g = lane >> 2, c = lane & 3;
-        const int bs = p.c.block;
+        // A warp has one group of 16 tokens of each tile, of K (loads of 8 tokens by 64
+        // dims) or V (32 dims).  The next tile's codes are loaded while this one's wait
+        // for their stage; blocks are looked up two tiles ahead.
+        const bool is_v = warp >= kVWarp0;
+        const int grp = warp & 3, g = lane >> 2, c = lane & 3, bs = p.c.block;
+        constexpr int kKLoads = 2 * (DK / 64), kVLoads = DV / 32, kLoads = kKLoads > kVLoads ? kKLoads : kVLoads;
+        uint32_t u = 0;
         while (ok && next_item(p, lo, span, few, r, it)) {
             const int nt = (it.keys + KT - 1) / KT;
             const int32_t *table = p.table + it.request * p.max_blocks;
-            // the block and head of this warp's group x of tile j
-            auto block_of = [&](int j, int x) -> int64_t {
-                const int tok = j * KT + (w * kOwn + x) * 16;
+            auto block_of = [&](int j) -> int64_t {
+                const int tok = j * KT + grp * 16;
                 if (tok >= it.keys) return -1;
                 const int64_t b = table[block_index(p, tok)];
                 return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
             };
-            auto off_of = [&](int j, int x) {
-                const int tok = j * KT + (w * kOwn + x) * 16;
-                return tok - block_index(p, tok) * bs;
-            };
-            uint4 kc[kOwn][kKLoads], vc[kOwn][kVLoads];
-            auto load_k = [&](int j, const int64_t (&bh)[kOwn]) {
+            uint4 codes[kLoads];
+            auto load = [&](int j, int64_t bh) {
+                const int tok = j * KT + grp * 16, off = tok - block_index(p, tok) * bs;
+                const int8_t *at = is_v ? p.c.v + ((bh * (bs / 16) + off / 16) * DV + lane) * 16
+                                        : p.c.k + (bh * (DK / 64) * bs + off + g) * 64 + c * 16;
 #pragma unroll
-                for (int x = 0; x < kOwn; ++x) {
-                    const int8_t *at = p.c.k + (bh[x] * (DK / 64) * bs + off_of(j, x) + g) * 64 + c * 16;
-#pragma unroll
-                    for (int y = 0; y < kKLoads; ++y)
-                        kc[x][y] = bh[x] >= 0 ? ldg_code(at + (y >> 1) * bs * 64 + (y & 1) * 512) : make_uint4(0, 0, 0, 0);
+                for (int y = 0; y < kLoads; ++y) {
+                    const int step = is_v ? y * 512 : (y >> 1) * bs * 64 + (y & 1) * 512;
+                    codes[y] = bh >= 0 && y < (is_v ? kVLoads : kKLoads) ? ldg_code(at + step) : make_uint4(0, 0, 0, 0);
                 }
             };
-            auto load_v = [&](int j, const int64_t (&bh)[kOwn]) {
-#pragma unroll
-                for (int x = 0; x < kOwn; ++x) {
-                    const int8_t *at = p.c.v + ((bh[x] * (bs / 16) + off_of(j, x) / 16) * DV + lane) * 16;
-#pragma unroll
-                    for (int y = 0; y < kVLoads; ++y)
-                        vc[x][y] = bh[x] >= 0 ? ldg_code(at + y * 512) : make_uint4(0, 0, 0, 0);
-                }
-            };
-            int64_t b0[kOwn], b1[kOwn], b2[kOwn];                    // of this tile, the next, the one after
-#pragma unroll
-            for (int x = 0; x < kOwn; ++x) {
-                b0[x] = block_of(0, x);
-                b1[x] = block_of(1, x);
-            }
-            float kr = 0.0f, vr = 127.0f;                           // ranges of group `lane` of the warp's
-            auto load_ranges = [&](const int64_t (&bh)[kOwn]) {
-                int64_t mine = -1;
-#pragma unroll
-                for (int x = 0; x < kOwn; ++x) mine = lane == x ? bh[x] : mine;
-                kr = mine >= 0 ? p.c.k_range[mine] : 0.0f;
-                vr = mine >= 0 ? p.c.v_range[mine] : -1.0f;          // none
+            int64_t b1 = block_of(1);
+            float kr = 0.0f, vr = -1.0f;              // of the group; vr -1: none
+            auto load_ranges = [&](int64_t bh) {
+                kr = bh >= 0 ? p.c.k_range[bh] : 0.0f;
+                vr = bh >= 0 ? p.c.v_range[bh] : -1.0f;
             };
             if (nt > 0) {
-                load_k(0, b0);
-                load_v(0, b0);
-                load_ranges(b0);
+                const int64_t b0 = block_of(0);
+                load(0, b0);
+                if (!is_v) load_ranges(b0);
             }
             for (int j = 0; j < nt; ++j, ++u) {
-                const uint32_t st = u & 1;
+                const uint32_t st = u % kStages, phase = (u / kStages) & 1;
+                const int64_t b2 = block_of(j + 2);
+                if (!(ok = mbar_wait_warp(is_v ? &S.v_empty[st] : &S.k_empty[st], phase ^ 1, abort, p.err))) break;
+                if (is_v) {
 #pragma unroll
-                for (int x = 0; x < kOwn; ++x) b2[x] = block_of(j + 2, x);
-                // The groups' scales.  Their slot was the tile's four back: the softmax is done
-                // with it, since this warp has seen the scores of the tile three back finished
-                // (the last wait for an empty K), and those wait for that tile's P.
-                if (lane < kOwn) {
-                    const bool none = vr == -1.0f;
-                    const float v1 = vr < kRangeFloor ? kRangeFloor : vr;
-                    S.f[u % kScaleRing][w * kOwn + lane] = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
-                    S.lv[u % kScaleRing][w * kOwn + lane] = none ? neg_inf() : log2f(__fdiv_rn(v1, 127.0f));
-                    S.iv[u % kScaleRing][w * kOwn + lane] = none ? 0.0f : __fdiv_rn(127.0f, v1);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.scale_full[u % kScaleRing]);
-                if (!(ok = mbar_wait_warp(&S.k_empty[st], ((u >> 1) & 1) ^ 1, abort, p.err))) break;
+                    for (int y = 0; y < kVLoads; ++y)
+                        store_codes(S.v[st] + (32 * y + lane) * 128, 2 * grp, lane, codes[y]);
+                } else {
 #pragma unroll
-                for (int x = 0; x < kOwn; ++x)
-#pragma unroll
-                    for (int y = 0; y < kKLoads; ++y) {
-                        const int t = (w * kOwn + x) * 16 + (y & 1) * 8 + g;
-                        store_codes(S.k[st] + (y >> 1) * (KT * 128) + t * 128, 2 * c, g, kc[x][y]);
+                    for (int y = 0; y < kKLoads; ++y)
+                        store_codes(S.k[st] + (y >> 1) * (KT * 128) + (grp * 16 + (y & 1) * 8 + g) * 128, 2 * c, g, codes[y]);
+                    if (lane == 0) {
+                        const float v1 = vr < kRangeFloor ? kRangeFloor : vr;
+                        S.f[u % kScaleRing][grp] = __fdiv_rn(kr, 127.0f);
+                        S.lv[u % kScaleRing][grp] = vr == -1.0f ? neg_inf() : kr != kr ? kr : log2f(__fdiv_rn(v1, 127.0f));
+                        S.iv[u % kScaleRing][grp] = vr == -1.0f ? 0.0f : __fdiv_rn(127.0f, v1);
                     }
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.k_full[st]);
+                if (lane == 0) mbar_arrive(is_v ? &S.v_full[st] : &S.k_full[st]);
                 if (j + 1 < nt) {
-                    load_k(j + 1, b1);
-                    load_ranges(b1);
+                    load(j + 1, b1);
+                    if (!is_v) load_ranges(b1);
                 }
-                if (!(ok = mbar_wait_warp(&S.v_empty[st], ((u >> 1) & 1) ^ 1, abort, p.err))) break;
-#pragma unroll
-                for (int x = 0; x < kOwn; ++x)
-#pragma unroll
-                    for (int y = 0; y < kVLoads; ++y) {
-                        const int grp = w * kOwn + x, d = 32 * y + lane;
-                        store_codes(S.v[st] + (grp >> 2) * (DV * 128) + d * 128, 2 * (grp & 3), lane, vc[x][y]);
-                    }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.v_full[st]);
-                if (j + 1 < nt) load_v(j + 1, b1);
-#pragma unroll
-                for (int x = 0; x < kOwn; ++x) {
-                    b0[x] = b1[x];
-                    b1[x] = b2[x];
-                }
+                b1 = b2;
             }
         }
-    } else if (fewer_registers<kMmaRegs>(), warp == kMmaWarp) {
+    } else {
         // ---------------------------------------------------------- MMA
         const uint32_t is = idesc_f16(128, KT), io = idesc_f16(128, DV);
         const uint64_t q0 = smem_desc(smem_u32(S.q[0]), 16, 1024, 2);
         const uint32_t desc_hi = (uint32_t)(q0 >> 32), q_lo = (uint32_t)q0,
                        k_lo = q_lo + (uint32_t)((S.k[0] - S.q[0]) >> 4), v_lo = q_lo + (uint32_t)((S.v[0] - S.q[0]) >> 4);
         bool issued = false;
+        uint32_t u = 0, items[2] = {0, 0}, asked[2] = {0, 0}, used[2] = {0, 0};   // tiles whose scores / P of m, so far
         auto scores = [&](int m, uint32_t st) {
-            const uint32_t d = tmem + m * kSCol, a = q_lo + ((m * Sm::kQ) >> 4), b = k_lo + ((st * Sm::kK) >> 4);
+            const uint32_t b = asked[m]++ & 1, d = tmem + m * 128 + 64 * b;
+            const uint32_t qa = q_lo + ((m * Sm::kQ) >> 4), ka = k_lo + st * (Sm::kK >> 4);
 #pragma unroll
             for (int x = 0; x < DK / 16; ++x)
-                warp_mma_f16_ss(d, a + ((x >> 2) * (128 * 128) >> 4) + 2 * (x & 3),
-                                b + ((x >> 2) * (KT * 128) >> 4) + 2 * (x & 3), desc_hi, is, x != 0);
-            warp_commit(&S.s_full[m]);
+                warp_mma_f16_ss(d, qa + ((x >> 2) * (128 * 128) >> 4) + 2 * (x & 3),
+                                ka + ((x >> 2) * (KT * 128) >> 4) + 2 * (x & 3), desc_hi, is, x != 0);
+            warp_commit(&S.s_full[m][b]);
+            // this warp has seen the stage's codes: its arrival passes the scales on too
+            if (lane == 0) mbar_arrive(&S.s_full[m][b]);
             issued = true;
         };
         while (ok && next_item(p, lo, span, few, r, it)) {
             const int nt = (it.keys + KT - 1) / KT;
             const int both = it.cnt > tq ? 2 : 1;                  // query tiles with tokens
-            for (int j = 0; j < nt && ok; ++j, ++u) {
-                const uint32_t st = u & 1, st1 = st ^ 1;
-                if (j == 0) {
-                    if (!(ok = mbar_wait_warp(&S.k_full[st], (u >> 1) & 1, abort, p.err))) break;
-                    for (int m = 0; m < both; ++m) {
-                        if (!(ok = mbar_wait_warp(&S.q_full[m], items[m] & 1, abort, p.err))) break;
-                        tc_fence_after();
-                        scores(m, st);
-                    }
-                    if (!ok) break;
-                    warp_commit(&S.k_empty[st]);
-                }
-                if (!(ok = mbar_wait_warp(&S.v_full[st], (u >> 1) & 1, abort, p.err))) break;
-                for (int m = 0; m < both; ++m) {
-                    if (!(ok = mbar_wait_warp(&S.p_full[m], tiles[m] & 1, abort, p.err))) break;
-                    ++tiles[m];
+            for (int j = 0; j < 2 && j < nt && ok; ++j) {          // the first two tiles' scores
+                const uint32_t st = (u + j) % kStages;
+                if (!(ok = mbar_wait_warp(&S.k_full[st], ((u + j) / kStages) & 1, abort, p.err))) break;
+                for (int m = 0; m < both && ok; ++m) {
+                    if (j == 0 && !(ok = mbar_wait_warp(&S.q_full[m], items[m]++ & 1, abort, p.err))) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + kOCol + m * 128, a = tmem + m * kSCol, b = v_lo + ((st * Sm::kV) >> 4);
+                    scores(m, st);
+                }
+                if (ok) warp_commit(&S.k_empty[st]);
+            }
+            for (int j = 0; j < nt && ok; ++j, ++u) {
+                const uint32_t st = u % kStages, st2 = (u + 2) % kStages;
+                if (!(ok = mbar_wait_warp(&S.v_full[st], (u / kStages) & 1, abort, p.err))) break;
+                for (int m = 0; m < both; ++m) {
+                    const uint32_t b = used[m] & 1;
+                    if (!(ok = mbar_wait_warp(&S.p_full[m][b], (used[m] >> 1) & 1, abort, p.err))) break;
+                    ++used[m];
+                    tc_fence_after();
+                    const uint32_t d = tmem + kOCol + m * 128, pa = tmem + m * 128 + 64 * b, va = v_lo + st * (Sm::kV >> 4);
 #pragma unroll
                     for (int x = 0; x < KT / 16; ++x)
-                        warp_mma_f16_ts(d, a + 8 * x, b + ((x >> 2) * (DV * 128) >> 4) + 2 * (x & 3), desc_hi, io, (j | x) != 0);
-                    if (j + 1 < nt) {
-                        if (m == 0 && !(ok = mbar_wait_warp(&S.k_full[st1], ((u + 1) >> 1) & 1, abort, p.err))) break;
+                        warp_mma_f16_ts(d, pa + 8 * x, va + 2 * x, desc_hi, io, (j | x) != 0);
+                    warp_commit(&S.pv_done[m][b]);
+                    issued = true;
+                    if (j + 2 < nt) {                              // in order after P V: its buffer is free
+                        if (m == 0 && !(ok = mbar_wait_warp(&S.k_full[st2], ((u + 2) / kStages) & 1, abort, p.err))) break;
                         tc_fence_after();
-                        scores(m, st1);
-                    } else {
-                        warp_commit(&S.o_full[m]);
-                        ++items[m];
+                        scores(m, st2);
                     }
                 }
                 if (!ok) break;
                 warp_commit(&S.v_empty[st]);
-                if (j + 1 < nt) warp_commit(&S.k_empty[st1]);
+                if (j + 2 < nt) warp_commit(&S.k_empty[st2]);
             }
         }
         // every MMA issued so far completes before TMEM is freed
         if (issued) {
             warp_commit(&S.drain);
-            __syncwarp();
             for (uint32_t n = 0; n < kMaxWaitProbes; ++n)
                 if (__all_sync(0xffffffffu, mbar_try_wait(&S.drain, 0))) break;
         }
@@ -559,23 +519,24 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     }
 }
 
-template <int DK, int DV, int KT>
+template <int DK, int DV>
 cudaError_t launch_dims(const AttendParams &p, int few, cudaStream_t s) {
     const int G = p.heads / p.c.heads, gq = G < 128 ? G : 128, tq = 128 / gq, hgroups = (G + gq - 1) / gq;
-    const size_t smem = sizeof(Shared<DK, DV, KT>) + 1024;
-    auto kernel = attend_prompt_kernel<DK, DV, KT>;
+    const size_t smem = sizeof(Shared<DK, DV>) + 1024;
+    auto kernel = attend_prompt_kernel<DK, DV>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)((p.T + 2 * tq - 1) / (2 * tq)), (unsigned)(p.c.heads * hgroups)),
-                      dim3(kThreads), smem, s, p, tq, gq, hgroups, few);
+    const int64_t windows = (p.T + 2 * tq - 1) / (2 * tq);
+    return launch_pdl(kernel, dim3((unsigned)(windows * p.c.heads * hgroups)), dim3(kThreads), smem, s, p, tq, gq, hgroups,
+                      few);
 }
 
 }  // namespace
 
 cudaError_t launch_attend_prompt(const AttendParams &p, int few, cudaStream_t s) {
-    if (p.c.k_dim == 64) return launch_dims<64, 64, 128>(p, few, s);
-    if (p.c.k_dim == 128) return launch_dims<128, 128, 128>(p, few, s);
-    return launch_dims<192, 128, 64>(p, few, s);   // q of two tiles takes 96 KB
+    if (p.c.k_dim == 64) return launch_dims<64, 64>(p, few, s);
+    if (p.c.k_dim == 128) return launch_dims<128, 128>(p, few, s);
+    return launch_dims<192, 128>(p, few, s);
 }
 
 }  // namespace qmoe
