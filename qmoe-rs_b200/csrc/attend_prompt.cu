@@ -10,18 +10,19 @@
 //   warps 0-3, 4-7   one row of a query tile a thread: q to fp16 in shared
 //                    memory, then per key tile the scores from tensor memory,
 //                    the running maximum and sum, P back to tensor memory
-//   warps 8-11       K: codes from the cache to fp16 operands in shared memory
-//                    ([token][dim], 128-byte swizzle), a group of 16 tokens a
-//                    warp, and the groups' scales
-//   warps 12-15      V likewise ([dim][token])
-//   warp 16          tcgen05: S = q K^T (both operands in shared memory), then
+//   warps 8-14       codes from the cache to fp16 operands in shared memory (K
+//                    [token][dim], V [dim][token], 128-byte swizzle) and the
+//                    scales; the eight 16-token groups of K and V of a tile go
+//                    round the seven warps
+//   warp 15          tcgen05: S = q K^T (both operands in shared memory), then
 //                    O += P V (P from tensor memory)
 //
 // Tensor memory holds two score tiles and O of each query tile.  The scores of
 // a tile are asked for two tiles ahead, so a softmax waits for no MMA, and the
-// two query tiles' softmaxes run side by side.  O is rescaled only where a row's
-// maximum has grown by more than 2^8 since it was last scaled; until then P may
-// reach 2^(8 + 6), which fp16 holds.  For 256 rows by 128 keys of 128 dims the
+// two query tiles' softmaxes run side by side.  O is scaled to a maximum that a
+// row's own may outgrow by 2^8: P is made with it before the tile's maximum is
+// known and made again, with O rescaled, only where that was too small (P then
+// reaches 2^(8 + 6), which fp16 holds).  For 256 rows by 128 keys of 128 dims the
 // exponentials take 2048 cycles of an SM (16 a cycle) and the MMAs as many.
 #include "attend.cuh"
 #include "kernels.h"
@@ -32,12 +33,12 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kSoftWarps = 8, kVWarp0 = 12, kMmaWarp = 16;
-constexpr int kThreads = 17 * 32;
-constexpr int KT = 64;                        // keys a tile: a group of 16 for each K and V warp
+constexpr int kSoftWarps = 8, kCodeWarps = 7, kMmaWarp = 15;
+constexpr int kThreads = 16 * 32;
+constexpr int KT = 64;                        // keys a tile
 constexpr float kGrow = 8.0f;                 // log2 of how far a maximum may outgrow the scaling
 constexpr float kShift = 6.0f;                // P = 2^6 at the scaling's maximum
-// Tiles whose scales are kept.  A K warp writes those of tile u once the scores
+// Tiles whose scales are kept.  Those of tile u are written once the scores
 // of tile u - stages are done; these were asked for after P of tile u - stages -
 // 2, so the softmax is done with the slot's tile u - 8.
 constexpr int kScaleRing = 8;
@@ -62,6 +63,14 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
     return (1u << 4)          // D = f32; A, B = f16 (format 0)
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+
+// Four bf16; `vec`: the address is a multiple of 8.
+QMOE_DEV uint2 load_bf16x4(const uint16_t *at, bool vec) {
+    if (vec) return __ldg(reinterpret_cast<const uint2 *>(at));
+    return make_uint2(at[0] | (uint32_t)at[1] << 16, at[2] | (uint32_t)at[3] << 16);
+}
+QMOE_DEV float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
+QMOE_DEV float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 QMOE_DEV uint4 ldg_code(const int8_t *at) { return __ldg(reinterpret_cast<const uint4 *>(at)); }
 
@@ -227,7 +236,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             constexpr int kRep = (DK + 127) / 128, kAtOnce = 8 / kRep;
 #pragma unroll 1
             for (int x = 0; x < 32; x += kAtOnce) {
-                float4 v[kAtOnce][kRep];
+                uint2 raw[kAtOnce][kRep];                                    // all in flight at once
                 const int64_t mine = live ? tok * p.ldq + (int64_t)(head0 + gg) * DK : -1;
 #pragma unroll
                 for (int y = 0; y < kAtOnce; ++y) {
@@ -235,7 +244,9 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
 #pragma unroll
                     for (int z = 0; z < kRep; ++z) {
                         const int d = 4 * lane + 128 * z;
-                        v[y][z] = at >= 0 && d < DK ? load_q4(p, at + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        const bool some = at >= 0 && d < DK;
+                        raw[y][z] = load_bf16x4(reinterpret_cast<const uint16_t *>(p.q) + (some ? at + d : 0), p.vec_q);
+                        if (!some) raw[y][z] = make_uint2(0, 0);
                     }
                 }
 #pragma unroll
@@ -243,7 +254,8 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     float mx = 0.0f;
 #pragma unroll
                     for (int z = 0; z < kRep; ++z)
-                        mx = max_abs(max_abs(max_abs(max_abs(mx, v[y][z].x), v[y][z].y), v[y][z].z), v[y][z].w);
+                        mx = max_abs(max_abs(max_abs(max_abs(mx, bf_lo(raw[y][z].x)), bf_hi(raw[y][z].x)), bf_lo(raw[y][z].y)),
+                                     bf_hi(raw[y][z].y));
                     const int e = q_exponent(warp_max(mx)), at = q * 32 + x + y;
                     const float up = sign * pow2i(14 - e);
                     if (lane == x + y) back = pow2i(e - 14);
@@ -253,7 +265,8 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                         if (d < DK)
                             *reinterpret_cast<uint2 *>(S.q[m] + (d >> 6) * (128 * 128) + at * 128 +
                                                        ((((d >> 3) & 7) ^ (at & 7)) << 4) + 2 * (d & 4)) =
-                                make_uint2(h2(v[y][z].x * up, v[y][z].y * up), h2(v[y][z].z * up, v[y][z].w * up));
+                                make_uint2(h2(bf_lo(raw[y][z].x) * up, bf_hi(raw[y][z].x) * up),
+                                           h2(bf_lo(raw[y][z].y) * up, bf_hi(raw[y][z].y) * up));
                     }
                 }
             }
@@ -271,13 +284,14 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 uint32_t t[2][32];
                 tmem_ld_x32(at, t[0]);
                 tmem_ld_x32(at + 32, t[1]);
-                // the groups' factors: a > 0, so that a masked score of -inf stays one and
-                // the largest score is the largest t (a poisoned group's NaN is in lv)
-                float a[4], b[4];
+                // the groups' factors: a > 0, so that a masked score of -inf stays one (a
+                // poisoned group's NaN is in lv)
+                float a[4], b[4], iv[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     a[x] = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
                     b[x] = S.lv[u % kScaleRing][x];
+                    iv[x] = S.iv[u % kScaleRing][x];
                 }
                 const int see = last - j * KT;                               // columns 0 .. see are visible
                 const bool whole = j * KT + KT - 1 <= first_last && j * KT + KT <= it.keys;
@@ -287,21 +301,42 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     for (int x = 0; x < 64; ++x)
                         if (x > see) t[x >> 5][x & 31] = 0xff800000u;        // -inf
                 }
-                float top = neg_inf();
+                uint32_t w[2][16];
+                // P, its sum, and the largest exponent of the tile over `base`
+                auto exponentials = [&](float base, float &top) {
+                    float part[4], m0 = neg_inf(), m1 = neg_inf();
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float g0 = neg_inf(), g1 = neg_inf();
+                    for (int x = 0; x < 4; ++x) {
+                        const float gb = b[x] - base;
+                        float p0 = 0.0f, p1 = 0.0f;
 #pragma unroll
-                    for (int y = 0; y < 16; y += 2) {
-                        g0 = fmaxf(g0, __uint_as_float(t[x >> 1][16 * (x & 1) + y]));
-                        g1 = fmaxf(g1, __uint_as_float(t[x >> 1][16 * (x & 1) + y + 1]));
+                        for (int y = 0; y < 16; y += 2) {
+                            const int z = 16 * (x & 1) + y;
+                            const float t0 = __fmaf_rn(__uint_as_float(t[x >> 1][z]), a[x], gb);
+                            const float t1 = __fmaf_rn(__uint_as_float(t[x >> 1][z + 1]), a[x], gb);
+                            m0 = fmaxf(m0, t0);
+                            m1 = fmaxf(m1, t1);
+                            const float e0 = ex2(t0), e1 = ex2(t1);
+                            p0 += e0;
+                            p1 += e1;
+                            w[x >> 1][z / 2] = h2(e0, e1);
+                        }
+                        part[x] = p0 + p1;
                     }
-                    top = fmaxf(top, __fmaf_rn(fmaxf(g0, g1), a[x], b[x]));
-                }
-                if (__any_sync(0xffffffffu, top > mx + kGrow)) {             // also the first tile: mx is -inf
-                    const float to = top > mx ? top : mx;
-                    const float by = to == neg_inf() ? 1.0f : ex2(mx - to);
-                    mx = to;
+                    top = fmaxf(m0, m1);
+                    float total = 0.0f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) total = __fmaf_rn(part[x], iv[x], total);
+                    return total;
+                };
+                float top, add = exponentials(mx == neg_inf() ? 0.0f : mx - kShift, top);
+                // too small a scaling; the first tile's is none at all
+                const bool grow = mx == neg_inf() ? top != neg_inf() : top > kGrow + kShift;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float to = top + (mx == neg_inf() ? 0.0f : mx - kShift);   // the tile's largest
+                    const float now = to > mx ? to : mx;
+                    const float by = now == neg_inf() ? 1.0f : ex2(mx - now);
+                    mx = now;
                     sum *= by;
                     if (j > 0) {                                             // O is the last tile's product's until it is done
                         if (!(ok = mbar_wait_warp(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
@@ -316,26 +351,11 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                             tmem_st_x16(o_at + c, o);
                         }
                     }
+                    add = exponentials(mx == neg_inf() ? 0.0f : mx - kShift, top);
                 }
-                const float base = mx == neg_inf() ? 0.0f : mx - kShift;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float ga = a[2 * c + half], gb = b[2 * c + half] - base;
-                        float part = 0.0f;
-#pragma unroll
-                        for (int x = 16 * half; x < 16 * half + 16; x += 2) {
-                            const float t0 = ex2(__fmaf_rn(__uint_as_float(t[c][x]), ga, gb));
-                            const float t1 = ex2(__fmaf_rn(__uint_as_float(t[c][x + 1]), ga, gb));
-                            part += t0 + t1;
-                            w[x / 2] = h2(t0, t1);
-                        }
-                        sum = __fmaf_rn(part, S.iv[u % kScaleRing][2 * c + half], sum);
-                    }
-                    tmem_st_x16(at + 16 * c, w);
-                }
+                sum += add;
+                tmem_st_x16(at, w[0]);
+                tmem_st_x16(at + 16, w[1]);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -378,25 +398,29 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         }
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------- codes to operands
-        // A warp has one group of 16 tokens of each tile, of K (loads of 8 tokens by 64
-        // dims) or V (32 dims).  The next tile's codes are loaded while this one's wait
-        // for their stage; blocks are looked up two tiles ahead.
-        const bool is_v = warp >= kVWarp0;
-        const int grp = warp & 3, g = lane >> 2, c = lane & 3, bs = p.c.block;
+        // Unit 8 u + x is group x of K (x < 4; loads of 8 tokens by 64 dims) or x - 4 of V
+        // (32 dims) of tile u.  The codes of a warp's next unit are loaded while this
+        // one's wait for their stage; blocks are looked up two units ahead.
+        const int g = lane >> 2, c = lane & 3, bs = p.c.block;
         constexpr int kKLoads = 2 * (DK / 64), kVLoads = DV / 32, kLoads = kKLoads > kVLoads ? kKLoads : kVLoads;
-        uint32_t u = 0;
+        uint32_t first = 0;                           // unit of the item's first tile
+        uint32_t unit = warp - kSoftWarps;            // this warp's next
         while (ok && next_item(p, lo, span, few, r, it)) {
             const int nt = (it.keys + KT - 1) / KT;
+            const uint32_t end = first + 8 * nt;
             const int32_t *table = p.table + it.request * p.max_blocks;
-            auto block_of = [&](int j) -> int64_t {
-                const int tok = j * KT + grp * 16;
-                if (tok >= it.keys) return -1;
+            auto token_of = [&](uint32_t x) { return (int)((x - first) >> 3) * KT + (int)(x & 3) * 16; };
+            auto block_of = [&](uint32_t x) -> int64_t {
+                const int tok = token_of(x);
+                if (x >= end || tok >= it.keys) return -1;
                 const int64_t b = table[block_index(p, tok)];
                 return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
             };
             uint4 codes[kLoads];
-            auto load = [&](int j, int64_t bh) {
-                const int tok = j * KT + grp * 16, off = tok - block_index(p, tok) * bs;
+            float kr = 0.0f, vr = -1.0f;              // ranges of a K unit's group; vr -1: no group
+            auto load = [&](uint32_t x, int64_t bh) {
+                const bool is_v = x & 4;
+                const int tok = token_of(x), off = tok - block_index(p, tok) * bs;
                 const int8_t *at = is_v ? p.c.v + ((bh * (bs / 16) + off / 16) * DV + lane) * 16
                                         : p.c.k + (bh * (DK / 64) * bs + off + g) * 64 + c * 16;
 #pragma unroll
@@ -404,21 +428,15 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     const int step = is_v ? y * 512 : (y >> 1) * bs * 64 + (y & 1) * 512;
                     codes[y] = bh >= 0 && y < (is_v ? kVLoads : kKLoads) ? ldg_code(at + step) : make_uint4(0, 0, 0, 0);
                 }
+                kr = bh >= 0 && !is_v ? p.c.k_range[bh] : 0.0f;
+                vr = bh >= 0 && !is_v ? p.c.v_range[bh] : -1.0f;
             };
-            int64_t b1 = block_of(1);
-            float kr = 0.0f, vr = -1.0f;              // of the group; vr -1: none
-            auto load_ranges = [&](int64_t bh) {
-                kr = bh >= 0 ? p.c.k_range[bh] : 0.0f;
-                vr = bh >= 0 ? p.c.v_range[bh] : -1.0f;
-            };
-            if (nt > 0) {
-                const int64_t b0 = block_of(0);
-                load(0, b0);
-                if (!is_v) load_ranges(b0);
-            }
-            for (int j = 0; j < nt; ++j, ++u) {
-                const uint32_t st = u % kStages, phase = (u / kStages) & 1;
-                const int64_t b2 = block_of(j + 2);
+            if (unit < end) load(unit, block_of(unit));
+            int64_t b1 = block_of(unit + kCodeWarps);
+            for (; unit < end; unit += kCodeWarps) {
+                const bool is_v = unit & 4;
+                const uint32_t u = unit >> 3, st = u % kStages, phase = (u / kStages) & 1, grp = unit & 3;
+                const int64_t b2 = block_of(unit + 2 * kCodeWarps);
                 if (!(ok = mbar_wait_warp(is_v ? &S.v_empty[st] : &S.k_empty[st], phase ^ 1, abort, p.err))) break;
                 if (is_v) {
 #pragma unroll
@@ -438,12 +456,10 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(is_v ? &S.v_full[st] : &S.k_full[st]);
-                if (j + 1 < nt) {
-                    load(j + 1, b1);
-                    if (!is_v) load_ranges(b1);
-                }
+                if (unit + kCodeWarps < end) load(unit + kCodeWarps, b1);
                 b1 = b2;
             }
+            first = end;
         }
     } else {
         // ---------------------------------------------------------- MMA
