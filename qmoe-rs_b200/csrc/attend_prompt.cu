@@ -11,7 +11,8 @@
 //                    memory, then per key tile the scores from tensor memory,
 //                    the running maximum and sum, P back to tensor memory
 //   warps 8-14       codes from the cache to fp16 operands in shared memory (K
-//                    [token][dim], V [dim][token], 128-byte swizzle) and the
+//                    [token][dim] as 1152 + c, whose 1152 sum q goes into the
+//                    row's constant; V [dim][token]; 128-byte swizzle) and the
 //                    scales; the eight 16-token groups of K and V of a tile go
 //                    round the seven warps
 //   warp 15          tcgen05: S = q K^T (both operands in shared memory), then
@@ -72,17 +73,48 @@ QMOE_DEV uint2 load_bf16x4(const uint16_t *at, bool vec) {
 QMOE_DEV float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
 QMOE_DEV float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// Pairs of f32 in one instruction each, every half rounded as the single form.
+QMOE_DEV uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+QMOE_DEV void unpair(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+QMOE_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+QMOE_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+QMOE_DEV float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 QMOE_DEV uint4 ldg_code(const int8_t *at) { return __ldg(reinterpret_cast<const uint4 *>(at)); }
 
-// Sixteen codes as fp16 to units `unit` and unit + 1 (16 bytes each) of row r of
+// Sixteen codes c as fp16, or (BIASED) 1152 + c, to units `unit` and unit + 1 (16 bytes each) of row r of
 // a 128-byte swizzled operand.  A quarter warp's units are distinct banks: two
 // rows of four even units (K), or eight rows of one (V).
+template <bool BIASED>
 QMOE_DEV void store_codes(uint8_t *row, int unit, int r, const uint4 &v) {
     uint4 a, b;
-    codes_to_half(v.x, a.x, a.y);
-    codes_to_half(v.y, a.z, a.w);
-    codes_to_half(v.z, b.x, b.y);
-    codes_to_half(v.w, b.z, b.w);
+    if (BIASED) {
+        codes_biased(v.x, a.x, a.y);
+        codes_biased(v.y, a.z, a.w);
+        codes_biased(v.z, b.x, b.y);
+        codes_biased(v.w, b.z, b.w);
+    } else {
+        codes_to_half(v.x, a.x, a.y);
+        codes_to_half(v.y, a.z, a.w);
+        codes_to_half(v.z, b.x, b.y);
+        codes_to_half(v.w, b.z, b.w);
+    }
     *reinterpret_cast<uint4 *>(row + ((unit ^ (r & 7)) << 4)) = a;
     *reinterpret_cast<uint4 *>(row + (((unit + 1) ^ (r & 7)) << 4)) = b;
 }
@@ -232,7 +264,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             }
             // q: rows by a power of two (and the scale's sign), as fp16, 64 dims a
             // 128-byte row; some of the warp's rows at a time, four dims a lane
-            float back = 0.0f;
+            float back = 0.0f, bias = 0.0f;                                  // bias: -1152 times the row's sum
             constexpr int kRep = (DK + 127) / 128, kAtOnce = 8 / kRep;
 #pragma unroll 1
             for (int x = 0; x < 32; x += kAtOnce) {
@@ -258,15 +290,22 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                                      bf_hi(raw[y][z].y));
                     const int e = q_exponent(warp_max(mx)), at = q * 32 + x + y;
                     const float up = sign * pow2i(14 - e);
-                    if (lane == x + y) back = pow2i(e - 14);
+                    float sum = 0.0f;
 #pragma unroll
                     for (int z = 0; z < kRep; ++z) {
                         const int d = 4 * lane + 128 * z;
+                        const uint2 f = make_uint2(h2(bf_lo(raw[y][z].x) * up, bf_hi(raw[y][z].x) * up),
+                                                   h2(bf_lo(raw[y][z].y) * up, bf_hi(raw[y][z].y) * up));
+                        sum += (h_lo(f.x) + h_hi(f.x)) + (h_lo(f.y) + h_hi(f.y));
                         if (d < DK)
                             *reinterpret_cast<uint2 *>(S.q[m] + (d >> 6) * (128 * 128) + at * 128 +
-                                                       ((((d >> 3) & 7) ^ (at & 7)) << 4) + 2 * (d & 4)) =
-                                make_uint2(h2(bf_lo(raw[y][z].x) * up, bf_hi(raw[y][z].x) * up),
-                                           h2(bf_lo(raw[y][z].y) * up, bf_hi(raw[y][z].y) * up));
+                                                       ((((d >> 3) & 7) ^ (at & 7)) << 4) + 2 * (d & 4)) = f;
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == x + y) {
+                        back = pow2i(e - 14);
+                        bias = -1152.0f * sum;
                     }
                 }
             }
@@ -279,54 +318,50 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             float mx = neg_inf(), sum = 0.0f;                                // mx: what O and sum are scaled to
             for (int j = 0; j < nt; ++j, ++u, ++n) {
                 const uint32_t at = s_at + 64 * (n & 1);
-                if (!(ok = mbar_wait_warp(&S.s_full[m][n & 1], (n >> 1) & 1, abort, p.err))) break;
+                if (!(ok = wait_long(&S.s_full[m][n & 1], (n >> 1) & 1, abort, p.err))) break;
                 tc_fence_after();
-                uint32_t t[2][32];
-                tmem_ld_x32(at, t[0]);
-                tmem_ld_x32(at + 32, t[1]);
-                // the groups' factors: a > 0, so that a masked score of -inf stays one (a
-                // poisoned group's NaN is in lv)
-                float a[4], b[4], iv[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    a[x] = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
-                    b[x] = S.lv[u % kScaleRing][x];
-                    iv[x] = S.iv[u % kScaleRing][x];
-                }
                 const int see = last - j * KT;                               // columns 0 .. see are visible
                 const bool whole = j * KT + KT - 1 <= first_last && j * KT + KT <= it.keys;
-                tmem_wait_ld();
-                if (!whole) {
+                uint32_t t[2][32];                                           // scores; dead once P is made
+                auto load_scores = [&] {
+                    tmem_ld_x32(at, t[0]);
+                    tmem_ld_x32(at + 32, t[1]);
+                    tmem_wait_ld();
+                    if (!whole) {
 #pragma unroll
-                    for (int x = 0; x < 64; ++x)
-                        if (x > see) t[x >> 5][x & 31] = 0xff800000u;        // -inf
-                }
+                        for (int x = 0; x < 64; ++x)
+                            if (x > see) t[x >> 5][x & 31] = 0xff800000u;    // -inf
+                    }
+                };
+                load_scores();
                 uint32_t w[2][16];
                 // P, its sum, and the largest exponent of the tile over `base`
                 auto exponentials = [&](float base, float &top) {
-                    float part[4], m0 = neg_inf(), m1 = neg_inf();
+                    float total = 0.0f, m4[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const float gb = b[x] - base;
-                        float p0 = 0.0f, p1 = 0.0f;
+                        // the group's factors: a > 0, so that a masked score of -inf stays one (a
+                        // poisoned group's NaN is in lv); b takes the 1152 off the codes
+                        const float a = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
+                        const float b = __fmaf_rn(bias, a, S.lv[u % kScaleRing][x]) - base;
+                        const uint64_t aa = pair(a, a), bb = pair(b, b);
+                        uint64_t acc = pair(0.0f, 0.0f);
+                        m4[x] = neg_inf();
 #pragma unroll
                         for (int y = 0; y < 16; y += 2) {
                             const int z = 16 * (x & 1) + y;
-                            const float t0 = __fmaf_rn(__uint_as_float(t[x >> 1][z]), a[x], gb);
-                            const float t1 = __fmaf_rn(__uint_as_float(t[x >> 1][z + 1]), a[x], gb);
-                            m0 = fmaxf(m0, t0);
-                            m1 = fmaxf(m1, t1);
+                            float t0, t1;
+                            unpair(fma2(pair(__uint_as_float(t[x >> 1][z]), __uint_as_float(t[x >> 1][z + 1])), aa, bb), t0, t1);
+                            m4[x] = max3(m4[x], t0, t1);
                             const float e0 = ex2(t0), e1 = ex2(t1);
-                            p0 += e0;
-                            p1 += e1;
+                            acc = add2(acc, pair(e0, e1));
                             w[x >> 1][z / 2] = h2(e0, e1);
                         }
-                        part[x] = p0 + p1;
+                        float p0, p1;
+                        unpair(acc, p0, p1);
+                        total = __fmaf_rn(p0 + p1, S.iv[u % kScaleRing][x], total);
                     }
-                    top = fmaxf(m0, m1);
-                    float total = 0.0f;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) total = __fmaf_rn(part[x], iv[x], total);
+                    top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
                     return total;
                 };
                 float top, add = exponentials(mx == neg_inf() ? 0.0f : mx - kShift, top);
@@ -339,7 +374,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     mx = now;
                     sum *= by;
                     if (j > 0) {                                             // O is the last tile's product's until it is done
-                        if (!(ok = mbar_wait_warp(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
+                        if (!(ok = wait_long(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DV; c += 16) {
@@ -351,6 +386,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                             tmem_st_x16(o_at + c, o);
                         }
                     }
+                    load_scores();
                     add = exponentials(mx == neg_inf() ? 0.0f : mx - kShift, top);
                 }
                 sum += add;
@@ -362,7 +398,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 if (lane == 0) mbar_arrive(&S.p_full[m][n & 1]);
             }
             if (!ok) break;
-            if (!(ok = mbar_wait_warp(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
+            if (!(ok = wait_long(&S.pv_done[m][(n - 1) & 1], ((n - 1) >> 1) & 1, abort, p.err))) break;
             tc_fence_after();
             const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
             const bool wide = p.vec_out;
@@ -437,15 +473,15 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                 const bool is_v = unit & 4;
                 const uint32_t u = unit >> 3, st = u % kStages, phase = (u / kStages) & 1, grp = unit & 3;
                 const int64_t b2 = block_of(unit + 2 * kCodeWarps);
-                if (!(ok = mbar_wait_warp(is_v ? &S.v_empty[st] : &S.k_empty[st], phase ^ 1, abort, p.err))) break;
+                if (!(ok = wait_long(is_v ? &S.v_empty[st] : &S.k_empty[st], phase ^ 1, abort, p.err))) break;
                 if (is_v) {
 #pragma unroll
                     for (int y = 0; y < kVLoads; ++y)
-                        store_codes(S.v[st] + (32 * y + lane) * 128, 2 * grp, lane, codes[y]);
+                        store_codes<false>(S.v[st] + (32 * y + lane) * 128, 2 * grp, lane, codes[y]);
                 } else {
 #pragma unroll
                     for (int y = 0; y < kKLoads; ++y)
-                        store_codes(S.k[st] + (y >> 1) * (KT * 128) + (grp * 16 + (y & 1) * 8 + g) * 128, 2 * c, g, codes[y]);
+                        store_codes<true>(S.k[st] + (y >> 1) * (KT * 128) + (grp * 16 + (y & 1) * 8 + g) * 128, 2 * c, g, codes[y]);
                     if (lane == 0) {
                         const float v1 = vr < kRangeFloor ? kRangeFloor : vr;
                         S.f[u % kScaleRing][grp] = __fdiv_rn(kr, 127.0f);
@@ -486,9 +522,9 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             const int both = it.cnt > tq ? 2 : 1;                  // query tiles with tokens
             for (int j = 0; j < 2 && j < nt && ok; ++j) {          // the first two tiles' scores
                 const uint32_t st = (u + j) % kStages;
-                if (!(ok = mbar_wait_warp(&S.k_full[st], ((u + j) / kStages) & 1, abort, p.err))) break;
+                if (!(ok = wait_long(&S.k_full[st], ((u + j) / kStages) & 1, abort, p.err))) break;
                 for (int m = 0; m < both && ok; ++m) {
-                    if (j == 0 && !(ok = mbar_wait_warp(&S.q_full[m], items[m]++ & 1, abort, p.err))) break;
+                    if (j == 0 && !(ok = wait_long(&S.q_full[m], items[m]++ & 1, abort, p.err))) break;
                     tc_fence_after();
                     scores(m, st);
                 }
@@ -496,10 +532,10 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             }
             for (int j = 0; j < nt && ok; ++j, ++u) {
                 const uint32_t st = u % kStages, st2 = (u + 2) % kStages;
-                if (!(ok = mbar_wait_warp(&S.v_full[st], (u / kStages) & 1, abort, p.err))) break;
+                if (!(ok = wait_long(&S.v_full[st], (u / kStages) & 1, abort, p.err))) break;
                 for (int m = 0; m < both; ++m) {
                     const uint32_t b = used[m] & 1;
-                    if (!(ok = mbar_wait_warp(&S.p_full[m][b], (used[m] >> 1) & 1, abort, p.err))) break;
+                    if (!(ok = wait_long(&S.p_full[m][b], (used[m] >> 1) & 1, abort, p.err))) break;
                     ++used[m];
                     tc_fence_after();
                     const uint32_t d = tmem + kOCol + m * 128, pa = tmem + m * 128 + 64 * b, va = v_lo + st * (Sm::kV >> 4);
@@ -509,7 +545,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                     warp_commit(&S.pv_done[m][b]);
                     issued = true;
                     if (j + 2 < nt) {                              // in order after P V: its buffer is free
-                        if (m == 0 && !(ok = mbar_wait_warp(&S.k_full[st2], ((u + 2) / kStages) & 1, abort, p.err))) break;
+                        if (m == 0 && !(ok = wait_long(&S.k_full[st2], ((u + 2) / kStages) & 1, abort, p.err))) break;
                         tc_fence_after();
                         scores(m, st2);
                     }

@@ -10,6 +10,27 @@
 namespace qmoe {
 namespace sm100 {
 
+// mbar_wait_warp whose probes suspend for up to two microseconds each: warps
+// that wait for long leave the issue slots to the others.
+QMOE_DEV bool wait_long(uint64_t *bar, uint32_t parity, volatile int *abort, int *err) {
+    for (uint32_t n = 0; n < kMaxWaitProbes; ++n) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+            : "memory");
+        if (__all_sync(0xffffffffu, done)) return true;
+        if (__any_sync(0xffffffffu, *abort != 0)) return false;
+    }
+    if ((threadIdx.x & 31) == 0) {
+        *abort = 1;
+        atomicOr(err, kErrWaitTimeout);
+    }
+    __syncwarp();
+    return false;
+}
+
 #define QMOE_MMA_WARP(kind, a_decl, a_op)                                                           \
     "{\n .reg .pred p, e;\n .reg .b64 ad, bd;\n setp.ne.b32 p, %5, 0;\n elect.sync _|e, 0xffffffff;\n" \
     a_decl " mov.b64 bd, {%2, %3};\n"                                                              \
