@@ -19,12 +19,19 @@ namespace qmoe {
 
 constexpr float kRangeFloor = 127.0f * 5.42101086242752217e-20f;   // a scale of 2^-64
 
+// Out of line: rare, and an f64 division at every use would fill the
+// instruction cache (64 single tokens' append took 23 us with it inlined, see
+// kv.cu).
+static __device__ __noinline__ int code8_exact(float a, float m, float r) {
+    return (int)rint((double)a * (double)m / (double)r);
+}
+
 // a * m / r as a code, |a * m| <= 127 r; mi = m / r in f32.
 QMOE_DEV int code8(float a, float m, float r, float mi) {
     const float q = __fmul_rn(a, mi);
     const float c = rintf(q);
     if (fabsf(fabsf(__fsub_rn(q, c)) - 0.5f) < 6.103515625e-05f)
-        return (int)rint((double)a * (double)m / (double)r);
+        return code8_exact(a, m, r);
     return (int)c;                                                 // NaN gives 0
 }
 

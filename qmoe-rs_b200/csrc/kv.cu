@@ -135,12 +135,19 @@ __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const KvPlanParam
 
 // ---- append --------------------------------------------------------------------
 //
-// One warp per (token, head) whose token starts a run: consecutive slots of
-// one block.  Offsets before the run are the block's earlier tokens.  The
-// range grows to the new tokens' largest magnitude, the earlier codes are
-// rounded to the new range (kept when it did not grow), the new ones written.
+// A run is a sequence of rows with consecutive slots of one block; offsets
+// before it are the block's earlier tokens.  The range grows to the new tokens'
+// largest magnitude, the earlier codes are rounded to the new range (left alone
+// when it did not grow), the new ones written.
+//
+// One warp a run, head and side (K or V).  It reads its rows twice, the second
+// time from L1 or L2: bound by HBM for prompts (two prompts of 4099 tokens, 16
+// heads of 192 and 128, f32: 210 MB) and by the latency of that chain of loads
+// for single tokens.  A warp looks for runs that start among `span` rows, one
+// row where rows are few.
 
 constexpr int kAppendWarps = 8;
+constexpr int kAhead = 8;                          // loads in flight a lane
 
 template <bool BF16>
 QMOE_DEV float4 load4(const void *x, int64_t i, bool vec) {
@@ -153,90 +160,204 @@ QMOE_DEV float4 load4(const void *x, int64_t i, bool vec) {
     return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// Place of (token, dim) among the codes of one block and head, from the first
-// of four dims; V steps 16 bytes a dim, K one.
-template <bool IS_V>
-QMOE_DEV int code_at(int tok, int d, int dim, int block) {
-    return IS_V ? ((tok >> 4) * dim + d) * 16 + (tok & 15) : ((d >> 6) * block + tok) * 64 + (d & 63);
+template <bool BF16>
+QMOE_DEV float load1(const void *x, int64_t i) {
+    return BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(x)[i])
+                : __ldg(reinterpret_cast<const float *>(x) + i);
 }
 
-template <bool BF16, bool IS_V>
-QMOE_DEV void append_run(const void *x, int64_t ld, int dim, bool vec, int8_t *codes, float *range, int head,
-                         int64_t t, int n, int off, int block) {
+// The largest magnitude of `n` rows of DIM elements from x[at], ld apart; bad:
+// an element is not finite.
+template <bool BF16, int DIM>
+QMOE_DEV float rows_max(const void *x, int64_t at, int64_t ld, int n, bool vec, bool &bad) {
+    constexpr int kPer = DIM / 4;                  // groups of four elements in a row
     const int lane = threadIdx.x & 31;
     float m = 0.0f;
-    bool bad = false;
-    const int per = dim / 4;                       // groups of four dims in a row
-    for (int e = lane; e < n * per; e += 32) {
-        const int i = e / per, d = (e - i * per) * 4;
-        const float4 v = load4<BF16>(x, (t + i) * ld + (int64_t)head * dim + d, vec);
-        m = max_abs(max_abs(max_abs(max_abs(m, v.x), v.y), v.z), v.w);
-        const float inf = __int_as_float(0x7f800000);
-        bad |= !(fabsf(v.x) < inf && fabsf(v.y) < inf && fabsf(v.z) < inf && fabsf(v.w) < inf);
+    bool odd = false;
+    for (int e0 = 0; e0 < n * kPer; e0 += 32 * kAhead) {
+        float4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int e = e0 + 32 * k + lane, i = e / kPer;
+            v[k] = e < n * kPer ? load4<BF16>(x, at + i * ld + (e - i * kPer) * 4, vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            m = max_abs(max_abs(max_abs(max_abs(m, v[k].x), v[k].y), v[k].z), v[k].w);
+            const float inf = __int_as_float(0x7f800000);
+            odd |= !(fabsf(v[k].x) < inf && fabsf(v[k].y) < inf && fabsf(v[k].z) < inf && fabsf(v[k].w) < inf);
+        }
     }
-    m = warp_max(m);
-    bad = __any_sync(0xffffffffu, bad);
+    bad = __any_sync(0xffffffffu, odd);
+    return warp_max(m);
+}
+
+// Byte j of four codes, the value c in its place.
+QMOE_DEV uint32_t put_byte(uint32_t w, int j, int c) {
+    const int sh = 8 * j;
+    return (w & ~(255u << sh)) | (uint32_t)(c & 255) << sh;
+}
+QMOE_DEV int get_byte(uint32_t w, int j) { return (int)(int8_t)(w >> (8 * j)); }
+
+// Rows t .. t + n - 1 to offsets off .. of a block, one head.
+template <bool BF16, int DIM>
+QMOE_DEV void append_k(const KvAppendParams &p, int8_t *codes, float *range, int64_t at, int n, int off) {
+    constexpr int kPer = DIM / 4;
+    const int lane = threadIdx.x & 31, bs = p.c.block;
     const float old = off > 0 ? *range : 0.0f;
+    bool bad;
+    const float m = rows_max<BF16, DIM>(p.k, at, p.ldk, n, p.vec_k, bad);
     bad |= !(fabsf(old) < __int_as_float(0x7f800000));
     const float r = range8(fmaxf(m, old), !bad), mi = __fdiv_rn(127.0f, r);
     __syncwarp();
     if (lane == 0) *range = r;
+    auto place = [&](int tok, int d) { return reinterpret_cast<uint32_t *>(codes + ((d >> 6) * bs + tok) * 64 + (d & 63)); };
     if (off > 0 && !(r == old)) {
         const float oi = __fdiv_rn(old, r);
-        for (int e = lane; e < off * per; e += 32) {
-            const int i = e / per, d = (e - i * per) * 4;
+        for (int e0 = 0; e0 < off * kPer; e0 += 32 * kAhead) {
+            uint32_t w[kAhead];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                int8_t *c = codes + code_at<IS_V>(i, d + j, dim, block);
-                *c = (int8_t)code8((float)*c, old, r, oi);
+            for (int k = 0; k < kAhead; ++k) {
+                const int e = e0 + 32 * k + lane, i = e / kPer;
+                w[k] = e < off * kPer ? *place(i, (e - i * kPer) * 4) : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int e = e0 + 32 * k + lane, i = e / kPer;
+                if (e >= off * kPer) continue;
+                *place(i, (e - i * kPer) * 4) =
+                    pack4(code8((float)get_byte(w[k], 0), old, r, oi), code8((float)get_byte(w[k], 1), old, r, oi),
+                          code8((float)get_byte(w[k], 2), old, r, oi), code8((float)get_byte(w[k], 3), old, r, oi));
             }
         }
     }
-    for (int e = lane; e < n * per; e += 32) {
-        const int i = e / per, d = (e - i * per) * 4;
-        const float4 v = load4<BF16>(x, (t + i) * ld + (int64_t)head * dim + d, vec);
-        const int c0 = code8(v.x, 127.0f, r, mi), c1 = code8(v.y, 127.0f, r, mi);
-        const int c2 = code8(v.z, 127.0f, r, mi), c3 = code8(v.w, 127.0f, r, mi);
-        int8_t *c = codes + code_at<IS_V>(off + i, d, dim, block);
-        if (IS_V) {
-            c[0] = (int8_t)c0;
-            c[16] = (int8_t)c1;
-            c[32] = (int8_t)c2;
-            c[48] = (int8_t)c3;
-        } else {
-            *reinterpret_cast<uint32_t *>(c) = pack4(c0, c1, c2, c3);
+    for (int e0 = 0; e0 < n * kPer; e0 += 32 * kAhead) {
+        float4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int e = e0 + 32 * k + lane, i = e / kPer;
+            v[k] = e < n * kPer ? load4<BF16>(p.k, at + i * p.ldk + (e - i * kPer) * 4, p.vec_k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int e = e0 + 32 * k + lane, i = e / kPer;
+            if (e < n * kPer)
+                *place(off + i, (e - i * kPer) * 4) = pack4(code8(v[k].x, 127.0f, r, mi), code8(v[k].y, 127.0f, r, mi),
+                                                            code8(v[k].z, 127.0f, r, mi), code8(v[k].w, 127.0f, r, mi));
         }
     }
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(const KvAppendParams p) {
+// V holds 16 tokens of a dim in 16 bytes: a lane has whole dims of a full
+// group, 16 loads (each a row's 128 bytes over the warp) and one 16-byte store;
+// the tokens of other groups go byte by byte.
+template <bool BF16, int DIM>
+QMOE_DEV void append_v(const KvAppendParams &p, int8_t *codes, float *range, int64_t at, int n, int off) {
+    const int lane = threadIdx.x & 31;
+    const float old = off > 0 ? *range : 0.0f;
+    bool bad;
+    const float m = rows_max<BF16, DIM>(p.v, at, p.ldv, n, p.vec_v, bad);
+    bad |= !(fabsf(old) < __int_as_float(0x7f800000));
+    const float r = range8(fmaxf(m, old), !bad), mi = __fdiv_rn(127.0f, r);
+    __syncwarp();
+    if (lane == 0) *range = r;
+    const bool moved = off > 0 && !(r == old);
+    const float oi = moved ? __fdiv_rn(old, r) : 0.0f;
+    constexpr int kPer = DIM / 4, kQ = DIM / 32;
+    if (moved)
+        for (int g = 0; 16 * g < off; ++g) {
+            uint4 w[kQ];
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) w[q] = *reinterpret_cast<const uint4 *>(codes + (g * DIM + 32 * q + lane) * 16);
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                uint32_t *words = reinterpret_cast<uint32_t *>(&w[q]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (16 * g + i < off)
+                        words[i >> 2] = put_byte(words[i >> 2], i & 3, code8((float)get_byte(words[i >> 2], i & 3), old, r, oi));
+                *reinterpret_cast<uint4 *>(codes + (g * DIM + 32 * q + lane) * 16) = w[q];
+            }
+        }
+    __syncwarp();
+    for (int i0 = 0; i0 < n;) {                    // tokens of one group at a time
+        const int tok = off + i0, g = tok >> 4, cnt = 16 - (tok & 15) < n - i0 ? 16 - (tok & 15) : n - i0;
+        if (cnt == 16) {
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                const int d = 32 * q + lane;
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = load1<BF16>(p.v, at + (i0 + i) * p.ldv + d);
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = pack4(code8(x[4 * i], 127.0f, r, mi), code8(x[4 * i + 1], 127.0f, r, mi),
+                                 code8(x[4 * i + 2], 127.0f, r, mi), code8(x[4 * i + 3], 127.0f, r, mi));
+                *reinterpret_cast<uint4 *>(codes + (g * DIM + d) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else {
+            for (int e = lane; e < cnt * kPer; e += 32) {
+                const int i = e / kPer, d = (e - i * kPer) * 4;
+                const float4 v = load4<BF16>(p.v, at + (i0 + i) * p.ldv + d, p.vec_v);
+                int8_t *c = codes + (g * DIM + d) * 16 + ((tok + i) & 15);
+                c[0] = (int8_t)code8(v.x, 127.0f, r, mi);
+                c[16] = (int8_t)code8(v.y, 127.0f, r, mi);
+                c[32] = (int8_t)code8(v.z, 127.0f, r, mi);
+                c[48] = (int8_t)code8(v.w, 127.0f, r, mi);
+            }
+        }
+        i0 += cnt;
+    }
+}
+
+template <bool BF16, int DK, int DV>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(const KvAppendParams p, int span) {
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
-    const int64_t t = w / p.c.heads;
-    const int h = (int)(w - t * p.c.heads);
-    if (t >= p.T) return;
+    const int side = (int)(w % (2 * p.c.heads)), h = side >> 1;
+    const int64_t t0 = w / (2 * p.c.heads) * span;
+    if (t0 >= p.T) return;
     const int64_t total = p.c.num_blocks * p.c.block;
-    const int slot = p.slots[t];
-    if (slot < 0 || slot >= total) return;
-    const int off = slot % p.c.block;
-    const int64_t blk = slot / p.c.block;
-    if (off > 0 && t > 0 && p.slots[t - 1] == slot - 1) return;   // inside another token's run
-    int n = 0;
-    for (int base = 0; base < p.c.block - off; base += 32) {
-        const int i = base + lane;
-        const bool in = off + i < p.c.block && t + i < p.T && p.slots[t + i] == slot + i;
-        const unsigned miss = ~__ballot_sync(0xffffffffu, in);
-        n += miss ? __ffs(miss) - 1 : 32;
-        if (miss) break;
+    const int bs = p.c.block;
+    // lane i: does a run start at row t0 + i?
+    const int64_t mine = t0 + lane;
+    int slot = -1;
+    bool starts = false;
+    if (lane < span && mine < p.T) {
+        slot = p.slots[mine];
+        starts = slot >= 0 && slot < total && !(slot % bs > 0 && mine > 0 && p.slots[mine - 1] == slot - 1);
     }
-    const int64_t bh = blk * p.c.heads + h;
-    append_run<BF16, false>(p.k, p.ldk, p.c.k_dim, p.vec_k, p.c.k + bh * p.c.block * p.c.k_dim, p.c.k_range + bh, h,
-                            t, n, off, p.c.block);
-    append_run<BF16, true>(p.v, p.ldv, p.c.v_dim, p.vec_v, p.c.v + bh * p.c.block * p.c.v_dim, p.c.v_range + bh, h,
-                           t, n, off, p.c.block);
+    for (unsigned left = __ballot_sync(0xffffffffu, starts); left; left &= left - 1) {
+        const int f = __ffs(left) - 1;
+        const int64_t t = t0 + f;
+        const int s = __shfl_sync(0xffffffffu, slot, f), off = s % bs;
+        const int64_t bh = (int64_t)(s / bs) * p.c.heads + h;
+        int n = 0;
+        for (int base = 0; base < bs - off; base += 32) {
+            const int i = base + lane;
+            const bool in = off + i < bs && t + i < p.T && p.slots[t + i] == s + i;
+            const unsigned miss = ~__ballot_sync(0xffffffffu, in);
+            n += miss ? __ffs(miss) - 1 : 32;
+            if (miss) break;
+        }
+        if (side & 1)
+            append_v<BF16, DV>(p, p.c.v + bh * bs * DV, p.c.v_range + bh, t * p.ldv + (int64_t)h * DV, n, off);
+        else
+            append_k<BF16, DK>(p, p.c.k + bh * bs * DK, p.c.k_range + bh, t * p.ldk + (int64_t)h * DK, n, off);
+    }
+}
+
+template <int DK, int DV>
+cudaError_t launch_append(const KvAppendParams &p, cudaStream_t s) {
+    // rows a warp looks at: one while that gives the device a few thousand warps
+    const int64_t sides = 2 * (int64_t)p.c.heads;
+    const int span = p.T * sides <= 64 * (int64_t)device_sm_count() ? 1 : p.T < 32 ? (int)p.T : p.c.block < 32 ? p.c.block : 32;
+    const int64_t warps = (p.T + span - 1) / span * sides;
+    return launch_pdl(p.dtype ? kv_append_kernel<true, DK, DV> : kv_append_kernel<false, DK, DV>,
+                      dim3((unsigned)((warps + kAppendWarps - 1) / kAppendWarps)), dim3(kAppendWarps * 32), 0, s, p, span);
 }
 
 }  // namespace
@@ -250,9 +371,9 @@ cudaError_t launch_kv_plan(const KvPlanParams &p, cudaStream_t s) {
 
 cudaError_t launch_kv_append(const KvAppendParams &p, cudaStream_t s) {
     if (p.T == 0) return cudaSuccess;
-    const int64_t warps = p.T * p.c.heads;
-    return launch_pdl(p.dtype ? kv_append_kernel<true> : kv_append_kernel<false>,
-                      dim3((unsigned)((warps + kAppendWarps - 1) / kAppendWarps)), dim3(kAppendWarps * 32), 0, s, p);
+    if (p.c.k_dim == 64) return launch_append<64, 64>(p, s);
+    if (p.c.k_dim == 128) return launch_append<128, 128>(p, s);
+    return launch_append<192, 128>(p, s);
 }
 
 }  // namespace qmoe
