@@ -512,12 +512,11 @@ QMOE_API int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t b
  *                             entry is not in 0 .. num_blocks - 1
  *   positions [capacity]      the token's place in its request, -1 likewise
  *   taken     [1]             blocks taken of free_blocks
- *   scratch   [requests]
  * The sum of new_lens must be below 2^31.  block_size: 16, 32, ... 256. */
 QMOE_API int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
                           int32_t block_size, const int32_t *free_blocks, int64_t n_free, int64_t num_blocks,
                           int32_t *block_table, int64_t max_blocks, int64_t capacity, int32_t *q_start,
-                          int32_t *kv_lens, int32_t *slots, int32_t *positions, int32_t *taken, int32_t *scratch);
+                          int32_t *kv_lens, int32_t *slots, int32_t *positions, int32_t *taken);
 
 /* The cache: codes in blocks of block_size tokens and one f32 range (the r
  * above) per block and head, in memory of the caller, 16-byte aligned:

@@ -2243,7 +2243,7 @@ int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t batch, int
 int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
                  int32_t block_size, const int32_t *free_blocks, int64_t n_free, int64_t num_blocks,
                  int32_t *block_table, int64_t max_blocks, int64_t capacity, int32_t *q_start, int32_t *kv_lens,
-                 int32_t *slots, int32_t *positions, int32_t *taken, int32_t *scratch) {
+                 int32_t *slots, int32_t *positions, int32_t *taken) {
     if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
     if (block_size < 16 || block_size > 256 || block_size % 16)
         return fail(QMOE_ERR_INVALID, "block_size %d must be a multiple of 16, at most 256", block_size);
@@ -2254,13 +2254,13 @@ int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_l
                     (long long)capacity);
     if (num_blocks >= (1LL << 31) / block_size || max_blocks >= (1LL << 31) / block_size)
         return fail(QMOE_ERR_INVALID, "num_blocks and max_blocks times block_size must be below 2^31");
-    if (!q_start || !taken || (requests > 0 && (!cached_lens || !new_lens || !kv_lens || !scratch)) ||
+    if (!q_start || !taken || (requests > 0 && (!cached_lens || !new_lens || !kv_lens)) ||
         (requests > 0 && max_blocks > 0 && !block_table) || (n_free > 0 && !free_blocks) ||
         (capacity > 0 && (!slots || !positions)))
         return fail(QMOE_ERR_INVALID, "NULL argument");
     DeviceGuard g(ctx->device);
     KvPlanParams p{cached_lens, new_lens, requests, block_size, free_blocks, n_free, num_blocks, block_table,
-                   max_blocks, capacity, q_start, kv_lens, slots, positions, taken, scratch};
+                   max_blocks, capacity, q_start, kv_lens, slots, positions, taken};
     QTRY_CUDA(launch_kv_plan(p, ctx->stream));
     return QMOE_OK;
 }

@@ -392,7 +392,6 @@ struct KvPlanParams {
     int32_t *q_start, *kv_lens;      // [R + 1], [R]
     int32_t *slots, *positions;      // [capacity]
     int32_t *taken;                  // [1]
-    int32_t *first;                  // [R] scratch: first place in the free list
 };
 struct KvAppendParams {
     KvCacheDev c;

@@ -14,26 +14,31 @@ namespace {
 // its tokens without a slot).  Needs are summed over the requests that only
 // the list could deny, so the granted ones take a prefix of it.
 //
-// Two launches.  The scan (one CTA, each thread a run of requests) writes
-// q_start, kv_lens and each request's first place in the free list; the fill
-// gives every token its request by bisection of q_start.  A new block's first
-// position belongs to exactly one new token, which writes the table entry.
+// One launch, bound by latency.  Every CTA sums up all requests for itself (a
+// thread a run of them, 8 bytes a request from L2) and keeps the sums before
+// each run; a token finds its run by bisection and its request by walking the
+// run.  CTA 0 writes the requests' results.  A new block's first position
+// belongs to exactly one new token, which writes the table's entry.
 
-constexpr int kScanThreads = 1024;
+constexpr int kPlanThreads = 1024;
 
 struct Need {
     int64_t fresh;   // rows in the token buffer
-    int64_t blocks;  // blocks wanted of the free list
+    int blocks;      // blocks wanted of the free list
     bool ok;         // fits the table and the token buffer
 };
 
-QMOE_DEV Need need_of(const KvPlanParams &p, int64_t r, int64_t end) {
-    const int64_t c = p.cached[r], f = p.fresh[r];
+QMOE_DEV Need need_of(const KvPlanParams &p, int64_t r, int64_t row) {
+    const int c = p.cached[r], f = p.fresh[r];
     Need n;
     n.fresh = f > 0 ? f : 0;
-    n.ok = c >= 0 && f >= 0 && c + f <= p.max_blocks * p.block && end + n.fresh <= p.capacity;
+    n.ok = c >= 0 && f >= 0 && (int64_t)c + f <= p.max_blocks * p.block && row + n.fresh <= p.capacity;
     n.blocks = n.ok ? (c + f + p.block - 1) / p.block - (c + p.block - 1) / p.block : 0;
     return n;
+}
+
+QMOE_DEV bool granted(const KvPlanParams &p, const Need &n, int64_t before) {
+    return n.ok && (n.blocks == 0 || before + n.blocks <= p.n_free);
 }
 
 // Exclusive sum over the CTA; `total` the sum of all.
@@ -48,26 +53,28 @@ QMOE_DEV int64_t block_scan(int64_t v, int64_t *part, int64_t &total) {
     __syncthreads();
     if (lane == 31) part[warp] = s;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
-    for (int w = 0; w < kScanThreads / 32; ++w) {
-        if (w < warp) before += part[w];
-        total += part[w];
+    int64_t w = part[lane];                        // kPlanThreads / 32 = 32 warps
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += u;
     }
-    return before + s - v;
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    return (warp > 0 ? before : 0) + s - v;
 }
 
-__global__ void __launch_bounds__(kScanThreads) kv_scan_kernel(const KvPlanParams p) {
-    __shared__ int64_t part[kScanThreads / 32];
+QMOE_DEV int clamp32(int64_t v) { return (int)(v < INT32_MAX ? v : INT32_MAX); }
+
+__global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanParams p) {
+    __shared__ int64_t part[32], rows[kPlanThreads], lacks[kPlanThreads];   // sums before each thread's run
     __shared__ int taken;
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int tid = threadIdx.x;
-    const int64_t free_count = p.n_free;
-    const int64_t per = (p.R + kScanThreads - 1) / kScanThreads;
+    const int64_t per = (p.R + kPlanThreads - 1) / kPlanThreads;
     const int64_t lo = tid * per < p.R ? tid * per : p.R, hi = lo + per < p.R ? lo + per : p.R;
-    if (tid == 0) taken = 0;
-    int64_t sum = 0, total;
+    int64_t sum = 0, total, all;
     for (int64_t r = lo; r < hi; ++r) sum += p.fresh[r] > 0 ? p.fresh[r] : 0;
     const int64_t row0 = block_scan(sum, part, total);
     int64_t row = row0;
@@ -77,60 +84,64 @@ __global__ void __launch_bounds__(kScanThreads) kv_scan_kernel(const KvPlanParam
         sum += n.blocks;
         row += n.fresh;
     }
-    int64_t all;
-    int64_t blk = block_scan(sum, part, all);
-    int most = 0;
-    row = row0;
-    for (int64_t r = lo; r < hi; ++r) {
-        const Need n = need_of(p, r, row);
-        const bool ok = n.ok && (n.blocks == 0 || blk + n.blocks <= free_count);
-        p.q_start[r] = (int32_t)(row < INT32_MAX ? row : INT32_MAX);
-        p.kv_lens[r] = ok ? p.cached[r] + p.fresh[r] : 0;
-        p.first[r] = (int32_t)(blk < INT32_MAX ? blk : INT32_MAX);
-        blk += n.blocks;
-        if (ok && n.blocks) most = (int)blk;
-        row += n.fresh;
-    }
-    atomicMax(&taken, most);
+    const int64_t lack0 = block_scan(sum, part, all);
+    rows[tid] = row0;
+    lacks[tid] = lack0;
+    if (tid == 0) taken = 0;
     __syncthreads();
-    if (tid == 0) {
-        p.q_start[p.R] = (int32_t)(total < INT32_MAX ? total : INT32_MAX);
-        p.taken[0] = taken;
-    }
-}
-
-constexpr int kFillThreads = 256;
-
-__global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const KvPlanParams p) {
-    QMOE_PDL_WAIT();
-    QMOE_PDL_TRIGGER();
-    const int64_t t = (int64_t)blockIdx.x * kFillThreads + threadIdx.x;
-    if (t >= p.capacity) return;
-    int slot = -1, pos = -1;
-    if (t < p.q_start[p.R]) {
-        int64_t lo = 0, hi = p.R;                 // q_start[lo] <= t < q_start[hi]
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (p.q_start[mid] <= t) lo = mid;
-            else hi = mid;
+    if (blockIdx.x == 0) {
+        int64_t lack = lack0;
+        int most = 0;
+        row = row0;
+        for (int64_t r = lo; r < hi; ++r) {
+            const Need n = need_of(p, r, row);
+            const bool ok = granted(p, n, lack);
+            p.q_start[r] = clamp32(row);
+            p.kv_lens[r] = ok ? p.cached[r] + p.fresh[r] : 0;
+            lack += n.blocks;
+            if (ok && n.blocks) most = (int)lack;
+            row += n.fresh;
         }
-        if (p.kv_lens[lo] > 0) {
-            const int c = p.cached[lo], have = (c + p.block - 1) / p.block;
-            pos = c + (int)(t - p.q_start[lo]);
-            const int b = pos / p.block, off = pos - b * p.block;
-            int32_t *entry = p.table + lo * p.max_blocks + b;
-            int id;
-            if (b >= have) {
-                id = p.free_blocks[p.first[lo] + b - have];
-                if (off == 0) *entry = id;
-            } else {
-                id = *entry;
+        if (most > 0) atomicMax(&taken, most);
+        __syncthreads();
+        if (tid == 0) {
+            p.q_start[p.R] = clamp32(total);
+            p.taken[0] = taken;
+        }
+    }
+    for (int64_t t = (int64_t)blockIdx.x * kPlanThreads + tid; t < p.capacity; t += (int64_t)gridDim.x * kPlanThreads) {
+        int slot = -1, pos = -1;
+        if (t < total) {
+            int c = 0;                             // the last run that starts at or before t
+#pragma unroll
+            for (int step = kPlanThreads / 2; step > 0; step >>= 1)
+                if (rows[c + step] <= t) c += step;
+            int64_t r = c * per, lack = lacks[c];
+            row = rows[c];
+            Need n = need_of(p, r, row);
+            while (row + n.fresh <= t) {
+                row += n.fresh;
+                lack += n.blocks;
+                n = need_of(p, ++r, row);
             }
-            if (id >= 0 && id < p.num_blocks) slot = id * p.block + off;
+            if (granted(p, n, lack)) {
+                const int cached = p.cached[r], have = (cached + p.block - 1) / p.block;
+                pos = cached + (int)(t - row);
+                const int b = pos / p.block, off = pos - b * p.block;
+                int32_t *entry = p.table + r * p.max_blocks + b;
+                int id;
+                if (b >= have) {
+                    id = p.free_blocks[lack + b - have];
+                    if (off == 0) *entry = id;
+                } else {
+                    id = *entry;
+                }
+                if (id >= 0 && id < p.num_blocks) slot = id * p.block + off;
+            }
         }
+        p.slots[t] = slot;
+        p.positions[t] = pos;
     }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
 }
 
 // ---- append --------------------------------------------------------------------
@@ -363,10 +374,10 @@ cudaError_t launch_append(const KvAppendParams &p, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_kv_plan(const KvPlanParams &p, cudaStream_t s) {
-    cudaError_t e = launch_pdl(kv_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, p);
-    if (e != cudaSuccess || p.capacity == 0) return e;
-    return launch_pdl(kv_fill_kernel, dim3((unsigned)((p.capacity + kFillThreads - 1) / kFillThreads)),
-                      dim3(kFillThreads), 0, s, p);
+    int64_t ctas = (p.capacity + kPlanThreads - 1) / kPlanThreads;
+    const int64_t most = 2 * (int64_t)device_sm_count();
+    ctas = ctas < 1 ? 1 : ctas < most ? ctas : most;
+    return launch_pdl(kv_plan_kernel, dim3((unsigned)ctas), dim3(kPlanThreads), 0, s, p);
 }
 
 cudaError_t launch_kv_append(const KvAppendParams &p, cudaStream_t s) {

@@ -20,17 +20,33 @@ from typing import Callable, Optional, Tuple
 import torch
 
 from . import capi
-from .layer import Context, _dtype_code, _ptr, default_context
+from .layer import Context, _ptr, default_context
 
 _I64 = ctypes.c_int64
+_CODE = {torch.float32: capi.QMOE_DTYPE_F32, torch.bfloat16: capi.QMOE_DTYPE_BF16}
+_fns: dict = {}
 
 
-def _on(ctx: Context, **tensors) -> None:
-    for name, t in tensors.items():
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{name} must be a CUDA tensor")
-        if t.device.index != ctx.device:
-            raise ValueError(f"{name} is on cuda:{t.device.index}, the context on cuda:{ctx.device}")
+def _fn(name: str):
+    """The entry point, looked up once: these calls are as short as a few microseconds."""
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(capi.lib(), name)
+    return f
+
+
+def _on(ctx: Context, name: str, t) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the context on cuda:{ctx.device}")
+
+
+def _code(t) -> int:
+    c = _CODE.get(t.dtype)
+    if c is None:
+        raise TypeError(f"activations must be float32 or bfloat16, got {t.dtype}")
+    return c
 
 
 def _context_of(x, ctx: Optional[Context]) -> Context:
@@ -39,8 +55,9 @@ def _context_of(x, ctx: Optional[Context]) -> Context:
     return default_context(x.device.index if isinstance(x, torch.Tensor) and x.is_cuda else 0)
 
 
-def _i32(t, name: str, shape) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+def _i32(ctx: Context, t, name: str, shape) -> int:
+    _on(ctx, name, t)
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
@@ -49,10 +66,10 @@ def quantize_int8(x, ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch
     """(codes int8 [rows, cols], scales f32 [rows]) of x [rows, cols]: with r
     the row's largest magnitude, code = round(127 x / r) and scale = r / 127."""
     ctx = _context_of(x, ctx)
-    _on(ctx, x=x)
+    _on(ctx, "x", x)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
-    dt = _dtype_code(x)
+    dt = _code(x)
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
@@ -90,7 +107,8 @@ class Int8Tensor:
         if kind != kind2:
             raise ValueError("codes and scales must both be host or both device memory")
         if kind == capi.QMOE_PTR_DEVICE:
-            _on(ctx, codes=codes, scales=scales)
+            _on(ctx, "codes", codes)
+            _on(ctx, "scales", scales)
         ctx.use_current_torch_stream()
         h = ctypes.c_void_p()
         capi.call("qmoe_int8_create", ctx.handle, cp, sp, out_f, in_f, kind, ctypes.byref(h))
@@ -107,28 +125,36 @@ class Int8Tensor:
 
         `out` may be `residual` itself."""
         out_f, in_f = self.shape
-        _on(self.ctx, x=x)
-        dt = _dtype_code(x)
+        ctx = self.ctx
+        _on(ctx, "x", x)
+        dt = _code(x)
         if x.dim() < 1 or x.shape[-1] != in_f:
             raise ValueError(f"x {list(x.shape)} does not end in in_features = {in_f}")
         rows = x if x.dim() == 2 else x.reshape(-1, in_f)
-        if rows.stride(1) != 1 or rows.stride(0) < in_f:
+        stride, unit = rows.stride()
+        if unit != 1 or stride < in_f:
             rows = rows.contiguous()
+            stride = in_f
         batch = rows.shape[0]
         shape = x.shape[:-1] + (out_f,)
         if out is None:
             out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        for name, a in (("residual", residual), ("out", out)):
-            if a is not None:
-                _on(self.ctx, **{name: a})
-                if a.shape != shape or a.dtype != x.dtype or not a.is_contiguous():
-                    raise ValueError(f"{name} must be contiguous {x.dtype} {list(shape)}")
+        else:
+            self._like(out, "out", shape, x.dtype)
+        if residual is not None:
+            self._like(residual, "residual", shape, x.dtype)
         need = batch * self._row_bytes
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        self.ctx.use_current_torch_stream()
-        capi.call("qmoe_int8_forward", self._h, rows.data_ptr(), dt, batch, rows.stride(0),
-                  residual.data_ptr() if residual is not None else None, out.data_ptr(), ws.data_ptr(), need)
+        ctx.use_current_torch_stream()
+        capi.check(_fn("qmoe_int8_forward")(
+            self._h, rows.data_ptr(), dt, batch, stride, residual.data_ptr() if residual is not None else None,
+            out.data_ptr(), ws.data_ptr(), need))
         return out
+
+    def _like(self, t, name: str, shape, dtype) -> None:
+        _on(self.ctx, name, t)
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
 
     def close(self):
         if getattr(self, "_h", None):
@@ -164,22 +190,26 @@ def plan_pages(cached_lens, new_lens, block_table, free_blocks, block_size: int,
     tensors int32 on the GPU; the host reads nothing.  A request that does not
     fit is denied: kv_lens 0, slots and positions -1."""
     ctx = _context_of(cached_lens, ctx)
-    _on(ctx, cached_lens=cached_lens, new_lens=new_lens, block_table=block_table, free_blocks=free_blocks)
+    for name, t in (("block_table", block_table), ("free_blocks", free_blocks)):
+        _on(ctx, name, t)
     if block_table.dim() != 2 or free_blocks.dim() != 1:
         raise ValueError("block_table must be [requests, max_blocks] and free_blocks [n]")
     R, width = block_table.shape
+    n_free = free_blocks.shape[0]
     T = int(num_tokens)
     if T < 0:
         raise ValueError(f"num_tokens {T} < 0")
-    args = (_i32(cached_lens, "cached_lens", (R,)), _i32(new_lens, "new_lens", (R,)),
-            _i32(free_blocks, "free_blocks", free_blocks.shape), _i32(block_table, "block_table", (R, width)))
-    buf = torch.empty(3 * R + 2 + 2 * T, dtype=torch.int32, device=block_table.device)
-    kv, scratch, q_start, taken, slots, positions = buf.split([R, R, R + 1, 1, T, T])
+    cp = _i32(ctx, cached_lens, "cached_lens", (R,))
+    np_ = _i32(ctx, new_lens, "new_lens", (R,))
+    fp = _i32(ctx, free_blocks, "free_blocks", (n_free,))
+    tp = _i32(ctx, block_table, "block_table", (R, width))
+    buf = torch.empty(2 * (R + 1 + T), dtype=torch.int32, device=block_table.device)
+    q_start, kv, taken, slots, positions = buf.split_with_sizes((R + 1, R, 1, T, T))
     at = buf.data_ptr()
     ctx.use_current_torch_stream()
-    capi.call("qmoe_kv_plan", ctx.handle, args[0], args[1], R, int(block_size), args[2], free_blocks.shape[0],
-              int(num_blocks), args[3], width, T, at + 8 * R, at, at + 12 * R + 8, at + 12 * R + 8 + 4 * T,
-              at + 12 * R + 4, at + 4 * R)
+    capi.check(_fn("qmoe_kv_plan")(
+        ctx.handle, cp, np_, R, int(block_size), fp, n_free, int(num_blocks), tp, width, T, at,
+        at + 4 * R + 4, at + 8 * R + 8, at + 8 * R + 8 + 4 * T, at + 8 * R + 4))
     return PagePlan(block_table, q_start, kv, slots, positions, taken, int(max_kv))
 
 
@@ -212,7 +242,8 @@ class KVCache:
         return self
 
     def _set(self, k, v, k_range, v_range, ctx: Context) -> None:
-        _on(ctx, k=k, v=v, k_range=k_range, v_range=v_range)
+        for name, t in (("k", k), ("v", v), ("k_range", k_range), ("v_range", v_range)):
+            _on(ctx, name, t)
         if k.dim() != 5 or v.dim() != 5:
             raise ValueError("k and v must have 5 dimensions")
         nb, heads, chunks, bs, w = k.shape
@@ -230,35 +261,50 @@ class KVCache:
         self._c = capi.KvCacheC(k.data_ptr(), v.data_ptr(), k_range.data_ptr(), v_range.data_ptr(), nb, bs, heads,
                                 self.k_dim, self.v_dim)
         self._p = ctypes.pointer(self._c)
-        n = _I64()
-        capi.call("qmoe_kv_attend_workspace", self._p, 0, 0, 0, heads, 0, 0, ctypes.byref(n))   # checks the shape
+        self._ws: dict = {}
+        self._workspace(0, 0, 0, heads, 0, 0)     # checks the shape
+
+    def _workspace(self, *key) -> int:
+        """Workspace bytes of (dtype, tokens, requests, heads, max_blocks, max_kv)."""
+        n = self._ws.get(key)
+        if n is None:
+            v = _I64()
+            capi.check(_fn("qmoe_kv_attend_workspace")(self._p, *key, ctypes.byref(v)))
+            if len(self._ws) >= 256:              # a server's batches come in few sizes
+                self._ws.clear()
+            n = self._ws[key] = v.value
+        return n
 
     def _rows(self, x, name: str, heads: int, dim: int, dtype) -> Tuple[int, int]:
         """(pointer, token stride) of [tokens, heads, dim] whose heads are packed."""
-        if x.dim() != 3 or tuple(x.shape[1:]) != (heads, dim):
+        _on(self.ctx, name, x)
+        if x.dim() != 3 or x.shape[1:] != (heads, dim):
             raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {list(x.shape)}")
         if x.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
-        if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
+        ts, hs, ds = x.stride()
+        if ds != 1 or (heads > 1 and hs != dim):
             raise ValueError(f"the heads of {name} must be packed")
-        if x.shape[0] > 1 and x.stride(0) < heads * dim:
-            raise ValueError(f"the tokens of {name} overlap")
-        return x.data_ptr(), max(x.stride(0), heads * dim)
+        if ts < heads * dim:
+            if x.shape[0] > 1:
+                raise ValueError(f"the tokens of {name} overlap")
+            ts = heads * dim
+        return x.data_ptr(), ts
 
     def append(self, k, v, slots) -> None:
         """Rows k [tokens, kv_heads, k_dim] and v [tokens, kv_heads, v_dim] (views
         whose heads are packed, e.g. of one projection's rows) to slots [tokens]
         (plan_pages); rows with slot -1 are skipped."""
-        _on(self.ctx, k=k, v=v, slots=slots)
-        dt = _dtype_code(k)
+        ctx = self.ctx
         kp, ks = self._rows(k, "k", self.kv_heads, self.k_dim, k.dtype)
         vp, vs = self._rows(v, "v", self.kv_heads, self.v_dim, k.dtype)
         T = k.shape[0]
         if v.shape[0] != T:
             raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
-        sp = _i32(slots, "slots", (T,))
-        self.ctx.use_current_torch_stream()
-        capi.call("qmoe_kv_append", self.ctx.handle, self._p, kp, vp, dt, T, ks, vs, sp)
+        sp = _i32(ctx, slots, "slots", (T,))
+        dt = _code(k)
+        ctx.use_current_torch_stream()
+        capi.check(_fn("qmoe_kv_append")(ctx.handle, self._p, kp, vp, dt, T, ks, vs, sp))
 
     def attend(self, q, q_start, kv_lens, block_table, scale: Optional[float] = None, max_kv: int = 0, out=None):
         """Causal attention of q [tokens, heads, k_dim] over the cache; rows
@@ -267,39 +313,41 @@ class KVCache:
         v_dim].  Rows that see nothing are zeros; rows past the last request are
         left as `out` has them (zeros without one).  max_kv: the longest kv_lens
         if the host knows it (for speed alone)."""
-        _on(self.ctx, q=q, q_start=q_start, kv_lens=kv_lens, block_table=block_table)
-        dt = _dtype_code(q)
+        ctx = self.ctx
+        _on(ctx, "q", q)
         if q.dim() != 3:
             raise ValueError(f"q must be [tokens, heads, {self.k_dim}], got {list(q.shape)}")
         T, heads, _ = q.shape
         qp, qs = self._rows(q, "q", heads, self.k_dim, q.dtype)
+        dt = _code(q)
+        _on(ctx, "block_table", block_table)
         if block_table.dim() != 2:
             raise ValueError("block_table must be [requests, max_blocks]")
         R, width = block_table.shape
-        sp, lp, tp = (_i32(q_start, "q_start", (R + 1,)), _i32(kv_lens, "kv_lens", (R,)),
-                      _i32(block_table, "block_table", (R, width)))
+        sp = _i32(ctx, q_start, "q_start", (R + 1,))
+        lp = _i32(ctx, kv_lens, "kv_lens", (R,))
+        tp = _i32(ctx, block_table, "block_table", (R, width))
         if out is None:
             out = torch.zeros(T, heads, self.v_dim, dtype=q.dtype, device=q.device)
-        else:
-            _on(self.ctx, out=out)
-            if out.shape[0] != T:
-                raise ValueError(f"out has {out.shape[0]} tokens, q {T}")
         op, os_ = self._rows(out, "out", heads, self.v_dim, q.dtype)
-        n = _I64()
-        capi.call("qmoe_kv_attend_workspace", self._p, dt, T, R, heads, width, int(max_kv), ctypes.byref(n))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
-        self.ctx.use_current_torch_stream()
-        capi.call("qmoe_kv_attend", self.ctx.handle, self._p, qp, dt, T, qs, heads, sp, lp, R, tp, width,
-                  int(max_kv), float(self.k_dim ** -0.5 if scale is None else scale), op, os_,
-                  ws.data_ptr() if ws is not None else None, n.value)
+        if out.shape[0] != T:
+            raise ValueError(f"out has {out.shape[0]} tokens, q {T}")
+        max_kv = int(max_kv)
+        need = self._workspace(dt, T, R, heads, width, max_kv)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        ctx.use_current_torch_stream()
+        capi.check(_fn("qmoe_kv_attend")(
+            ctx.handle, self._p, qp, dt, T, qs, heads, sp, lp, R, tp, width, max_kv,
+            self.k_dim ** -0.5 if scale is None else scale, op, os_, ws.data_ptr() if ws is not None else None, need))
         return out
 
 
 def layer_norm(x, weight, bias, eps: float = 1e-6, ctx: Optional[Context] = None):
     """The block's LayerNorm (qmoe-rs src/model.rs:366-367) of x [tokens, hidden_dim]."""
     ctx = _context_of(x, ctx)
-    _on(ctx, x=x, weight=weight, bias=bias)
-    dt = _dtype_code(x)
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        _on(ctx, name, t)
+    dt = _code(x)
     if x.dim() != 2 or weight.shape != (x.shape[1],) or bias.shape != weight.shape:
         raise ValueError(f"x {list(x.shape)}, weight {list(weight.shape)}, bias {list(bias.shape)}")
     if weight.dtype != torch.float32 or bias.dtype != torch.float32:

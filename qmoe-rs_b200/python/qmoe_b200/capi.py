@@ -139,7 +139,7 @@ SIGNATURES = {
     "qmoe_int8_workspace": (_I, [_P, _I64, ctypes.POINTER(_I64)]),
     "qmoe_int8_forward": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _P, _I64]),
     "qmoe_kv_plan": (_I, [_P, _P, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P,
-                          _P, _P]),
+                          _P]),
     "qmoe_kv_append": (_I, [_P, ctypes.POINTER(KvCacheC), _P, _P, _I, _I64, _I64, _I64, _P]),
     "qmoe_kv_attend_workspace": (_I, [ctypes.POINTER(KvCacheC), _I, _I64, _I64, _I32, _I64, _I64,
                                       ctypes.POINTER(_I64)]),

@@ -67,10 +67,9 @@ def test_attend_arguments(ctx):
 
 
 def test_plan_arguments(ctx):
-    ok = [ctx, 64, 64, 2, 16, 64, 4, 8, 64, 4, 3, 64, 64, 64, 64, 64, 64]
+    ok = [ctx, 64, 64, 2, 16, 64, 4, 8, 64, 4, 3, 64, 64, 64, 64, 64]
     for i, v in ((0, None), (1, None), (2, None), (3, -1), (4, 15), (4, 0), (5, None), (6, -1), (7, -1), (7, 1 << 27), (8, None),
-                 (9, -1), (9, 1 << 27), (10, -1), (10, 1 << 31), (11, None), (12, None), (13, None), (14, None), (15, None),
-                 (16, None)):
+                 (9, -1), (9, 1 << 27), (10, -1), (10, 1 << 31), (11, None), (12, None), (13, None), (14, None), (15, None)):
         a = list(ok)
         a[i] = v
         assert rc("qmoe_kv_plan", *a)[0] == capi.QMOE_ERR_INVALID, (i, v)
