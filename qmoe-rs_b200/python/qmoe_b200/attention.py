@@ -35,6 +35,17 @@ def _fn(name: str):
     return f
 
 
+# the current stream's handle without a Stream object around it (1.3 us less)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _use_stream(ctx: Context) -> None:
+    stream = _raw_stream(ctx.device)
+    if stream != ctx._stream:
+        ctx.use_stream(stream)
+
+
 def _on(ctx: Context, name: str, t) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
@@ -74,7 +85,7 @@ def quantize_int8(x, ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch
         x = x.contiguous()
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-    ctx.use_current_torch_stream()
+    _use_stream(ctx)
     capi.call("qmoe_quantize_int8", ctx.handle, x.data_ptr(), dt, x.shape[0], x.shape[1],
               max(x.stride(0), x.shape[1]), codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -109,7 +120,7 @@ class Int8Tensor:
         if kind == capi.QMOE_PTR_DEVICE:
             _on(ctx, "codes", codes)
             _on(ctx, "scales", scales)
-        ctx.use_current_torch_stream()
+        _use_stream(ctx)
         h = ctypes.c_void_p()
         capi.call("qmoe_int8_create", ctx.handle, cp, sp, out_f, in_f, kind, ctypes.byref(h))
         return cls(h, ctx, shape, scales)
@@ -128,15 +139,16 @@ class Int8Tensor:
         ctx = self.ctx
         _on(ctx, "x", x)
         dt = _code(x)
-        if x.dim() < 1 or x.shape[-1] != in_f:
-            raise ValueError(f"x {list(x.shape)} does not end in in_features = {in_f}")
-        rows = x if x.dim() == 2 else x.reshape(-1, in_f)
+        shape = x.shape
+        if len(shape) < 1 or shape[-1] != in_f:
+            raise ValueError(f"x {list(shape)} does not end in in_features = {in_f}")
+        rows = x if len(shape) == 2 else x.reshape(-1, in_f)
         stride, unit = rows.stride()
         if unit != 1 or stride < in_f:
             rows = rows.contiguous()
             stride = in_f
         batch = rows.shape[0]
-        shape = x.shape[:-1] + (out_f,)
+        shape = (*shape[:-1], out_f)
         if out is None:
             out = torch.empty(shape, dtype=x.dtype, device=x.device)
         else:
@@ -145,7 +157,7 @@ class Int8Tensor:
             self._like(residual, "residual", shape, x.dtype)
         need = batch * self._row_bytes
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        ctx.use_current_torch_stream()
+        _use_stream(ctx)
         capi.check(_fn("qmoe_int8_forward")(
             self._h, rows.data_ptr(), dt, batch, stride, residual.data_ptr() if residual is not None else None,
             out.data_ptr(), ws.data_ptr(), need))
@@ -206,7 +218,7 @@ def plan_pages(cached_lens, new_lens, block_table, free_blocks, block_size: int,
     buf = torch.empty(2 * (R + 1 + T), dtype=torch.int32, device=block_table.device)
     q_start, kv, taken, slots, positions = buf.split_with_sizes((R + 1, R, 1, T, T))
     at = buf.data_ptr()
-    ctx.use_current_torch_stream()
+    _use_stream(ctx)
     capi.check(_fn("qmoe_kv_plan")(
         ctx.handle, cp, np_, R, int(block_size), fp, n_free, int(num_blocks), tp, width, T, at,
         at + 4 * R + 4, at + 8 * R + 8, at + 8 * R + 8 + 4 * T, at + 8 * R + 4))
@@ -303,7 +315,7 @@ class KVCache:
             raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
         sp = _i32(ctx, slots, "slots", (T,))
         dt = _code(k)
-        ctx.use_current_torch_stream()
+        _use_stream(ctx)
         capi.check(_fn("qmoe_kv_append")(ctx.handle, self._p, kp, vp, dt, T, ks, vs, sp))
 
     def attend(self, q, q_start, kv_lens, block_table, scale: Optional[float] = None, max_kv: int = 0, out=None):
@@ -335,7 +347,7 @@ class KVCache:
         max_kv = int(max_kv)
         need = self._workspace(dt, T, R, heads, width, max_kv)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        ctx.use_current_torch_stream()
+        _use_stream(ctx)
         capi.check(_fn("qmoe_kv_attend")(
             ctx.handle, self._p, qp, dt, T, qs, heads, sp, lp, R, tp, width, max_kv,
             self.k_dim ** -0.5 if scale is None else scale, op, os_, ws.data_ptr() if ws is not None else None, need))
@@ -354,7 +366,7 @@ def layer_norm(x, weight, bias, eps: float = 1e-6, ctx: Optional[Context] = None
         raise TypeError("weight and bias must be float32")
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
     out = torch.empty_like(x)
-    ctx.use_current_torch_stream()
+    _use_stream(ctx)
     capi.call("qmoe_layer_norm", ctx.handle, x.data_ptr(), dt, x.shape[0], x.shape[1], weight.data_ptr(),
               bias.data_ptr(), float(eps), out.data_ptr())
     return out
