@@ -67,6 +67,11 @@ QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int
     return lo;
 }
 
+// What the slots of a launch are: tokens, where each request has one at most;
+// requests with one token; requests with 2 .. tq; tiles of tq tokens of the
+// requests with more than one.
+enum class Slots { kTokens, kSingles, kFew, kTiles };
+
 struct Rows {                                    // of one CTA: rows of one request and kv head
     int64_t t0;                                  // token of row 0
     int tokens, head0;                           // row i * gq + g: token t0 + i, head head0 + g
@@ -75,11 +80,11 @@ struct Rows {                                    // of one CTA: rows of one requ
     int64_t request;
 };
 
-// by_request: slot r is request r, if it has up to tq tokens.
-QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, bool by_request, Rows &w) {
+QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind, Rows &w) {
+    const bool by_request = kind == Slots::kSingles || kind == Slots::kFew;
     const int64_t r = by_request ? slot : find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    if (by_request && n > tq) return false;
+    if (kind == Slots::kSingles ? n != 1 : kind == Slots::kFew ? n < 2 || n > tq : kind == Slots::kTiles && n < 2) return false;
     const int64_t i0 = by_request ? 0 : (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
@@ -101,8 +106,10 @@ QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, bool by_req
 // of 64 tokens, then their V), fetched by bulk copies a 16-token group each,
 // the next ones in flight while one is worked on.  16 tokens of V start 32
 // bytes off a multiple of 128 from the ones before, so the lanes of a quarter
-// warp (two dims, four groups) read 128 bytes of distinct banks.
-constexpr int kSlots = 3;
+// warp (two dims, four groups) read 128 bytes of distinct banks.  Two halves a
+// warp are enough with eight or twelve warps an SM (64 KB and more in flight);
+// a third slot gained nothing.
+constexpr int kSlots = 2;
 
 template <int DK, int DV, int NT>
 struct Shared {
@@ -131,13 +138,27 @@ QMOE_DEV uint32_t transpose8(uint32_t v) {
     return r;
 }
 
+// Dims 64 J + 0 .. 15 from q[at] on.
+template <int DK, bool BF16, bool VEC>
+QMOE_DEV void load_row(const AttendParams &p, int64_t at, float (&v)[DK / 64][16]) {
+#pragma unroll
+    for (int J = 0; J < DK / 64; ++J)
+#pragma unroll
+        for (int d = 0; d < 16; d += 4) {
+            const float4 f = load_q4<BF16, VEC>(p, at + 64 * J + d);
+            v[J][d] = f.x;
+            v[J][d + 1] = f.y;
+            v[J][d + 2] = f.z;
+            v[J][d + 3] = f.w;
+        }
+}
+
 // A CTA's rows on NT * 8 columns: row i * gq + g of w.
 template <int DK, int DV, bool BF16, int NT>
-QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split, int gq, int heads_here,
-                          uint8_t *smem_raw) {
+QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split, int gq, int heads_here, Shared<DK, DV, NT> &S,
+                          uint32_t &done) {
     constexpr int kTerms = BF16 ? 1 : 2;
     using Sm = Shared<DK, DV, NT>;
-    Sm &S = *reinterpret_cast<Sm *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int bs = p.c.block;
 
@@ -157,13 +178,14 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         const int64_t b = row_table[block_index(p, tok)];
         return b >= 0 && b < p.c.num_blocks ? b * p.c.heads + h : -1;
     };
-    // copies of item n (K of tile n / 2, or its V) into slot n % kSlots: an even
-    // lane g a piece of 64 dims each of K, or c = 0 its group of V
+    // copies of item n (K of tile n / 2, or its V) into its slot (`done` items were
+    // worked on before): an even lane g a piece of 64 dims each of K, or c = 0 its
+    // group of V
     auto fetch = [&](int n, int64_t bh) {
         if (n >= 2 * mine) return;
         const int tok = (t_lo + warp + (n >> 1) * kWarps) * 64 + 16 * grp, off = tok - block_index(p, tok) * bs;
-        uint8_t *dst = S.ring[warp][n % kSlots];
-        uint64_t *bar = &S.full[warp][n % kSlots];
+        uint8_t *dst = S.ring[warp][(done + n) % kSlots];
+        uint64_t *bar = &S.full[warp][(done + n) % kSlots];
         const bool is_v = n & 1;
         const bool copy = bh >= 0 && (g & 1) == 0 && c < (is_v ? 1 : DK / 64);
         const uint32_t bytes = is_v ? DV * 16 : 1024;
@@ -179,15 +201,8 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     };
 
     int64_t blk = block_of(0), blk1 = block_of(1), blk2 = block_of(2);
-    if (tid == 0) {
-        for (int i = 0; i < kWarps * kSlots; ++i) sm100::mbar_init(&S.full[0][0] + i, 1);
-        S.abort = 0;
-        sm100::fence_mbar_init();
-    }
-    __syncthreads();
     fetch(0, blk);
     fetch(1, blk);
-    fetch(2, blk1);
     float kr = blk >= 0 ? p.c.k_range[blk] : 0.0f, vr = blk >= 0 ? p.c.v_range[blk] : 127.0f;
 
     // ---- q: rows brought to fp16 by a power of two, as B fragments: lane 4 g + c
@@ -199,19 +214,17 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     for (int x = 0; x < NT; ++x) {
         const int row = 8 * x + g, i = row / gq, gg = row - i * gq;
         const bool live = i < w.tokens && gg < heads_here;
-        const int64_t at = live ? (w.t0 + i) * p.ldq + (int64_t)(w.head0 + gg) * DK + 16 * c : 0;
+        const int64_t at = (live ? (w.t0 + i) * p.ldq + (int64_t)(w.head0 + gg) * DK : w.t0 * p.ldq) + 16 * c;
         float v[DK / 64][16];
+        if (p.vec_q) load_row<DK, BF16, true>(p, at, v);
+        else load_row<DK, BF16, false>(p, at, v);
         float m = 0.0f;
 #pragma unroll
         for (int J = 0; J < DK / 64; ++J)
 #pragma unroll
-            for (int d = 0; d < 16; d += 4) {
-                const float4 f = live ? load_q4(p, at + 64 * J + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                v[J][d] = f.x;
-                v[J][d + 1] = f.y;
-                v[J][d + 2] = f.z;
-                v[J][d + 3] = f.w;
-                m = max_abs(max_abs(max_abs(max_abs(m, f.x), f.y), f.z), f.w);
+            for (int d = 0; d < 16; ++d) {
+                v[J][d] = live ? v[J][d] : 0.0f;
+                m = max_abs(m, v[J][d]);
             }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -266,8 +279,8 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         // the start (its rounding, 2^-24 of 1152 sum q, is small beside bf16's);
         // two terms: the codes themselves, the small term first and each 64 dims
         // in sums of their own, added in f32.
-        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][n % kSlots], (n / kSlots) & 1, &S.abort, p.err))) break;
-        const uint8_t *slot = S.ring[warp][n % kSlots] + (16 * grp + (g & 1)) * 64 + c * 16;
+        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][(done + n) % kSlots], ((done + n) / kSlots) & 1, &S.abort, p.err))) break;
+        const uint8_t *slot = S.ring[warp][(done + n) % kSlots] + (16 * grp + (g & 1)) * 64 + c * 16;
         float s[4][NT][4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -321,7 +334,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
             }
         }
         __syncwarp();
-        fetch(n + 3, blk1);                       // V of the next tile
+        fetch(n + 2, blk1);                       // K of the next tile
         ++n;
         // ---- softmax
         vr = vr < kRangeFloor ? kRangeFloor : vr; // a block of zeros of another writer; NaN stays
@@ -382,8 +395,8 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
             }
         }
         // ---- P V
-        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][n % kSlots], (n / kSlots) & 1, &S.abort, p.err))) break;
-        slot = S.ring[warp][n % kSlots] + c * Sm::kVGroup + g * 16;
+        if (!(ok = sm100::mbar_wait_warp(&S.full[warp][(done + n) % kSlots], ((done + n) / kSlots) & 1, &S.abort, p.err))) break;
+        slot = S.ring[warp][(done + n) % kSlots] + c * Sm::kVGroup + g * 16;
         constexpr int kSide = NT >= 4 ? 2 : 4;    // 16-dim tiles side by side
 #pragma unroll
         for (int t0 = 0; t0 < DV / 16; t0 += kSide) {
@@ -420,7 +433,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
                         acc[t0 + t][x][i] = __fmaf_rn(acc[t0 + t][x][i], fix[x][i & 1], o[t][x][i]);
         }
         __syncwarp();
-        fetch(n + 3, blk2);                       // K of the tile after the next
+        fetch(n + 2, blk1);                       // its V
         ++n;
         blk = blk1;
         blk1 = blk2;
@@ -431,8 +444,9 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     if (!ok) {                                    // let the copies already issued land before the CTA exits
         for (int i = n; i < n + kSlots && i < 2 * mine; ++i)
             for (uint32_t tries = 0; tries < sm100::kMaxWaitProbes; ++tries)
-                if (sm100::mbar_try_wait(&S.full[warp][i % kSlots], (i / kSlots) & 1)) break;
+                if (sm100::mbar_try_wait(&S.full[warp][(done + i) % kSlots], ((done + i) / kSlots) & 1)) break;
     }
+    done += 2 * mine;
     __syncthreads();                              // the ring is free
 
     // ---- join the warps
@@ -492,25 +506,38 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
 // more, the less often the keys are read.
 __host__ __device__ constexpr int most_columns(bool bf16) { return bf16 ? 4 : 2; }
 
-// Up to tq tokens of a request by gq heads of a kv head.  One token (its heads
-// on N1 * 8 columns) and several may meet in a batch; SEVERAL says whether they
-// can.
-template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
-__global__ void __launch_bounds__(kThreads, 8 / kWarps) attend_kernel(const AttendParams p, int tq, int gq, int hgroups, bool by_request) {
+// CTAs an SM holds: three where the registers of a single token's few columns
+// allow it, which evens out batches of ragged lengths (64 requests 99 -> 91 us).
+__host__ __device__ constexpr int ctas_per_sm(int dk, bool bf16, int nt) { return bf16 && nt == 1 && dk <= 128 ? 3 : 2; }
+
+// Up to tq tokens of a request by gq heads of a kv head, on NT * 8 columns.
+template <int DK, int DV, bool BF16, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(DK, BF16, NT))
+attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int64_t slots) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
+    Shared<DK, DV, NT> &S = *reinterpret_cast<Shared<DK, DV, NT> *>(smem_raw);
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups;
     const int G = p.heads / p.c.heads;
-    Rows w;
-    if (!find_rows(p, blockIdx.x, tq, by_request, w)) return;                // the whole CTA alike
-    w.head0 = h * G + hg * gq;
     const int heads_here = G - hg * gq < gq ? G - hg * gq : gq;
-    constexpr int kMost = most_columns(BF16);
-    if (SEVERAL && N1 != kMost && w.tokens > 1)
-        attend_rows<DK, DV, BF16, kMost>(p, w, h, blockIdx.z, gq, heads_here, smem_raw);
-    else
-        attend_rows<DK, DV, BF16, N1>(p, w, h, blockIdx.z, gq, heads_here, smem_raw);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kWarps * kSlots; ++i) sm100::mbar_init(&S.full[0][0] + i, 1);
+        S.abort = 0;
+        sm100::fence_mbar_init();
+    }
+    __syncthreads();
+    uint32_t done = 0;                            // items of this warp's ring so far
+    for (int64_t slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+        Rows w;
+        if (!find_rows(p, slot, tq, kind, w)) continue;                  // the whole CTA alike
+        w.head0 = h * G + hg * gq;
+        attend_rows<DK, DV, BF16, NT>(p, w, h, blockIdx.z, gq, heads_here, S, done);
+        if (slot + gridDim.x < slots) {           // the ring is written by copies again
+            sm100::fence_proxy_async_smem();
+            __syncthreads();
+        }
+    }
 }
 
 // Joins the pieces, one CTA per (token, head): thread s weighs piece s, the
@@ -595,69 +622,66 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 }
 
 struct RowShape {
-    int n1;                                       // columns / 8 of a single token
-    int gq, tq, hgroups;
-    bool several;                                 // a request may have more than one token
-    bool by_request;                              // requests of more than tq tokens are the prompt kernel's
+    int nt, gq, tq, hgroups;
 };
-RowShape row_shape(int64_t T, int64_t R, int G, int dtype) {
+// gq heads by tq tokens on nt * 8 columns: one token, or several.
+RowShape row_shape(bool single, int G, int dtype) {
     const int most = most_columns(dtype != 0);
     RowShape r;
-    r.several = T > R;
     r.gq = G < 8 * most ? G : 8 * most;
-    r.n1 = r.gq <= 8 ? 1 : r.gq <= 16 ? 2 : 4;
-    r.tq = r.several ? 8 * most / r.gq : 1;
+    r.nt = !single ? most : r.gq <= 8 ? 1 : r.gq <= 16 ? 2 : most;
+    r.tq = single ? 1 : 8 * most / r.gq;
     r.hgroups = (G + r.gq - 1) / r.gq;
-    r.by_request = r.several && dtype != 0;
     return r;
 }
 
-template <int DK, int DV, bool BF16, int N1, bool SEVERAL>
-cudaError_t launch_n1(const AttendParams &p, const RowShape &r, cudaStream_t s) {
-    const size_t smem = sizeof(Shared<DK, DV, SEVERAL ? most_columns(BF16) : N1>);
-    auto kernel = attend_kernel<DK, DV, BF16, N1, SEVERAL>;
+template <int DK, int DV, bool BF16, int NT>
+cudaError_t launch_nt(const AttendParams &p, const RowShape &r, Slots kind, int64_t slots, int64_t grid, cudaStream_t s) {
+    const size_t smem = sizeof(Shared<DK, DV, NT>);
+    auto kernel = attend_kernel<DK, DV, BF16, NT>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    const int64_t slots = r.by_request ? p.R : r.tq == 1 ? p.T : p.T / r.tq + p.R;
-    return launch_pdl(kernel, dim3((unsigned)slots, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits),
-                      dim3(kThreads), smem, s, p, r.tq, r.gq, r.hgroups, r.by_request);
+    return launch_pdl(kernel, dim3((unsigned)grid, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits), dim3(kThreads),
+                      smem, s, p, r.tq, r.gq, r.hgroups, kind, slots);
 }
 
 template <int DK, int DV, bool BF16>
 cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
-    const RowShape r = row_shape(p.T, p.R, p.heads / p.c.heads, p.dtype);
+    const int G = p.heads / p.c.heads;
     constexpr int kMost = most_columns(BF16);
-    cudaError_t e;
-    if (r.n1 == 1) e = r.several ? launch_n1<DK, DV, BF16, 1, true>(p, r, s) : launch_n1<DK, DV, BF16, 1, false>(p, r, s);
-    else if (r.n1 == 2) e = r.several ? launch_n1<DK, DV, BF16, 2, true>(p, r, s) : launch_n1<DK, DV, BF16, 2, false>(p, r, s);
-    else e = launch_n1<DK, DV, BF16, kMost, false>(p, r, s);
+    const bool several = p.T > p.R;               // a request may have more than one token
+    const RowShape one = row_shape(true, G, p.dtype), more = row_shape(false, G, p.dtype);
+    const Slots kind = several ? Slots::kSingles : Slots::kTokens;
+    const int64_t slots = several ? p.R : p.T;
+    cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, slots, slots, s)
+                    : one.nt == 2 ? launch_nt<DK, DV, BF16, 2>(p, one, kind, slots, slots, s)
+                                  : launch_nt<DK, DV, BF16, kMost>(p, one, kind, slots, slots, s);
+    if (e == cudaSuccess && several) {
+        // often none: a grid that the device holds at once looks through the slots
+        const int64_t n = BF16 ? p.R : p.T / more.tq + p.R;
+        int64_t grid = 2 * (int64_t)device_sm_count() / ((int64_t)p.c.heads * more.hgroups * p.splits);
+        grid = grid < 1 ? 1 : grid < n ? grid : n;
+        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, n, grid, s);
+    }
+    const bool prompts = several && BF16;         // the requests of more than more.tq tokens
     if (e == cudaSuccess && p.splits > 1)
-        e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(r.by_request ? p.R : p.T), (unsigned)p.heads),
-                       dim3(kJoinWarps * 32), 0, s, p, r.tq, r.by_request);
-    if (e == cudaSuccess && r.by_request) e = launch_attend_prompt(p, r.tq, s);
+        e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(prompts ? p.R : p.T), (unsigned)p.heads),
+                       dim3(kJoinWarps * 32), 0, s, p, more.tq, prompts);
+    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, more.tq, s);
     return e;
-}
-
-// CTAs of the single-token kernel that an SM holds.
-int resident(int k_dim, int v_dim) {
-    const size_t smem = k_dim == 64    ? sizeof(Shared<64, 64, 1>)
-                        : k_dim == 128 ? sizeof(Shared<128, 128, 1>)
-                                       : sizeof(Shared<192, 128, 1>);
-    const int most = 8 / kWarps, fit = (int)(228 * 1024 / (smem + 1024));
-    return fit < most ? fit : most;
 }
 
 }  // namespace
 
-// A batch of few CTAs is cut so that they fill the device once (a request of
-// the longest length each); one of many into pieces of a quarter of that, since
-// its requests may be of any length.
+// A batch of few CTAs is cut so that two an SM fill the device once (a request
+// of the longest length each); one of many into a piece's quarter of that,
+// since its requests may be of any length.
 void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
                    int &chunk) {
-    const RowShape r = row_shape(T, R, heads / c.heads, dtype);
-    const int64_t rows = r.by_request || (T + r.tq - 1) / r.tq < R ? R : (T + r.tq - 1) / r.tq;
+    const RowShape r = row_shape(true, heads / c.heads, dtype);
+    const int64_t rows = T <= R ? T : R;
     const int64_t ctas = (rows < 1 ? 1 : rows) * c.heads * r.hgroups;
-    const int64_t fill = (int64_t)device_sm_count() * resident(c.k_dim, c.v_dim);
+    const int64_t fill = 2 * (int64_t)device_sm_count();
     const int64_t tiles = max_kv < 1 ? 1 : (max_kv + 63) / 64;
     int64_t s = 4 * ctas <= fill ? fill / ctas : (4 * fill + ctas - 1) / ctas;
     int64_t ch = (tiles + s - 1) / s;

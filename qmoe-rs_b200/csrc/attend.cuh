@@ -48,11 +48,14 @@ QMOE_DEV int block_index(const AttendParams &p, int tok) {
     return (int)(((uint64_t)(uint32_t)(tok >> 4) * p.per_block) >> 36);
 }
 
-// Four elements of q.
+// Four elements of q; the type and the form of the load are the caller's
+// constants, so that several calls' loads are in flight together (a test of
+// either between them had each wait for the one before).
+template <bool BF16, bool VEC>
 QMOE_DEV float4 load_q4(const AttendParams &p, int64_t at) {
-    return p.vec_q ? load_act4(p.q, p.dtype, at)
-                   : make_float4(load_act(p.q, p.dtype, at), load_act(p.q, p.dtype, at + 1),
-                                 load_act(p.q, p.dtype, at + 2), load_act(p.q, p.dtype, at + 3));
+    if (VEC) return load_act4(p.q, BF16 ? 1 : 0, at);
+    return make_float4(load_act(p.q, BF16 ? 1 : 0, at), load_act(p.q, BF16 ? 1 : 0, at + 1),
+                       load_act(p.q, BF16 ? 1 : 0, at + 2), load_act(p.q, BF16 ? 1 : 0, at + 3));
 }
 
 // A row of q whose largest magnitude is m goes to fp16 times 2^(14 - e): below
