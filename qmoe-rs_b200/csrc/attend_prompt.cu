@@ -499,7 +499,10 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         }
     } else {
         // ---------------------------------------------------------- MMA
-        const uint32_t is = idesc_f16(128, KT), io = idesc_f16(128, DV);
+        // Counts come through warp reductions: uniform registers, which the MMAs take
+        // (an MMA whose descriptors sit in ordinary registers takes 100 cycles to issue,
+        // twice its time).
+        constexpr uint32_t is = idesc_f16(128, KT), io = idesc_f16(128, DV);
         const uint64_t q0 = smem_desc(smem_u32(S.q[0]), 16, 1024, 2);
         const uint32_t desc_hi = (uint32_t)(q0 >> 32), q_lo = (uint32_t)q0,
                        k_lo = q_lo + (uint32_t)((S.k[0] - S.q[0]) >> 4), v_lo = q_lo + (uint32_t)((S.v[0] - S.q[0]) >> 4);
@@ -518,12 +521,14 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             issued = true;
         };
         while (ok && next_item(p, lo, span, few, r, it)) {
-            const int nt = (it.keys + KT - 1) / KT;
-            const int both = it.cnt > tq ? 2 : 1;                  // query tiles with tokens
+            const int nt = __reduce_max_sync(0xffffffffu, (it.keys + KT - 1) / KT);
+            const bool two = __any_sync(0xffffffffu, it.cnt > tq);           // both query tiles have tokens
             for (int j = 0; j < 2 && j < nt && ok; ++j) {          // the first two tiles' scores
                 const uint32_t st = (u + j) % kStages;
                 if (!(ok = wait_long(&S.k_full[st], ((u + j) / kStages) & 1, abort, p.err))) break;
-                for (int m = 0; m < both && ok; ++m) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    if (!ok || (m == 1 && !two)) break;
                     if (j == 0 && !(ok = wait_long(&S.q_full[m], items[m]++ & 1, abort, p.err))) break;
                     tc_fence_after();
                     scores(m, st);
@@ -533,7 +538,10 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             for (int j = 0; j < nt && ok; ++j, ++u) {
                 const uint32_t st = u % kStages, st2 = (u + 2) % kStages;
                 if (!(ok = wait_long(&S.v_full[st], (u / kStages) & 1, abort, p.err))) break;
-                for (int m = 0; m < both; ++m) {
+                if (j + 2 < nt && !(ok = wait_long(&S.k_full[st2], ((u + 2) / kStages) & 1, abort, p.err))) break;
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    if (m == 1 && !two) break;
                     const uint32_t b = used[m] & 1;
                     if (!(ok = wait_long(&S.p_full[m][b], (used[m] >> 1) & 1, abort, p.err))) break;
                     ++used[m];
@@ -544,11 +552,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
                         warp_mma_f16_ts(d, pa + 8 * x, va + 2 * x, desc_hi, io, (j | x) != 0);
                     warp_commit(&S.pv_done[m][b]);
                     issued = true;
-                    if (j + 2 < nt) {                              // in order after P V: its buffer is free
-                        if (m == 0 && !(ok = wait_long(&S.k_full[st2], ((u + 2) / kStages) & 1, abort, p.err))) break;
-                        tc_fence_after();
-                        scores(m, st2);
-                    }
+                    if (j + 2 < nt) scores(m, st2);                // in order after P V: its buffer is free
                 }
                 if (!ok) break;
                 warp_commit(&S.v_empty[st]);
