@@ -558,7 +558,7 @@ QMOE_API int qmoe_kv_append(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const voi
  * row that sees no token (kv_lens 0) gives zeros; rows from q_start[requests]
  * on are left as they were; a table entry that is not a block of the cache
  * hides its tokens.  out [T, heads, v_dim], tokens out_stride elements apart.
- * heads is a multiple of kv_heads.  max_kv: the longest kv_lens if the caller
+ * heads is a multiple of kv_heads; T * heads < 2^31.  max_kv: the longest kv_lens if the caller
  * knows it, else 0 (max_blocks * block_size is taken); only the time depends
  * on it.  Repeated calls give the same bits. */
 QMOE_API int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int dtype, int64_t T, int64_t requests,

@@ -2218,6 +2218,9 @@ int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t batch, int
     int64_t need = 0;
     QTRY(qmoe_int8_workspace(t, batch, &need));
     if (batch == 0) return QMOE_OK;
+    if (((batch + 15) / 16) * ((t->out_f + 127) / 128) > INT32_MAX)
+        return fail(QMOE_ERR_UNSUPPORTED, "batch %lld times out_features %lld: too many tiles", (long long)batch,
+                    (long long)t->out_f);
     if (!x || !y || !workspace) return fail(QMOE_ERR_INVALID, "NULL argument");
     if (batch > 1 && row_stride < t->in_f)
         return fail(QMOE_ERR_INVALID, "row_stride %lld < in_features %lld", (long long)row_stride, (long long)t->in_f);
@@ -2318,6 +2321,8 @@ static int check_attend(const qmoe_kv_cache *cache, KvCacheDev &c, int64_t T, in
         return fail(QMOE_ERR_INVALID, "T %lld, requests %lld (at most 2^24)", (long long)T, (long long)requests);
     if (heads < 1 || heads > 65535 || heads % c.heads)
         return fail(QMOE_ERR_INVALID, "heads %d must be a multiple of kv_heads %d", heads, c.heads);
+    if (T * heads > INT32_MAX)
+        return fail(QMOE_ERR_INVALID, "T %lld times heads %d must be below 2^31", (long long)T, heads);
     if (max_blocks < 0 || max_blocks >= (1LL << 31) / c.block)
         return fail(QMOE_ERR_INVALID, "max_blocks %lld times block_size must be below 2^31", (long long)max_blocks);
     if (max_kv <= 0 || max_kv > max_blocks * c.block) max_kv = max_blocks * c.block;

@@ -41,7 +41,7 @@ def make_plan(R, bs, seed, new_max, cached_max, spare=3):
 
 
 @pytest.mark.parametrize("R,bs,new_max,cached_max", [(1, 16, 1, 0), (1, 16, 40, 100), (7, 16, 40, 100), (32, 64, 1, 300),
-                                                     (300, 32, 9, 200), (1500, 48, 5, 120), (2100, 128, 3, 300)])
+                                                     (300, 32, 9, 200), (1500, 48, 5, 120), (2100, 128, 3, 300), (5000, 16, 2, 40)])
 @pytest.mark.parametrize("room", ["all", "short", "none"])
 def test_plan(R, bs, new_max, cached_max, room):
     cached, new, table, free = make_plan(R, bs, R + bs, new_max, cached_max)
@@ -292,6 +292,33 @@ def test_attend_extreme_scores(dtype):
     assert (got[0, 0] - one).abs().le(one.abs() * half * 1.01 + 1e-5).all()
     mean = ref.attend(q, *flat, starts, kv, table, bs, 1.0, torch.zeros(3, 1, 128, dtype=torch.float64))
     assert (got[1:] - mean[1:]).abs().max() <= ref.attend_bound(DT[dtype]) * flat[3].max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, None])
+def test_attend_views_scales_and_wrong_hints(dtype, scale):
+    """q and out that start at odd places, negative and zero scales, and a max_kv below the truth."""
+    bs, H, G, dk, dv = 32, 2, 3, 128, 128
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, [(700, 1), (90, 70), (400, 5), (2, 2)], 12)
+    width = H * G * dk
+    wide = torch.zeros(q.shape[0], width + 9, dtype=q.dtype, device="cuda")
+    view = wide[:, 3:3 + width].unflatten(1, (H * G, dk))
+    view.copy_(q)
+    out = torch.zeros(q.shape[0], H * G * dv + 7, dtype=q.dtype, device="cuda")
+    args = (i32(starts), i32(kv), i32([x for r in table for x in r], len(table), len(table[0])))
+    got = cache.attend(view, *args, scale=scale, max_kv=16, out=out[:, 1:1 + H * G * dv].unflatten(1, (H * G, dv)))
+    s = ref.new_scale(dk) if scale is None else scale
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, s, torch.zeros(q.shape[0], H * G, dv, dtype=torch.float64))
+    check_attend(got, want, flat[3], dtype)
+    assert (out[:, 0] == 0).all() and (out[:, 1 + H * G * dv:] == 0).all()
+
+
+@pytest.mark.parametrize("G", [33, 100, 160])
+def test_attend_many_heads_to_one(G):
+    cache, flat, q, starts, kv, table = attend_case("bf16", 16, 1, G, 64, 64, [(50, 1), (70, 9), (33, 2)], 13)
+    got = cache.attend(q.cuda(), i32(starts), i32(kv), i32([x for r in table for x in r], 3, len(table[0])))
+    want = ref.attend_dense(q, *flat, starts, kv, table, 16, ref.new_scale(64), torch.zeros(q.shape[0], G, 64, dtype=torch.float64))
+    check_attend(got, want, flat[3], "bf16")
 
 
 def test_attend_poisoned_rows_stay_apart():
