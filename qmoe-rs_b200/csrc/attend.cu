@@ -513,10 +513,10 @@ __host__ __device__ constexpr int ctas_per_sm(int dk, bool bf16, int nt) { retur
 // Up to tq tokens of a request by gq heads of a kv head, on NT * 8 columns.
 template <int DK, int DV, bool BF16, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(DK, BF16, NT))
-attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int64_t slots) {
+attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int64_t slots, bool beside) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Shared<DK, DV, NT> &S = *reinterpret_cast<Shared<DK, DV, NT> *>(smem_raw);
-    QMOE_PDL_WAIT();
+    if (!beside) QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int h = blockIdx.y / hgroups, hg = blockIdx.y % hgroups;
     const int G = p.heads / p.c.heads;
@@ -538,6 +538,7 @@ attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int
             __syncthreads();
         }
     }
+    if (beside) QMOE_PDL_WAIT();
 }
 
 // Joins the pieces, one CTA per (token, head): thread s weighs piece s, the
@@ -636,13 +637,14 @@ RowShape row_shape(bool single, int G, int dtype) {
 }
 
 template <int DK, int DV, bool BF16, int NT>
-cudaError_t launch_nt(const AttendParams &p, const RowShape &r, Slots kind, int64_t slots, int64_t grid, cudaStream_t s) {
+cudaError_t launch_nt(const AttendParams &p, const RowShape &r, Slots kind, int64_t slots, int64_t grid, bool beside,
+                      cudaStream_t s) {
     const size_t smem = sizeof(Shared<DK, DV, NT>);
     auto kernel = attend_kernel<DK, DV, BF16, NT>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)grid, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits), dim3(kThreads),
-                      smem, s, p, r.tq, r.gq, r.hgroups, kind, slots);
+                      smem, s, p, r.tq, r.gq, r.hgroups, kind, slots, beside);
 }
 
 template <int DK, int DV, bool BF16>
@@ -653,21 +655,26 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     const RowShape one = row_shape(true, G, p.dtype), more = row_shape(false, G, p.dtype);
     const Slots kind = several ? Slots::kSingles : Slots::kTokens;
     const int64_t slots = several ? p.R : p.T;
-    cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, slots, slots, s)
-                    : one.nt == 2 ? launch_nt<DK, DV, BF16, 2>(p, one, kind, slots, slots, s)
-                                  : launch_nt<DK, DV, BF16, kMost>(p, one, kind, slots, slots, s);
+    cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, slots, slots, false, s)
+                    : one.nt == 2 ? launch_nt<DK, DV, BF16, 2>(p, one, kind, slots, slots, false, s)
+                                  : launch_nt<DK, DV, BF16, kMost>(p, one, kind, slots, slots, false, s);
+    // The kinds of requests are launches side by side: a launch may start once
+    // every CTA of the one before has, which the first does only after its wait
+    // for what came before this call; so the others read nothing too early.  They
+    // wait for the launch before them at their end, so that what comes after the
+    // last has all of them behind it.
+    const bool prompts = several && BF16;         // the requests of more than more.tq tokens
+    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, more.tq, s);
     if (e == cudaSuccess && several) {
         // often none: a grid that the device holds at once looks through the slots
         const int64_t n = BF16 ? p.R : p.T / more.tq + p.R;
-        int64_t grid = 2 * (int64_t)device_sm_count() / ((int64_t)p.c.heads * more.hgroups * p.splits);
+        int64_t grid = 8 * (int64_t)device_sm_count() / ((int64_t)p.c.heads * more.hgroups * p.splits);
         grid = grid < 1 ? 1 : grid < n ? grid : n;
-        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, n, grid, s);
+        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, n, grid, true, s);
     }
-    const bool prompts = several && BF16;         // the requests of more than more.tq tokens
     if (e == cudaSuccess && p.splits > 1)
         e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(prompts ? p.R : p.T), (unsigned)p.heads),
                        dim3(kJoinWarps * 32), 0, s, p, more.tq, prompts);
-    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, more.tq, s);
     return e;
 }
 

@@ -191,8 +191,6 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     extern __shared__ uint8_t smem_raw[];
     Sm &S = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    QMOE_PDL_WAIT();
-    QMOE_PDL_TRIGGER();
     // late windows of all heads first: their rows see the most keys
     const int span = 2 * tq, groups = p.c.heads * hgroups, windows = gridDim.x / groups;
     const int window = blockIdx.x / groups, hh = blockIdx.x - window * groups;
@@ -202,7 +200,11 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     int64_t r = first_request(p.q_start, p.R, lo);
     const int64_t r0 = r;
     Item it;
-    if (!next_item(p, lo, span, few, r, it)) return;      // the whole CTA alike
+    if (!next_item(p, lo, span, few, r, it)) {            // the whole CTA alike
+        QMOE_PDL_TRIGGER();
+        QMOE_PDL_WAIT();
+        return;
+    }
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -230,6 +232,9 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // Beside the launch before (attend.cu): the wait is at the end.  A later
+    // kernel that holds TMEM while it waits must find this one's columns taken.
+    QMOE_PDL_TRIGGER();
     const uint32_t tmem = S.tmem_base;
     // columns: scores (P in a tile's first half) of query tile m, buffer b at
     // 128 m + 64 b; O of query tile m at 256 + 128 m
@@ -573,6 +578,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    QMOE_PDL_WAIT();
 }
 
 template <int DK, int DV>

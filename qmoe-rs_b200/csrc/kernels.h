@@ -427,7 +427,7 @@ void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dty
                    int &chunk);
 size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits);
 cudaError_t launch_attend(const AttendParams &p, cudaStream_t s);
-// The requests of more than `few` tokens (bf16), after launch_attend's own.
+// The requests of more than `few` tokens (bf16); launch_attend's.
 cudaError_t launch_attend_prompt(const AttendParams &p, int few, cudaStream_t s);
 
 }  // namespace qmoe
