@@ -119,7 +119,8 @@ QMOE_DEV void store_codes(uint8_t *row, int unit, int r, const uint4 &v) {
     *reinterpret_cast<uint4 *>(row + (((unit + 1) ^ (r & 7)) << 4)) = b;
 }
 
-// 2 * tq tokens of a request that begin in a window of as many rows of q.
+// `span` tokens of a request (both query tiles', or the first one's) that begin
+// in a window of rows of q.
 struct Item {
     int64_t request;
     int t0, cnt;                              // first row of q, tokens
@@ -130,9 +131,8 @@ struct Item {
 // The item of the first request from `r` on that has one in the window; false
 // when there is none.  Requests of up to `few` tokens are attend.cu's.  The
 // whole warp alike.
-QMOE_DEV bool next_item(const AttendParams &p, int64_t lo, int span, int few, int64_t &r, Item &it) {
+QMOE_DEV bool next_item(const AttendParams &p, int64_t lo, int64_t hi, int span, int few, int64_t &r, Item &it) {
     const int lane = threadIdx.x & 31;
-    const int64_t hi = lo + span < p.T ? lo + span : p.T;
     for (; r < p.R; r += 32) {
         const int64_t mine = r + lane;
         int64_t s0 = 0, n = 0, at = -1;
@@ -185,22 +185,23 @@ QMOE_DEV int64_t first_request(const int32_t *start, int64_t R, int64_t lo) {
 
 template <int DK, int DV>
 __global__ void __launch_bounds__(kThreads, 1)
-attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int hgroups, const int few) {
+attend_prompt_kernel(const AttendParams p, const int tq, const int span, const int rows, const int gq, const int hgroups,
+                     const int few) {
     using Sm = Shared<DK, DV>;
     constexpr int kStages = Sm::kStages;
     extern __shared__ uint8_t smem_raw[];
     Sm &S = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // late windows of all heads first: their rows see the most keys
-    const int span = 2 * tq, groups = p.c.heads * hgroups, windows = gridDim.x / groups;
+    const int groups = p.c.heads * hgroups, windows = gridDim.x / groups;
     const int window = blockIdx.x / groups, hh = blockIdx.x - window * groups;
-    const int64_t lo = (int64_t)(windows - 1 - window) * span;
+    const int64_t lo = (int64_t)(windows - 1 - window) * rows, hi = lo + rows < p.T ? lo + rows : p.T;
     const int h = hh / hgroups, hg = hh - h * hgroups, G = p.heads / p.c.heads;
     const int head0 = h * G + hg * gq, heads_here = G - hg * gq < gq ? G - hg * gq : gq;
     int64_t r = first_request(p.q_start, p.R, lo);
     const int64_t r0 = r;
     Item it;
-    if (!next_item(p, lo, span, few, r, it)) {            // the whole CTA alike
+    if (!next_item(p, lo, hi, span, few, r, it)) {            // the whole CTA alike
         QMOE_PDL_TRIGGER();
         QMOE_PDL_WAIT();
         return;
@@ -250,7 +251,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + kOCol + m * 128;
         const float scale = fabsf(p.scale) * kLog2e, sign = p.scale < 0.0f ? -1.0f : 1.0f;
         uint32_t u = 0, n = 0;                        // key tiles of the CTA, and those with this query tile, so far
-        while (ok && next_item(p, lo, span, few, r, it)) {
+        while (ok && next_item(p, lo, hi, span, few, r, it)) {
             const int cnt = it.cnt - m * tq < tq ? it.cnt - m * tq : tq;      // tokens of this query tile
             const int nt = (it.keys + KT - 1) / KT;
             const int i = row / gq, gg = row - i * gq;
@@ -446,7 +447,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
         constexpr int kKLoads = 2 * (DK / 64), kVLoads = DV / 32, kLoads = kKLoads > kVLoads ? kKLoads : kVLoads;
         uint32_t first = 0;                           // unit of the item's first tile
         uint32_t unit = warp - kSoftWarps;            // this warp's next
-        while (ok && next_item(p, lo, span, few, r, it)) {
+        while (ok && next_item(p, lo, hi, span, few, r, it)) {
             const int nt = (it.keys + KT - 1) / KT;
             const uint32_t end = first + 8 * nt;
             const int32_t *table = p.table + it.request * p.max_blocks;
@@ -525,7 +526,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int gq, const int
             if (lane == 0) mbar_arrive(&S.s_full[m][b]);
             issued = true;
         };
-        while (ok && next_item(p, lo, span, few, r, it)) {
+        while (ok && next_item(p, lo, hi, span, few, r, it)) {
             const int nt = __reduce_max_sync(0xffffffffu, (it.keys + KT - 1) / KT);
             const bool two = __any_sync(0xffffffffu, it.cnt > tq);           // both query tiles have tokens
             for (int j = 0; j < 2 && j < nt && ok; ++j) {          // the first two tiles' scores
@@ -588,8 +589,16 @@ cudaError_t launch_dims(const AttendParams &p, int few, cudaStream_t s) {
     auto kernel = attend_prompt_kernel<DK, DV>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    const int64_t windows = (p.T + 2 * tq - 1) / (2 * tq);
-    return launch_pdl(kernel, dim3((unsigned)(windows * p.c.heads * hgroups)), dim3(kThreads), smem, s, p, tq, gq, hgroups,
+    // Batches that leave SMs idle: one query tile an item, windows of fewer rows
+    // (649 tokens after 1112, 8 kv heads 48 -> 40 us; 2 requests of some 20 tokens
+    // 29 -> 19 us; nothing where the SMs are full).
+    const int64_t groups = (int64_t)p.c.heads * hgroups, sms = device_sm_count();
+    const int span = p.T * groups <= sms * tq ? tq : 2 * tq;
+    const int64_t even = (p.T * groups + sms - 1) / sms;
+    // never above span: a window holds one item of a request
+    const int rows = even >= span || span < 16 ? span : even < 16 ? 16 : (int)even;
+    const int64_t windows = (p.T + rows - 1) / rows;
+    return launch_pdl(kernel, dim3((unsigned)(windows * groups)), dim3(kThreads), smem, s, p, tq, span, rows, gq, hgroups,
                       few);
 }
 
