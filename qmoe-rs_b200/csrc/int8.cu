@@ -34,8 +34,11 @@ QMOE_DEV void load8(const void *x, int64_t i, float (&v)[8]) {
 
 // THREADS per row, each 8 * GROUPS elements of it in registers (GROUPS 0: any
 // length or alignment, read twice).  A row is one load latency and one
-// reduction, so short rows share a CTA (a warp each) and long ones take 1024
-// threads: 4096 rows of 7168 bf16 are read once and written once.
+// reduction, so short rows share a CTA (a warp each) and longer ones take as many
+// threads as leave each one or two groups (2624 bf16 on 256 threads instead of
+// 512: 4096 rows and their product to 64 channels 34 -> 25 us; four groups a
+// thread are faster at 4096 rows of 7168, 49 -> 42, and slower at 400 of 8192,
+// 13.5 -> 15.0).
 template <bool BF16, int THREADS, int GROUPS>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS)
 quant_rows_kernel(const Int8RowsParams p) {
@@ -135,16 +138,21 @@ cudaError_t launch_rows(const Int8RowsParams &p, cudaStream_t s) {
 // Every wait is bounded; on a time-out the kernel flags the device error word,
 // drains its copies and MMAs (again bounded), frees TMEM and returns.
 
-constexpr int kThreads = 256;
 constexpr int kABytes = 128 * 128;
 
 // Up to 64 tokens two CTAs share an SM, so that one streams while the other
-// starts or ends.
+// starts or ends (four with half the stages: 32 tokens by 16384 to 7168 29.3 us,
+// with two 27.3).  Wider tiles have eight warps for the epilogue: at K = 1024 it
+// is what bounds the product (4096 tokens to 4096 channels, a residual added:
+// 95 us with four warps and the residual loaded as it was needed, 50 us with
+// eight that load a chunk ahead; 61 -> 30 without a residual).
 template <int BN>
 struct Tile {
     static constexpr int stage = kABytes + BN * 128;
     static constexpr int stages = (BN <= 64 ? 100 : 200) * 1024 / stage;
     static constexpr int ctas = BN <= 64 ? 2 : 1;
+    static constexpr int epilogue = BN <= 64 ? 4 : 8;                 // warps
+    static constexpr int threads = 128 + epilogue * 32;
     static constexpr uint32_t cols = 2 * BN < 32 ? 32 : 2 * BN;
     static_assert(stages * stage >= BN * 512, "the sums of a tile do not fit the ring");
     static_assert(ctas * cols <= 512, "tensor memory");
@@ -157,16 +165,32 @@ struct Smem {
     uint64_t dfull[2], dempty[2], drain;
     uint32_t tmem_base;
     int abort;
-    float sx[4][256];                             // each epilogue warp's copy of a tile's token scales
+    alignas(16) float sx[8][256];                             // each epilogue warp's copy of a tile's token scales
 };
 
+// Without a residual res is -0: adding it changes no value.
+QMOE_DEV float finish(int sum, float sx, float sw, float res) {
+    return __fadd_rn(__fmul_rn(__fmul_rn((float)sum, sx), sw), res);
+}
 template <bool BF16>
-QMOE_DEV void finish(const Int8GemmParams &p, int64_t t, int n, int sum, float sx, float sw, float res) {
-    const int64_t at = t * p.N + n;
-    float y = __fmul_rn(__fmul_rn((float)sum, sx), sw);
-    if (p.residual) y = __fadd_rn(y, res);
-    if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(y);
-    else reinterpret_cast<float *>(p.y)[at] = y;
+QMOE_DEV void store1(void *out, int64_t at, float y) {
+    if (BF16) reinterpret_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(y);
+    else reinterpret_cast<float *>(out)[at] = y;
+}
+
+// A lane's channel of rows row .. row + CH - 1 (up to `count`) of the residual
+// at `at`, all in flight at once.
+template <bool BF16, int CH>
+QMOE_DEV void load_rows(const void *residual, int64_t at, int N, int row, int count, float (&res)[CH]) {
+    if (row + CH <= count) {
+        at += (int64_t)row * N;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) res[j] = load1<BF16>(residual, at + (int64_t)j * N);
+    } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (row + j < count) res[j] = load1<BF16>(residual, at + (int64_t)(row + j) * N);
+    }
 }
 
 QMOE_DEV void cluster_barrier() {
@@ -183,7 +207,7 @@ QMOE_DEV int load_cluster(const int *at, int rank) {
 }
 
 template <int BN, bool BF16>
-__global__ void __launch_bounds__(kThreads, Tile<BN>::ctas)
+__global__ void __launch_bounds__(Tile<BN>::threads, Tile<BN>::ctas)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                  const Int8GemmParams p, const int parts) {
     using Cfg = Tile<BN>;
@@ -207,7 +231,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&S->dfull[i], 1);
-            mbar_init(&S->dempty[i], 4);
+            mbar_init(&S->dempty[i], Cfg::epilogue);
         }
         mbar_init(&S->drain, 1);
         S->abort = 0;
@@ -287,18 +311,26 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
         }
         __syncwarp();
     } else if (warp >= 4) {
-        constexpr int CH = BN < 32 ? 16 : 32;
-        const int q = warp & 3;
+        // chunks of tokens, dealt to the warps of a quarter of tensor memory
+        constexpr int CH = BN < 32 ? 16 : 32, kStep = CH * (Cfg::epilogue / 4);
+        const int q = warp & 3, c0 = CH * ((warp - 4) >> 2);
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        const bool adds = parts == 1 && p.residual;
+        const int N = (int)p.N;
+        float *sx = S->sx[warp - 4];
         uint32_t i = 0;
         bool ok = true;
         QMOE_PDL_WAIT();
         for (int tile = tile0; ok && tile < total; tile += step, ++i) {
             const int64_t t0 = (int64_t)(tile % tiles_t) * BN;
-            const int n = (tile / tiles_t) * 128 + q * 32 + lane;
+            const int n = (tile / tiles_t) * 128 + q * 32 + lane, nn = n < p.N ? n : p.N - 1;
             const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
-            const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
-            float *sx = S->sx[q];
+            const int64_t at = t0 * p.N + nn;
+            const float sw = __ldg(p.sw + nn);
+            float next[CH];                       // residual of the chunk to come
+#pragma unroll
+            for (int j = 0; j < CH; ++j) next[j] = -0.0f;
+            if (adds) load_rows<BF16>(p.residual, at, N, c0, count, next);
             __syncwarp();
             for (int j = lane; j < count; j += 32) sx[j] = p.sx[t0 + j];
             __syncwarp();
@@ -306,37 +338,44 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
             tc_fence_after();
             // rolled: a tile's code stays small beside the other warps'
 #pragma unroll 1
-            for (int c = 0; c < count; c += CH) {
-                float res[CH];
-                if (parts == 1 && p.residual) {   // all in flight at once; rows and channels past the end read the last
-                    const int64_t nn = n < p.N ? n : p.N - 1;
-#pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        res[j] = load1<BF16>(p.residual, (t0 + (c + j < count ? c + j : count - 1)) * p.N + nn);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < CH; ++j) res[j] = 0.0f;
-                }
+            for (int c = c0; c < count; c += kStep) {
                 uint32_t v[CH];
                 if constexpr (CH == 32) tmem_ld_x32(tmem + lane_addr + (i & 1) * BN + c, v);
                 else tmem_ld_x16(tmem + lane_addr + (i & 1) * BN + c, v);
+                float res[CH];
+#pragma unroll
+                for (int j = 0; j < CH; ++j) res[j] = next[j];
+                if (adds) load_rows<BF16>(p.residual, at, N, c + kStep, count, next);
                 tmem_wait_ld();
-                if (c + CH >= count) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&S->dempty[i & 1]);
-                }
                 if (parts > 1) {                  // every MMA has read its operands: the ring is free
                     int *sums = reinterpret_cast<int *>(ring);
 #pragma unroll
                     for (int j = 0; j < CH; ++j) sums[(c + j) * 128 + q * 32 + lane] = (int)v[j];
-                } else if (n < p.N) {
+                } else {
+                    float y[CH];
 #pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        if (c + j < count) finish<BF16>(p, t0 + c + j, n, (int)v[j], sx[c + j], sw, res[j]);
+                    for (int j = 0; j < CH; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(sx + c + j);
+                        y[j] = finish((int)v[j], f.x, sw, res[j]);
+                        y[j + 1] = finish((int)v[j + 1], f.y, sw, res[j + 1]);
+                        y[j + 2] = finish((int)v[j + 2], f.z, sw, res[j + 2]);
+                        y[j + 3] = finish((int)v[j + 3], f.w, sw, res[j + 3]);
+                    }
+                    const int64_t first = at + (int64_t)c * N;
+                    if (n < p.N && c + CH <= count) {
+#pragma unroll
+                        for (int j = 0; j < CH; ++j) store1<BF16>(p.y, first + (int64_t)j * N, y[j]);
+                    } else if (n < p.N) {
+#pragma unroll
+                        for (int j = 0; j < CH; ++j)
+                            if (c + j < count) store1<BF16>(p.y, first + (int64_t)j * N, y[j]);
+                    }
                 }
                 __syncwarp();
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->dempty[i & 1]);
         }
     }
 
@@ -355,12 +394,13 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
         const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
         const int *sums = reinterpret_cast<const int *>(ring);
         const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
-        for (int j = rank + parts * (tid >> 7); j < count; j += 2 * parts) {
+        for (int j = rank + parts * (tid >> 7); j < count; j += Cfg::threads / 128 * parts) {
             int sum = 0;
             for (int r = 0; r < parts; ++r) sum += load_cluster(sums + j * 128 + (tid & 127), r);
             if (n < p.N)
-                finish<BF16>(p, t0 + j, n, sum, p.sx[t0 + j], sw,
-                             p.residual ? load1<BF16>(p.residual, (t0 + j) * p.N + n) : 0.0f);
+                store1<BF16>(p.y, (t0 + j) * p.N + n,
+                             finish(sum, p.sx[t0 + j], sw,
+                                    p.residual ? load1<BF16>(p.residual, (t0 + j) * p.N + n) : -0.0f));
         }
         cluster_barrier();                        // the others may still read this CTA's sums
     }
@@ -399,7 +439,7 @@ cudaError_t launch_bn(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const In
     const int64_t grid = parts > 1 ? total * parts : total < room ? total : room;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(Cfg::threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -427,6 +467,7 @@ cudaError_t launch_quant_rows(const Int8RowsParams &p, cudaStream_t s) {
     if (!vec) return p.ldc <= 1024 ? launch_rows<32, 0>(p, s) : launch_rows<256, 0>(p, s);
     if (p.ldc <= 512) return launch_rows<32, 2>(p, s);
     if (p.ldc <= 2048) return launch_rows<128, 2>(p, s);
+    if (p.ldc <= 4096) return launch_rows<256, 2>(p, s);
     if (p.ldc <= 8192) return launch_rows<512, 2>(p, s);
     if (p.ldc <= 16384) return launch_rows<1024, 2>(p, s);
     return launch_rows<1024, 0>(p, s);
