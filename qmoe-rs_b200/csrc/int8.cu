@@ -99,10 +99,8 @@ quant_rows_kernel(const Int8RowsParams p) {
         for (int q = 0; q < GROUPS; ++q) {
             const int k = (q * THREADS + tid) * 8;
             if (k >= p.ldc) continue;
-            int c[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = code8(v[q][j], 127.0f, r, mi);
-            *reinterpret_cast<uint2 *>(o + k) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+            *reinterpret_cast<uint2 *>(o + k) = make_uint2(codes4(v[q][0], v[q][1], v[q][2], v[q][3], 127.0f, r, mi),
+                                                           codes4(v[q][4], v[q][5], v[q][6], v[q][7], 127.0f, r, mi));
         }
     } else {
         for (int k = tid; k < p.ldc; k += THREADS)

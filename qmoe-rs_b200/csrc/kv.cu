@@ -152,9 +152,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanParam
 // when it did not grow), the new ones written.
 //
 // One warp a run, head and side (K or V).  It reads its rows twice, the second
-// time from L1 or L2: bound by HBM for prompts (two prompts of 4099 tokens, 16
-// heads of 192 and 128, f32: 210 MB) and by the latency of that chain of loads
-// for single tokens.  A warp looks for runs that start among `span` rows, one
+// time from L1 or L2: bound by HBM for prompts (two prompts of up to 4099
+// tokens, 16 heads of 192 and 128, f32: 146 MB) and by the latency of that chain of loads
+// for single tokens.  Three CTAs an SM hide the loads best (those prompts, 5720
+// rows of them, take 51 us; with two 55, with four, whose registers hold fewer
+// loads in flight, 53).  A warp looks for runs that start among `span` rows, one
 // row where rows are few.
 
 constexpr int kAppendWarps = 8;
@@ -237,8 +239,8 @@ QMOE_DEV void append_k(const KvAppendParams &p, int8_t *codes, float *range, int
                 const int e = e0 + 32 * k + lane, i = e / kPer;
                 if (e >= off * kPer) continue;
                 *place(i, (e - i * kPer) * 4) =
-                    pack4(code8((float)get_byte(w[k], 0), old, r, oi), code8((float)get_byte(w[k], 1), old, r, oi),
-                          code8((float)get_byte(w[k], 2), old, r, oi), code8((float)get_byte(w[k], 3), old, r, oi));
+                    codes4((float)get_byte(w[k], 0), (float)get_byte(w[k], 1), (float)get_byte(w[k], 2),
+                           (float)get_byte(w[k], 3), old, r, oi);
             }
         }
     }
@@ -253,8 +255,7 @@ QMOE_DEV void append_k(const KvAppendParams &p, int8_t *codes, float *range, int
         for (int k = 0; k < kAhead; ++k) {
             const int e = e0 + 32 * k + lane, i = e / kPer;
             if (e < n * kPer)
-                *place(off + i, (e - i * kPer) * 4) = pack4(code8(v[k].x, 127.0f, r, mi), code8(v[k].y, 127.0f, r, mi),
-                                                            code8(v[k].z, 127.0f, r, mi), code8(v[k].w, 127.0f, r, mi));
+                *place(off + i, (e - i * kPer) * 4) = codes4(v[k].x, v[k].y, v[k].z, v[k].w, 127.0f, r, mi);
         }
     }
 }
@@ -303,8 +304,7 @@ QMOE_DEV void append_v(const KvAppendParams &p, int8_t *codes, float *range, int
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    w[i] = pack4(code8(x[4 * i], 127.0f, r, mi), code8(x[4 * i + 1], 127.0f, r, mi),
-                                 code8(x[4 * i + 2], 127.0f, r, mi), code8(x[4 * i + 3], 127.0f, r, mi));
+                    w[i] = codes4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], 127.0f, r, mi);
                 *reinterpret_cast<uint4 *>(codes + (g * DIM + d) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else {
@@ -323,7 +323,7 @@ QMOE_DEV void append_v(const KvAppendParams &p, int8_t *codes, float *range, int
 }
 
 template <bool BF16, int DK, int DV>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(const KvAppendParams p, int span) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(const KvAppendParams p, int span) {
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int lane = threadIdx.x & 31;
