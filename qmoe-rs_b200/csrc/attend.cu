@@ -666,7 +666,8 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     const bool prompts = several && BF16;         // the requests of more than more.tq tokens
     if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, more.tq, s);
     if (e == cudaSuccess && several) {
-        // often none: a grid that the device holds at once looks through the slots
+        // often none: a bounded grid looks through the slots (eight CTAs an SM: 5
+        // requests of 2 tokens at 256 heads 102 us, with two 113)
         const int64_t n = BF16 ? p.R : p.T / more.tq + p.R;
         int64_t grid = 8 * (int64_t)device_sm_count() / ((int64_t)p.c.heads * more.hgroups * p.splits);
         grid = grid < 1 ? 1 : grid < n ? grid : n;

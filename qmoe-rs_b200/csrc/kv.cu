@@ -154,13 +154,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanParam
 // One warp a run, head and side (K or V).  It reads its rows twice, the second
 // time from L1 or L2: bound by HBM for prompts (two prompts of up to 4099
 // tokens, 16 heads of 192 and 128, f32: 146 MB) and by the latency of that chain of loads
-// for single tokens.  Three CTAs an SM hide the loads best (those prompts, 5720
-// rows of them, take 51 us; with two 55, with four, whose registers hold fewer
-// loads in flight, 53).  A warp looks for runs that start among `span` rows, one
+// for single tokens.  Four CTAs an SM with four loads in flight a lane hide them
+// best (those prompts, 5720 rows of them, take 49 us, 64 single tokens 3.5; three
+// CTAs with eight loads 51 and 3.9, two 55 and 3.8).  A warp looks for runs that start among `span` rows, one
 // row where rows are few.
 
 constexpr int kAppendWarps = 8;
-constexpr int kAhead = 8;                          // loads in flight a lane
+constexpr int kAhead = 4;                          // loads in flight a lane
 
 template <bool BF16>
 QMOE_DEV float4 load4(const void *x, int64_t i, bool vec) {
@@ -323,7 +323,7 @@ QMOE_DEV void append_v(const KvAppendParams &p, int8_t *codes, float *range, int
 }
 
 template <bool BF16, int DK, int DV>
-__global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(const KvAppendParams p, int span) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) kv_append_kernel(const KvAppendParams p, int span) {
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int lane = threadIdx.x & 31;

@@ -150,3 +150,24 @@ def test_large_matches_exact_integers():
     x[:, 0] = 127
     y = w.forward(x.cuda()).cpu()
     assert np.array_equal(y.numpy(), (x.double() @ codes.double().T).numpy())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("t,k,n", [(2000, 96, 5000), (700, 130, 4200), (301, 2624, 64), (190, 5000, 4097)])
+def test_wide_products_add_in_place(dtype, t, k, n):
+    """Tiles of 256 and 128 tokens, several a CTA, with ragged ends both ways and a
+    residual that is the output itself."""
+    from qmoe_b200 import Int8Tensor
+    dt = DT[dtype]
+    codes, scales = weights(n, k, t)
+    x, res = rows(t, k, dt, n), rows(t, n, dt, 9)
+    w = Int8Tensor.from_bytes(codes.cuda(), (n, k), scales.cuda())
+    y = res.cuda()
+    fresh = w.forward(x.cuda(), residual=y)
+    w.forward(x.cuda(), residual=y, out=y)
+    assert torch.equal(y, fresh)
+    plain, want = ref.product(x, codes, scales), ref.product(x, codes, scales, res)
+    # five f32 roundings of the parts, one of the result
+    tol = (plain.abs() + res.double().abs()) * 6 * 2.0 ** -24 + want.abs() * torch.finfo(dt).eps / 2 * 1.01
+    assert (y.cpu().double() - want).abs().le(tol).all()
+    check_product(w.forward(x.cuda()), plain, dt, k)

@@ -375,3 +375,31 @@ def test_attend_of_nothing():
     none = cache.attend(q, i32([0, 3]), i32([0]), torch.empty(1, 0, dtype=torch.int32, device="cuda"))
     assert (none == 0).all()
     cache.append(q[:0, :2], q[:0, :2], e)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(16, 16, 8, 64, 64), (64, 8, 4, 128, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("lens", [[(310, 300), (1, 1), (3, 2), (60, 7), (260, 259)], [(700, 650), (90, 1), (40, 40)]])
+def test_attend_prompts_that_fill_the_device(dtype, shape, lens):
+    """Query tiles by the hundred, with every other kind of request beside them,
+    written by a launch right in front and read by one right behind."""
+    bs, H, G, dk, dv = shape
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, lens, 8, pad=2, spread=1.0)
+    q[starts[-1]:] = 0.0
+    args = i32(starts), i32(kv), i32([x for r in table for x in r], len(table), len(table[0]))
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, ref.new_scale(dk), torch.zeros(q.shape[0], H * G, dv, dtype=torch.float64))
+    src, out = q.cuda(), torch.zeros(q.shape[0], H * G, dv, dtype=q.dtype, device="cuda")
+    graph, side, buf = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.empty_like(src)
+    copies = [torch.empty_like(out) for _ in range(3)]
+    with torch.cuda.graph(graph, stream=side):
+        for c in copies:
+            buf.copy_(src)
+            cache.attend(buf, *args, out=out)
+            c.copy_(out)
+            buf.fill_(float("nan"))
+            out.zero_()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    check_attend(copies[0], want, flat[3], dtype)
+    assert torch.equal(copies[0], copies[1]) and torch.equal(copies[0], copies[2])
