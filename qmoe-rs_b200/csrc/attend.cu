@@ -68,8 +68,9 @@ QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int
 }
 
 // What the slots of a launch are: tokens, where each request has one at most;
-// requests with one token; requests with 2 .. tq; tiles of tq tokens of the
-// requests with more than one.
+// requests with one token; `tiles` tiles of tq tokens for each request, of those
+// with that many tokens at most; tiles of tq tokens of the requests with
+// more than one.
 enum class Slots { kTokens, kSingles, kFew, kTiles };
 
 struct Rows {                                    // of one CTA: rows of one request and kv head
@@ -80,12 +81,12 @@ struct Rows {                                    // of one CTA: rows of one requ
     int64_t request;
 };
 
-QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind, Rows &w) {
+QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind, int tiles, Rows &w) {
     const bool by_request = kind == Slots::kSingles || kind == Slots::kFew;
-    const int64_t r = by_request ? slot : find_request(p.q_start, p.R, slot, tq);
+    const int64_t r = kind == Slots::kFew ? slot / tiles : by_request ? slot : find_request(p.q_start, p.R, slot, tq);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    if (kind == Slots::kSingles ? n != 1 : kind == Slots::kFew ? n < 2 || n > tq : kind == Slots::kTiles && n < 2) return false;
-    const int64_t i0 = by_request ? 0 : (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
+    if (kind == Slots::kSingles ? n != 1 : kind == Slots::kFew ? n < 2 || n > tiles * tq : kind == Slots::kTiles && n < 2) return false;
+    const int64_t i0 = kind == Slots::kFew ? slot % tiles * tq : by_request ? 0 : (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
     if (i0 < 0 || i0 >= n || s0 < 0) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
     w.t0 = s0 + i0;
@@ -513,7 +514,8 @@ __host__ __device__ constexpr int ctas_per_sm(int dk, bool bf16, int nt) { retur
 // Up to tq tokens of a request by gq heads of a kv head, on NT * 8 columns.
 template <int DK, int DV, bool BF16, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(DK, BF16, NT))
-attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int64_t slots, bool beside) {
+attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int tiles, int64_t slots,
+              bool beside) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Shared<DK, DV, NT> &S = *reinterpret_cast<Shared<DK, DV, NT> *>(smem_raw);
     if (!beside) QMOE_PDL_WAIT();
@@ -530,7 +532,7 @@ attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int
     uint32_t done = 0;                            // items of this warp's ring so far
     for (int64_t slot = blockIdx.x; slot < slots; slot += gridDim.x) {
         Rows w;
-        if (!find_rows(p, slot, tq, kind, w)) continue;                  // the whole CTA alike
+        if (!find_rows(p, slot, tq, kind, tiles, w)) continue;           // the whole CTA alike
         w.head0 = h * G + hg * gq;
         attend_rows<DK, DV, BF16, NT>(p, w, h, blockIdx.z, gq, heads_here, S, done);
         if (slot + gridDim.x < slots) {           // the ring is written by copies again
@@ -547,7 +549,7 @@ constexpr int kJoinWarps = 4;
 constexpr int kMaxSplits = 256;
 
 template <int DV, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p, int tq,
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p, int few,
                                                                        bool by_request) {
     constexpr int kPer = DV / 32;
     __shared__ float weight[kMaxSplits];
@@ -555,16 +557,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // the tokens of request blockIdx.x, or token blockIdx.x
-    int64_t t = blockIdx.x, t_hi = t + 1;
+    // every gridDim.x / R-th token of a request, or token blockIdx.x
+    int64_t t = blockIdx.x, t_hi = t + 1, step = 1;
     if (by_request) {
-        t = p.q_start[blockIdx.x];
-        t_hi = p.q_start[blockIdx.x + 1];
-        if (t_hi - t > tq || t < 0) return;
+        step = gridDim.x / p.R;
+        const int64_t r = blockIdx.x / step, first = p.q_start[r];
+        t_hi = p.q_start[r + 1];
+        if (t_hi - first > few || first < 0) return;
+        t = first + blockIdx.x % step;
     }
     const int64_t rows = p.q_start[p.R] < p.T ? p.q_start[p.R] : p.T;
     t_hi = t_hi < rows ? t_hi : rows;
-    for (; t < t_hi; ++t) {
+    for (; t < t_hi; t += step) {
     const int64_t row = t * p.heads + blockIdx.y;
     const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + row * p.splits;
     const float *part = p.ws + p.T * p.heads * p.splits * 2 + row * p.splits * DV;
@@ -637,14 +641,14 @@ RowShape row_shape(bool single, int G, int dtype) {
 }
 
 template <int DK, int DV, bool BF16, int NT>
-cudaError_t launch_nt(const AttendParams &p, const RowShape &r, Slots kind, int64_t slots, int64_t grid, bool beside,
+cudaError_t launch_nt(const AttendParams &p, const RowShape &r, Slots kind, int tiles, int64_t slots, int64_t grid, bool beside,
                       cudaStream_t s) {
     const size_t smem = sizeof(Shared<DK, DV, NT>);
     auto kernel = attend_kernel<DK, DV, BF16, NT>;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)grid, (unsigned)(p.c.heads * r.hgroups), (unsigned)p.splits), dim3(kThreads),
-                      smem, s, p, r.tq, r.gq, r.hgroups, kind, slots, beside);
+                      smem, s, p, r.tq, r.gq, r.hgroups, kind, tiles, slots, beside);
 }
 
 template <int DK, int DV, bool BF16>
@@ -655,27 +659,43 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     const RowShape one = row_shape(true, G, p.dtype), more = row_shape(false, G, p.dtype);
     const Slots kind = several ? Slots::kSingles : Slots::kTokens;
     const int64_t slots = several ? p.R : p.T;
-    cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, slots, slots, false, s)
-                    : one.nt == 2 ? launch_nt<DK, DV, BF16, 2>(p, one, kind, slots, slots, false, s)
-                                  : launch_nt<DK, DV, BF16, kMost>(p, one, kind, slots, slots, false, s);
+    cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, 1, slots, slots, false, s)
+                    : one.nt == 2 ? launch_nt<DK, DV, BF16, 2>(p, one, kind, 1, slots, slots, false, s)
+                                  : launch_nt<DK, DV, BF16, kMost>(p, one, kind, 1, slots, slots, false, s);
     // The kinds of requests are launches side by side: a launch may start once
     // every CTA of the one before has, which the first does only after its wait
     // for what came before this call; so the others read nothing too early.  They
     // wait for the launch before them at their end, so that what comes after the
     // last has all of them behind it.
-    const bool prompts = several && BF16;         // the requests of more than more.tq tokens
-    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, more.tq, s);
+    const bool prompts = several && BF16;         // the requests of more than `few` tokens
+    // Up to 32 tokens (a tile of the prompts' kernel at most) stay here, where their
+    // keys are cut into pieces, while the batch is small: 6 requests of up to 9
+    // tokens after 3756, 8 heads to a kv head, 34 us, by the prompts' kernel 102.  In
+    // larger ones only a tile does: the search for such requests costs single tokens
+    // 5 us (64 of them), and 63 requests of up to 231 tokens take 43 us instead of 35
+    // with up to 64 tokens here.
+    const int64_t cap = 8 * (int64_t)device_sm_count(), each = (int64_t)p.c.heads * more.hgroups * p.splits;
+    int tiles = more.tq >= 32 ? 1 : more.tq > 8 ? 32 / more.tq : 4;
+    if (p.R * tiles * each > 2 * cap) tiles = 1;
+    const int few = tiles * more.tq;
+    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, few, s);
     if (e == cudaSuccess && several) {
         // often none: a bounded grid looks through the slots (eight CTAs an SM: 5
         // requests of 2 tokens at 256 heads 102 us, with two 113)
-        const int64_t n = BF16 ? p.R : p.T / more.tq + p.R;
-        int64_t grid = 8 * (int64_t)device_sm_count() / ((int64_t)p.c.heads * more.hgroups * p.splits);
+        const int64_t n = BF16 ? p.R * tiles : p.T / more.tq + p.R;
+        int64_t grid = (tiles > 1 ? 2 * cap : cap) / each;
         grid = grid < 1 ? 1 : grid < n ? grid : n;
-        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, n, grid, true, s);
+        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, tiles, n, grid, true, s);
     }
-    if (e == cudaSuccess && p.splits > 1)
-        e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)(prompts ? p.R : p.T), (unsigned)p.heads),
-                       dim3(kJoinWarps * 32), 0, s, p, more.tq, prompts);
+    if (e == cudaSuccess && p.splits > 1) {
+        int64_t grid = p.T;
+        if (prompts) {                            // a request's tokens side by side while the device has room
+            const int64_t room = 8 * (int64_t)device_sm_count() / (p.R * p.heads);
+            grid = p.R * (room < 1 ? 1 : room < few ? room : few);
+        }
+        e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)grid, (unsigned)p.heads), dim3(kJoinWarps * 32), 0, s, p,
+                       few, prompts);
+    }
     return e;
 }
 
