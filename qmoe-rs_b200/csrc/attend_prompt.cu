@@ -26,7 +26,7 @@
 // reaches 2^(8 + 6), which fp16 holds).  For 256 rows by 128 keys of 128 dims the
 // exponentials take 2048 cycles of an SM (16 a cycle) and the MMAs as many.
 // Measured: three prompts of up to 2048 tokens after up to 6000, 32 query and 8 kv
-// heads of 128, 352 us = 710 TFLOP/s, the tensor pipe busy 37 % of the time: the
+// heads of 128, 356 us = 700 TFLOP/s, the tensor pipe busy 37 % of the time: the
 // chain score, softmax, P V of two query tiles and the barriers between its warps
 // bound it, then the tail of 256 long items on 148 SMs.
 #include "attend.cuh"
