@@ -81,13 +81,15 @@ def quantize_int8(x, ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
     dt = _code(x)
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    rows, cols = x.shape
+    stride, unit = x.stride()
+    if unit != 1 or stride < cols:                # rows that repeat or overlap (expand, unfold) as well
         x = x.contiguous()
+        stride = cols
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
     _use_stream(ctx)
-    capi.call("qmoe_quantize_int8", ctx.handle, x.data_ptr(), dt, x.shape[0], x.shape[1],
-              max(x.stride(0), x.shape[1]), codes.data_ptr(), scales.data_ptr())
+    capi.call("qmoe_quantize_int8", ctx.handle, x.data_ptr(), dt, rows, cols, stride, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
