@@ -349,6 +349,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         for (int x = 0; x < NT; ++x) {
             float top[2] = {neg_inf(), neg_inf()};
             const float f[2] = {ks * back[x][0], ks * back[x][1]};
+            float ic[2] = {iv, iv};               // NaN for a poisoned group: 0 where this lane's rows see nothing of it
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -356,8 +357,10 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
             if (!whole) {
                 int see[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i) {
                     see[i] = blk >= 0 ? (last[x][i] < w.keys - 1 ? last[x][i] : w.keys - 1) - tg : -1;
+                    ic[i] = see[i] < 0 ? 0.0f : iv;
+                }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -384,7 +387,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[u][x][i] = ex2(s[u][x][i] - base[i & 1]);
-                    sum[x][i & 1] = __fmaf_rn(s[u][x][i], iv, sum[x][i & 1]);
+                    sum[x][i & 1] = __fmaf_rn(s[u][x][i], ic[i & 1], sum[x][i & 1]);
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {

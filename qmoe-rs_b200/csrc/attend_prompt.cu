@@ -351,9 +351,11 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         // the group's factors: a > 0, so that a masked score of -inf stays one (a
-                        // poisoned group's NaN is in lv); b takes the 1152 off the codes
+                        // poisoned group's NaN is in lv); b takes the 1152 off the codes.  A row that
+                        // sees none of the group takes neither its lv nor its iv, which may be NaN.
+                        const bool seen = 16 * x <= see;
                         const float a = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
-                        const float b = __fmaf_rn(bias, a, S.lv[u % kScaleRing][x]) - base;
+                        const float b = __fmaf_rn(bias, a, seen ? S.lv[u % kScaleRing][x] : neg_inf()) - base;
                         const uint64_t aa = pair(a, a), bb = pair(b, b);
                         uint64_t acc = pair(0.0f, 0.0f);
                         m4[x] = neg_inf();
@@ -369,7 +371,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
                         }
                         float p0, p1;
                         unpair(acc, p0, p1);
-                        total = __fmaf_rn(p0 + p1, S.iv[u % kScaleRing][x], total);
+                        total = __fmaf_rn(p0 + p1, seen ? S.iv[u % kScaleRing][x] : 0.0f, total);
                     }
                     top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
                     return total;
@@ -379,7 +381,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
                 const bool grow = mx == neg_inf() ? top != neg_inf() : top > kGrow + kShift;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float to = top + (mx == neg_inf() ? 0.0f : mx - kShift);   // the tile's largest
-                    const float now = to > mx ? to : mx;
+                    const float now = grow ? to : mx;    // a row's bits do not depend on the warp's other rows
                     const float by = now == neg_inf() ? 1.0f : ex2(mx - now);
                     mx = now;
                     sum *= by;

@@ -26,3 +26,60 @@ def test_quantize_views_whose_rows_repeat_or_overlap(dtype):
     w = Int8Tensor.from_float(views[1])
     assert w.shape == tuple(views[1].shape)
     assert torch.equal(w.forward(x[:128][None]), Int8Tensor.from_float(views[1].contiguous()).forward(x[:128][None]))
+
+
+# ---- attention: poisoned blocks and rows of nobody --------------------------------
+
+def attend_case(dtype, bs, H, G, dk, dv, lens, seed, pad=0, spread=1.0, ranges=(0.5, 3.5)):
+    """A cache, its 64-bit parts, q and the lists of a batch; lens: (kv tokens, new tokens)."""
+    from qmoe_b200 import KVCache
+    g = torch.Generator().manual_seed(seed)
+    blocks = [-(-kv // bs) for kv, _ in lens]
+    nb, width = sum(blocks) + 2, max(blocks + [0]) + 1
+    k = torch.randint(-127, 128, (nb, H, dk // 64, bs, 64), generator=g, dtype=torch.int8)
+    v = torch.randint(-127, 128, (nb, H, bs // 16, dv, 16), generator=g, dtype=torch.int8)
+    kr, vr = (torch.rand(nb, H, generator=g) * (ranges[1] - ranges[0]) + ranges[0] for _ in range(2))
+    ids = torch.randperm(nb, generator=g).tolist()
+    table = [[ids.pop() for _ in range(b)] + [-1] * (width - b) for b in blocks]
+    starts = [0]
+    for _, n in lens:
+        starts.append(starts[-1] + n)
+    q = (torch.randn(starts[-1] + pad, H * G, dk, generator=g) * spread).to(DT[dtype])
+    cache = KVCache.from_tensors(k.cuda(), v.cuda(), kr.cuda(), vr.cuda())
+    return cache, (ref.k_flat(k), kr, ref.v_flat(v), vr), q, starts, [kv for kv, _ in lens], table
+
+
+def device_args(starts, kv, table):
+    return i32(starts), i32(kv), i32([x for r in table for x in r], len(table), len(table[0]))
+
+
+# requests of one kind each beside a single token: tiles of the matrix kernel and
+# few tokens' rows (bf16), the streaming kernel's tiles (f32)
+POISONED = [[(300, 300), (5, 1)], [(700, 100), (5, 1)], [(90, 9), (5, 1)], [(40, 7), (5, 1)], [(86, 9), (5, 1)], [(35, 7), (5, 1)]]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", POISONED, ids=str)
+@pytest.mark.parametrize("shape", [(16, 2, 1, 64, 64), (16, 1, 4, 128, 128), (32, 2, 2, 192, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_poison_reaches_only_rows_that_see_it(dtype, shape, lens, which):
+    """A block whose range is NaN, in the middle of a request's new tokens and at
+    their end: the tokens before it keep their bits."""
+    bs, H, G, dk, dv = shape
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, lens, 21)
+    args = device_args(starts, kv, table)
+    clean = cache.attend(q.cuda(), *args)
+    assert not clean.isnan().any()
+    total, new = lens[0]
+    for token in (total - 1, total - 1 - new // 2):
+        block = token // bs
+        ranges = getattr(cache, which + "_range")
+        old = ranges[table[0][block], H - 1].item()
+        ranges[table[0][block], H - 1] = float("nan")
+        got = cache.attend(q.cuda(), *args)
+        ranges[table[0][block], H - 1] = old
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        first = max(0, block * bs - (total - new))   # the first new token that sees the block
+        bad[first:new, (H - 1) * G:] = True
+        assert got[bad].isnan().all()
+        assert torch.equal(got[~bad], clean[~bad])
