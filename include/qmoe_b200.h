@@ -555,9 +555,9 @@ QMOE_API int qmoe_kv_append(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const voi
  * attends to the tokens 0 .. kv_lens[r] - n + i:
  *   out[row, h] = sum_j softmax_j(scale * q[row, h] . k[j, h / (heads / kv_heads)]) v[j, ...]
  * One token a request is the decode step, more a prompt or a chunk of one.  A
- * row that sees no token (kv_lens 0) gives zeros; rows from q_start[requests]
- * on are left as they were; a table entry that is not a block of the cache
- * hides its tokens.  out [T, heads, v_dim], tokens out_stride elements apart.
+ * row that sees no token (kv_lens 0) gives zeros; rows in front of q_start[0]
+ * and from q_start[requests] on are left as they were; a table entry that is
+ * not a block of the cache hides its tokens.  out [T, heads, v_dim], tokens out_stride elements apart.
  * heads is a multiple of kv_heads; T * heads < 2^31.  max_kv: the longest kv_lens if the caller
  * knows it, else 0 (max_blocks * block_size is taken); only the time depends
  * on it.  Repeated calls give the same bits. */

@@ -568,6 +568,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
         t_hi = p.q_start[r + 1];
         if (t_hi - first > few || first < 0) return;
         t = first + blockIdx.x % step;
+    } else if (t < p.q_start[0]) {                // nobody's: no piece was written
+        return;
     }
     const int64_t rows = p.q_start[p.R] < p.T ? p.q_start[p.R] : p.T;
     t_hi = t_hi < rows ? t_hi : rows;

@@ -324,8 +324,8 @@ class KVCache:
         """Causal attention of q [tokens, heads, k_dim] over the cache; rows
         q_start[r] .. q_start[r + 1] are the last tokens of request r, whose
         kv_lens[r] tokens are in the blocks of block_table[r].  -> [tokens, heads,
-        v_dim].  Rows that see nothing are zeros; rows past the last request are
-        left as `out` has them (zeros without one).  max_kv: the longest kv_lens
+        v_dim].  Rows that see nothing are zeros; rows in front of the first request
+        and past the last are left as `out` has them (zeros without one).  max_kv: the longest kv_lens
         if the host knows it (for speed alone)."""
         ctx = self.ctx
         _on(ctx, "q", q)

@@ -53,6 +53,18 @@ def device_args(starts, kv, table):
     return i32(starts), i32(kv), i32([x for r in table for x in r], len(table), len(table[0]))
 
 
+def check_rows(got, want, vr, dtype, slack=0.0):
+    """Element by element: half a step of the result, and of the largest value what
+    the weights may be off by, once each in numerator and denominator.  P in fp16:
+    2^-12 (two terms 2^-22).  Exponents: at most 16 additions in f32, each off by a
+    step, 2^-23 of a partial sum below 8: 2^-16.  `slack`: what a case adds to that."""
+    half = torch.finfo(DT[dtype]).eps / 2
+    w = (2.0 ** -12 if dtype == "bf16" else 2.0 ** -22) + 2.0 ** -16
+    err = (got.cpu().double() - want).abs()
+    bound = half * 1.01 * want.abs() + 2 * (w + slack) * vr.max().item()
+    assert (err <= bound).all(), ((err - bound).max().item(), err.max().item())
+
+
 # requests of one kind each beside a single token: tiles of the matrix kernel and
 # few tokens' rows (bf16), the streaming kernel's tiles (f32)
 POISONED = [[(300, 300), (5, 1)], [(700, 100), (5, 1)], [(90, 9), (5, 1)], [(40, 7), (5, 1)], [(86, 9), (5, 1)], [(35, 7), (5, 1)]]
@@ -83,3 +95,20 @@ def test_poison_reaches_only_rows_that_see_it(dtype, shape, lens, which):
         bad[first:new, (H - 1) * G:] = True
         assert got[bad].isnan().all()
         assert torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[(3000, 1), (1500, 1)], [(3000, 3), (1500, 1), (60, 40)], [(2000, 0), (1500, 1), (900, 2), (5, 0)]], ids=str)
+@pytest.mark.parametrize("first", [1, 6])
+def test_rows_in_front_of_the_first_request_stay(dtype, lens, first):
+    """A later part of a batch: q_start does not begin at 0, the rows before and behind it are others'."""
+    bs, H, G, dk, dv = 16, 2, 2, 128, 128
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, lens, 31, pad=first + 3)
+    starts = [s + first for s in starts]
+    live = slice(first, starts[-1])
+    q[:first] = q[starts[-1]:] = float("nan")
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, ref.new_scale(dk), torch.zeros(q.shape[0], H * G, dv, dtype=torch.float64))
+    out = torch.full((q.shape[0], H * G, dv), 0.25, dtype=q.dtype, device="cuda")
+    cache.attend(q.cuda(), *device_args(starts, kv, table), out=out)
+    assert (out[:first] == 0.25).all() and (out[starts[-1]:] == 0.25).all()
+    check_rows(out[live], want[live], flat[3], dtype)
