@@ -2335,9 +2335,7 @@ int qmoe_kv_attend_workspace(const qmoe_kv_cache *cache, int dtype, int64_t T, i
     QTRY(check_dtype(dtype));
     KvCacheDev c{};
     QTRY(check_attend(cache, c, T, requests, heads, max_blocks, max_kv));
-    int splits, chunk;
-    attend_pieces(c, T, requests, heads, dtype, max_kv, splits, chunk);
-    *bytes = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, c.v_dim, splits));
+    *bytes = (int64_t)(sizeof(float) * attend_cut(c, T, requests, heads, dtype, max_kv).floats);
     return QMOE_OK;
 }
 
@@ -2357,11 +2355,11 @@ int qmoe_kv_attend(qmoe_ctx *ctx, const qmoe_kv_cache *cache, const void *q, int
                     (long long)out_stride);
     if (!(scale == scale) || scale - scale != 0.0f) return fail(QMOE_ERR_INVALID, "scale must be finite");
     DeviceGuard g(ctx->device);
-    attend_pieces(p.c, T, requests, heads, dtype, max_kv, p.splits, p.chunk);
+    p.cut = attend_cut(p.c, T, requests, heads, dtype, max_kv);
     p.vec_q = reinterpret_cast<uintptr_t>(q) % (4 * dtype_size(dtype)) == 0 && q_stride % 4 == 0;
     p.vec_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_stride % 8 == 0;
     p.err = error_flag();
-    const int64_t need = (int64_t)(sizeof(float) * attend_workspace_floats(T, heads, p.c.v_dim, p.splits));
+    const int64_t need = (int64_t)(sizeof(float) * p.cut.floats);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
         return fail(QMOE_ERR_INVALID, "workspace of %lld bytes (16-byte aligned), %lld needed",
                     (long long)workspace_bytes, (long long)need);

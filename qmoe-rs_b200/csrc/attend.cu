@@ -79,6 +79,7 @@ struct Rows {                                    // of one CTA: rows of one requ
     int pos0;                                    // last key of token t0 (may be negative)
     int keys;                                    // keys of the last token
     int64_t request;
+    int64_t scratch;                             // row of scratch of token t0
 };
 
 QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind, int tiles, Rows &w) {
@@ -97,6 +98,7 @@ QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind,
     const int64_t pos0 = (kv < 0 ? 0 : kv) - n + i0;
     const int64_t keys = pos0 + cnt;             // one past the last token's last key
     w.request = r;
+    w.scratch = p.cut.by_token ? w.t0 : r * p.cut.few + i0;
     w.tokens = (int)cnt;
     w.pos0 = (int)(pos0 < -(1 << 30) ? -(1 << 30) : pos0);
     w.keys = (int)(keys < 0 ? 0 : keys > most ? most : keys);
@@ -164,8 +166,8 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     const int bs = p.c.block;
 
     const int tiles = (w.keys + 63) / 64;
-    // pieces of p.chunk tiles, larger where the request is longer than the host was told
-    const int even = (tiles + p.splits - 1) / p.splits, chunk = p.chunk > even ? p.chunk : even;
+    // pieces of cut.chunk tiles, larger where the request is longer than the host was told
+    const int even = (tiles + p.splits - 1) / p.splits, chunk = p.cut.chunk > even ? p.cut.chunk : even;
     const int t_lo = split * chunk, t_hi = t_lo + chunk < tiles ? t_lo + chunk : tiles;
     const int mine = t_hi > t_lo + warp ? (t_hi - t_lo - warp + kWarps - 1) / kWarps : 0;   // tiles of this warp
     const int32_t *row_table = p.table + w.request * p.max_blocks;
@@ -494,13 +496,13 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
                 if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
                 else reinterpret_cast<float *>(p.out)[at] = y;
             } else {
-                const int64_t at = (t * p.heads + head) * p.splits + split;
+                const int64_t at = ((w.scratch + i) * p.heads + head) * p.splits + split;
                 float *ml = p.ws + at * 2;
                 if (d == 0) {
                     ml[0] = m;
                     ml[1] = l;
                 }
-                p.ws[p.T * p.heads * p.splits * 2 + at * DV + d] = o;
+                p.ws[p.cut.rows * p.heads * p.splits * 2 + at * DV + d] = o;
             }
         }
     }
@@ -551,38 +553,57 @@ attend_kernel(const AttendParams p, int tq, int gq, int hgroups, Slots kind, int
 constexpr int kJoinWarps = 4;
 constexpr int kMaxSplits = 256;
 
+// How a CTA finds its tokens: every gridDim.x / R-th one of a request of up to
+// cut.few; token blockIdx.x; or that token, whose request says which of the two
+// kinds of pieces it has (`tile`: the second kind).
+enum class Joins { kRequests, kTokens, kBoth };
+
 template <int DV, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p, int few,
-                                                                       bool by_request) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendParams p, const AttendParams tile,
+                                                                       Joins kind) {
     constexpr int kPer = DV / 32;
     __shared__ float weight[kMaxSplits];
     __shared__ float red[kJoinWarps], part_sum[kJoinWarps][DV];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // Before the wait: q_start was written in front of this call's first launch,
+    // and this one starts after that has waited for it.
+    const int64_t rows = p.q_start[p.R] < p.T ? p.q_start[p.R] : p.T;
+    int64_t t = blockIdx.x, t_hi = t + 1, step = 1, scratch = t, scratch_rows = p.cut.rows;
+    int splits = p.splits;
+    const float *ws = p.ws;
+    if (kind == Joins::kRequests) {
+        step = gridDim.x / p.R;
+        const int64_t r = blockIdx.x / step, first = p.q_start[r], i = blockIdx.x % step;
+        t = first + i;
+        t_hi = p.q_start[r + 1];
+        if (t_hi - first > p.cut.few || first < 0) t_hi = 0;
+        scratch = p.cut.by_token ? t : r * p.cut.few + i;
+    } else if (t < p.q_start[0]) {                // nobody's: no piece was written
+        t_hi = 0;
+    } else if (kind == Joins::kBoth) {
+        const int64_t r = find_request(p.q_start, p.R, t, 1), first = p.q_start[r];
+        if (p.q_start[r + 1] - first > p.cut.few) {
+            splits = tile.splits;
+            ws = tile.ws;
+            scratch_rows = tile.cut.rows;
+            if (splits == 1) t_hi = 0;            // written in one piece
+        } else if (!p.cut.by_token) {
+            scratch = r * p.cut.few + t - first;
+        }
+    }
+    t_hi = t_hi < rows ? t_hi : rows;
     QMOE_PDL_WAIT();
     QMOE_PDL_TRIGGER();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // every gridDim.x / R-th token of a request, or token blockIdx.x
-    int64_t t = blockIdx.x, t_hi = t + 1, step = 1;
-    if (by_request) {
-        step = gridDim.x / p.R;
-        const int64_t r = blockIdx.x / step, first = p.q_start[r];
-        t_hi = p.q_start[r + 1];
-        if (t_hi - first > few || first < 0) return;
-        t = first + blockIdx.x % step;
-    } else if (t < p.q_start[0]) {                // nobody's: no piece was written
-        return;
-    }
-    const int64_t rows = p.q_start[p.R] < p.T ? p.q_start[p.R] : p.T;
-    t_hi = t_hi < rows ? t_hi : rows;
-    for (; t < t_hi; t += step) {
-    const int64_t row = t * p.heads + blockIdx.y;
-    const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + row * p.splits;
-    const float *part = p.ws + p.T * p.heads * p.splits * 2 + row * p.splits * DV;
+    for (; t < t_hi; t += step, scratch += step) {
+    const int64_t row = scratch * p.heads + blockIdx.y;
+    const float2 *ml = reinterpret_cast<const float2 *>(ws) + row * splits;
+    const float *part = ws + scratch_rows * p.heads * splits * 2 + row * splits * DV;
     float2 v[kMaxSplits / (kJoinWarps * 32)];
     float m = neg_inf();
 #pragma unroll
     for (int k = 0; k < kMaxSplits / (kJoinWarps * 32); ++k) {
         const int s = k * kJoinWarps * 32 + tid;
-        v[k] = s < p.splits ? ml[s] : make_float2(neg_inf(), 0.0f);
+        v[k] = s < splits ? ml[s] : make_float2(neg_inf(), 0.0f);
         m = fmaxf(m, v[k].x);
     }
     m = warp_max(m);
@@ -596,7 +617,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     for (int k = 0; k < kMaxSplits / (kJoinWarps * 32); ++k) {
         const int s = k * kJoinWarps * 32 + tid;
         const float f = m == neg_inf() ? 1.0f : ex2(v[k].x - m);
-        if (s < p.splits) weight[s] = f;
+        if (s < splits) weight[s] = f;
         l = __fmaf_rn(v[k].y, f, l);
     }
 #pragma unroll
@@ -610,7 +631,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
     for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
 #pragma unroll 4
-    for (int s = warp; s < p.splits; s += kJoinWarps) {
+    for (int s = warp; s < splits; s += kJoinWarps) {
         const float f = weight[s];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) o[j] = __fmaf_rn(part[(int64_t)s * DV + 32 * j + lane], f, o[j]);
@@ -660,8 +681,8 @@ template <int DK, int DV, bool BF16>
 cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     const int G = p.heads / p.c.heads;
     constexpr int kMost = most_columns(BF16);
-    const bool several = p.T > p.R;               // a request may have more than one token
     const RowShape one = row_shape(true, G, p.dtype), more = row_shape(false, G, p.dtype);
+    const bool several = p.cut.several;
     const Slots kind = several ? Slots::kSingles : Slots::kTokens;
     const int64_t slots = several ? p.R : p.T;
     cudaError_t e = one.nt == 1   ? launch_nt<DK, DV, BF16, 1>(p, one, kind, 1, slots, slots, false, s)
@@ -672,34 +693,30 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     // for what came before this call; so the others read nothing too early.  They
     // wait for the launch before them at their end, so that what comes after the
     // last has all of them behind it.
-    const bool prompts = several && BF16;         // the requests of more than `few` tokens
-    // Up to 32 tokens (a tile of the prompts' kernel at most) stay here, where their
-    // keys are cut into pieces, while the batch is small: 6 requests of up to 9
-    // tokens after 3756, 8 heads to a kv head, 34 us, by the prompts' kernel 102.  In
-    // larger ones only a tile does: the search for such requests costs single tokens
-    // 5 us (64 of them), and 63 requests of up to 231 tokens take 43 us instead of 35
-    // with up to 64 tokens here.
-    const int64_t cap = 8 * (int64_t)device_sm_count(), each = (int64_t)p.c.heads * more.hgroups * p.splits;
-    int tiles = more.tq >= 32 ? 1 : more.tq > 8 ? 32 / more.tq : 4;
-    if (p.R * tiles * each > 2 * cap) tiles = 1;
-    const int few = tiles * more.tq;
-    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, few, s);
+    const bool prompts = several && BF16;         // the requests of more than cut.few tokens
+    AttendParams tile = p;                        // those in f32: pieces of their own
+    tile.splits = p.cut.tile_splits;
+    tile.ws = p.ws ? p.ws + p.cut.rows * p.heads * p.splits * (DV + 2) : nullptr;
+    tile.cut.rows = p.T;
+    tile.cut.by_token = true;
+    if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, p.cut.few, s);
     if (e == cudaSuccess && several) {
         // often none: a bounded grid looks through the slots (eight CTAs an SM: 5
         // requests of 2 tokens at 256 heads 102 us, with two 113)
-        const int64_t n = BF16 ? p.R * tiles : p.T / more.tq + p.R;
-        int64_t grid = (tiles > 1 ? 2 * cap : cap) / each;
+        const int64_t n = BF16 ? p.R * p.cut.tiles : p.T / more.tq + p.R, cap = 8 * (int64_t)device_sm_count();
+        const AttendParams &q = BF16 ? p : tile;
+        int64_t grid = (p.cut.tiles > 1 ? 2 * cap : cap) / ((int64_t)p.c.heads * more.hgroups * q.splits);
         grid = grid < 1 ? 1 : grid < n ? grid : n;
-        e = launch_nt<DK, DV, BF16, kMost>(p, more, BF16 ? Slots::kFew : Slots::kTiles, tiles, n, grid, true, s);
+        e = launch_nt<DK, DV, BF16, kMost>(q, more, BF16 ? Slots::kFew : Slots::kTiles, p.cut.tiles, n, grid, true, s);
     }
     if (e == cudaSuccess && p.splits > 1) {
         int64_t grid = p.T;
         if (prompts) {                            // a request's tokens side by side while the device has room
             const int64_t room = 8 * (int64_t)device_sm_count() / (p.R * p.heads);
-            grid = p.R * (room < 1 ? 1 : room < few ? room : few);
+            grid = p.R * (room < 1 ? 1 : room < p.cut.few ? room : p.cut.few);
         }
         e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)grid, (unsigned)p.heads), dim3(kJoinWarps * 32), 0, s, p,
-                       few, prompts);
+                       tile, prompts ? Joins::kRequests : several ? Joins::kBoth : Joins::kTokens);
     }
     return e;
 }
@@ -709,12 +726,20 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
 // A batch of few CTAs is cut so that two an SM fill the device once (a request
 // of the longest length each); one of many into a piece's quarter of that,
 // since its requests may be of any length.
-void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
-                   int &chunk) {
-    const RowShape r = row_shape(true, heads / c.heads, dtype);
+//
+// Scratch has rows for the requests that are cut this way only: few tokens of
+// each, a few ten MB whatever the batch (a row for every token of it was 5 GB at
+// 8192 tokens, 32 heads of 128 and a table of 131072 tokens).  Longer requests
+// have CTAs enough of their own in bf16 (attend_prompt.cu); in f32 they are cut
+// into as many pieces as kTileScratch holds, which is all of them while their
+// rows are too few to fill the device.
+constexpr size_t kTileScratch = (size_t)128 << 20;
+
+AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv) {
+    const RowShape r = row_shape(true, heads / c.heads, dtype), more = row_shape(false, heads / c.heads, dtype);
     const int64_t rows = T <= R ? T : R;
     const int64_t ctas = (rows < 1 ? 1 : rows) * c.heads * r.hgroups;
-    const int64_t fill = 2 * (int64_t)device_sm_count();
+    const int64_t sms = device_sm_count(), fill = 2 * sms;
     const int64_t tiles = max_kv < 1 ? 1 : (max_kv + 63) / 64;
     int64_t s = 4 * ctas <= fill ? fill / ctas : (4 * fill + ctas - 1) / ctas;
     int64_t ch = (tiles + s - 1) / s;
@@ -724,12 +749,32 @@ void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dty
         s = kMaxSplits;
         ch = (tiles + s - 1) / s;
     }
-    chunk = (int)ch;
-    splits = (int)s;
-}
-
-size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits) {
-    return splits <= 1 ? 0 : (size_t)T * heads * splits * (v_dim + 2);
+    AttendCut cut{};
+    cut.splits = (int)s;
+    cut.chunk = (int)ch;
+    cut.several = T > R;
+    cut.tiles = cut.few = 1;
+    if (cut.several && dtype != 0) {
+        // Up to 32 tokens (a tile of the prompts' kernel at most) stay here, where their
+        // keys are cut into pieces, while the batch is small: 6 requests of up to 9
+        // tokens after 3756, 8 heads to a kv head, 34 us, by the prompts' kernel 102.  In
+        // larger ones only a tile does: the search for such requests costs single tokens
+        // 5 us (64 of them), and 63 requests of up to 231 tokens take 43 us instead of 35
+        // with up to 64 tokens here.
+        cut.tiles = more.tq >= 32 ? 1 : more.tq > 8 ? 32 / more.tq : 4;
+        if (R * cut.tiles * c.heads * more.hgroups * s > 16 * sms) cut.tiles = 1;
+        cut.few = cut.tiles * more.tq;
+    }
+    cut.by_token = T <= R * cut.few;
+    cut.rows = cut.by_token ? T : R * cut.few;
+    const size_t row = (size_t)heads * (c.v_dim + 2);                 // floats of a piece of a row
+    cut.tile_splits = 1;
+    if (cut.several && dtype == 0 && s > 1) {
+        const int64_t room = (int64_t)(kTileScratch / (sizeof(float) * row * T));
+        cut.tile_splits = (int)(room < 1 ? 1 : room < s ? room : s);
+    }
+    cut.floats = s > 1 ? row * (cut.rows * s + (cut.tile_splits > 1 ? T * cut.tile_splits : 0)) : 0;
+    return cut;
 }
 
 cudaError_t launch_attend(const AttendParams &params, cudaStream_t s) {
@@ -737,6 +782,7 @@ cudaError_t launch_attend(const AttendParams &params, cudaStream_t s) {
     AttendParams p = params;
     const uint64_t d = (uint64_t)p.c.block / 16;
     p.per_block = ((1ull << 36) + d - 1) / d;
+    p.splits = p.cut.splits;
     const bool bf = p.dtype != 0;
     if (p.c.k_dim == 64 && p.c.v_dim == 64) return bf ? launch_dims<64, 64, true>(p, s) : launch_dims<64, 64, false>(p, s);
     if (p.c.k_dim == 128 && p.c.v_dim == 128)

@@ -401,6 +401,16 @@ struct KvAppendParams {
     bool vec_k, vec_v;      // four elements may be loaded at once
     const int32_t *slots;   // [T]
 };
+// How the keys of a batch are cut into pieces that are joined through scratch.
+struct AttendCut {
+    int splits, chunk;      // pieces of the requests of up to `few` tokens, 64 chunk tokens each at least
+    int few, tiles;         // tiles: of the streaming kernel that hold `few` tokens
+    bool several;           // a request may have more than one token
+    int64_t rows;           // of scratch: tokens of the batch, or `few` for each request
+    bool by_token;
+    int tile_splits;        // pieces of the other requests (f32), their scratch behind the first
+    size_t floats;          // of scratch in all
+};
 struct AttendParams {
     KvCacheDev c;
     const void *q;          // [T, heads, k_dim], tokens ldq apart
@@ -414,18 +424,16 @@ struct AttendParams {
     float scale;
     void *out;              // [T, heads, v_dim], tokens ldo apart
     int64_t ldo;
-    int splits, chunk;      // pieces of the keys (64 chunk tokens each); > 1 joins through ws
+    AttendCut cut;
+    int splits;             // cut.splits, or cut.tile_splits where launch_attend says so; > 1 joins through ws
     int *err;               // device error word
-    float *ws;              // attend_workspace_floats floats
-    uint64_t per_block;     // set by launch_attend
+    float *ws;              // cut.floats floats
+    uint64_t per_block;     // and splits: set by launch_attend
 };
 cudaError_t launch_kv_plan(const KvPlanParams &p, cudaStream_t s);
 cudaError_t launch_kv_append(const KvAppendParams &p, cudaStream_t s);
-// Pieces that the keys of a request are cut into, for a batch whose longest
-// request holds max_kv tokens.
-void attend_pieces(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv, int &splits,
-                   int &chunk);
-size_t attend_workspace_floats(int64_t T, int heads, int v_dim, int splits);
+// For a batch whose longest request holds max_kv tokens.
+AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv);
 cudaError_t launch_attend(const AttendParams &p, cudaStream_t s);
 // The requests of more than `few` tokens (bf16); launch_attend's.
 cudaError_t launch_attend_prompt(const AttendParams &p, int few, cudaStream_t s);

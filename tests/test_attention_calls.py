@@ -56,3 +56,37 @@ def test_quantize_hands_over_the_rows_of_a_view(monkeypatch, calls, view):
     monkeypatch.setattr(capi, "call", call)
     codes, scales = quantize_int8(x, Ctx())
     assert len(calls) == 1 and codes.shape == x.shape and scales.shape == x.shape[:1]
+
+
+def scratch_bytes(dtype, T, R, heads, kv_heads, dims, block, max_blocks, max_kv=0):
+    cache = capi.KvCacheC(4096, 4096, 4096, 4096, max_blocks, block, kv_heads, *dims)
+    n = ctypes.c_int64()
+    assert capi.lib().qmoe_kv_attend_workspace(ctypes.byref(cache), dtype, T, R, heads, max_blocks, max_kv,
+                                               ctypes.byref(n)) == capi.QMOE_OK
+    return n.value
+
+
+F32, BF16 = capi.QMOE_DTYPE_F32, capi.QMOE_DTYPE_BF16
+
+
+@pytest.mark.parametrize("heads,kv_heads,dims", [(32, 8, (128, 128)), (64, 8, (128, 128)), (128, 1, (64, 64)), (16, 16, (192, 128)),
+                                                 (8, 8, (64, 64)), (112, 16, (128, 128))])
+@pytest.mark.parametrize("R", [1, 2, 7, 64, 300, 4096])
+def test_attention_scratch_stays_small(heads, kv_heads, dims, R):
+    """Long prompts over a wide table: what is cut into pieces has scratch, not every
+    token of the batch.  Pieces are cut for at most 16 CTAs on each of 148 SMs, of up
+    to 32 columns (heads by tokens) with 130 floats each: 39.4 MB; in f32 128 MiB for
+    the requests of several tokens come on top."""
+    few, many = 16 * 148 * 32 * 130 * 4, 128 << 20
+    for T in (1, 2, R, R + 1, 3 * R, 700, 8192, 65536):
+        for tokens in (64, 4096, 131072, 1 << 20):
+            args = (T, R, heads, kv_heads, dims, 64, tokens // 64)
+            assert scratch_bytes(BF16, *args) <= few, args
+            assert scratch_bytes(F32, *args) <= few + many, args
+
+
+def test_attention_scratch_of_few_rows():
+    # nothing is cut: no scratch; two rows after 131072 tokens: pieces of both
+    assert scratch_bytes(BF16, 5, 1, 32, 8, (128, 128), 64, 1) == 0
+    n = scratch_bytes(BF16, 2, 2, 32, 8, (128, 128), 64, 2048)
+    assert n > 0 and n % (2 * 32 * 130 * 4) == 0

@@ -112,3 +112,44 @@ def test_rows_in_front_of_the_first_request_stay(dtype, lens, first):
     cache.attend(q.cuda(), *device_args(starts, kv, table), out=out)
     assert (out[:first] == 0.25).all() and (out[starts[-1]:] == 0.25).all()
     check_rows(out[live], want[live], flat[3], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G,lens", [
+    (4, [(9000, 1), (4000, 70), (3000, 5), (2500, 1), (700, 33)]),          # every kind, all of them in pieces
+    (1, [(20000, 2), (30, 30)]), (16, [(16500, 1)]), (2, [(5000, 12)] * 5 + [(40, 0)] * 90 + [(6000, 1)]),
+], ids=str)
+def test_many_pieces_of_every_kind(dtype, G, lens):
+    """Requests of one, few and many tokens of one batch, each with many pieces of scratch to itself."""
+    bs, H, dk, dv = 64, 1, 128, 128
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, lens, 41, pad=2)
+    q[starts[-1]:] = float("nan")
+    args = device_args(starts, kv, table)
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, ref.new_scale(dk), torch.full((q.shape[0], H * G, dv), 0.25, dtype=torch.float64))
+    for max_kv in (0, 200):                       # by the table's width; told far too little
+        out = torch.full((q.shape[0], H * G, dv), 0.25, dtype=q.dtype, device="cuda")
+        cache.attend(q.cuda(), *args, max_kv=max_kv, out=out)
+        assert (out[starts[-1]:] == 0.25).all()
+        check_rows(out[:starts[-1]], want[:starts[-1]], flat[3], dtype)
+
+
+def test_scratch_is_all_that_is_written():
+    """A workspace of just the bytes asked for, with a guard behind it."""
+    import ctypes
+    from qmoe_b200 import capi
+    for dtype in ("bf16", "f32"):
+        cache, flat, q, starts, kv, table = attend_case(dtype, 64, 2, 4, 128, 128, [(9000, 1), (4000, 70), (3000, 5), (10, 0), (2500, 1)], 42)
+        args = device_args(starts, kv, table)
+        want = cache.attend(q.cuda(), *args)
+        T, R, width, code = q.shape[0], len(kv), len(table[0]), capi.QMOE_DTYPE_BF16 if dtype == "bf16" else capi.QMOE_DTYPE_F32
+        n = ctypes.c_int64()
+        capi.call("qmoe_kv_attend_workspace", cache._p, code, T, R, 8, width, 0, ctypes.byref(n))
+        assert n.value > 0
+        ws = torch.full((n.value + 4096,), 171, dtype=torch.uint8, device="cuda")
+        qd, out = q.cuda(), torch.zeros_like(want)
+        cache.ctx.use_current_torch_stream()
+        a = [cache.ctx.handle, cache._p, qd.data_ptr(), code, T, 8 * 128, 8, *(x.data_ptr() for x in args[:2]), R,
+             args[2].data_ptr(), width, 0, 128 ** -0.5, out.data_ptr(), 8 * 128, ws.data_ptr()]
+        capi.call("qmoe_kv_attend", *a, n.value)
+        assert torch.equal(out, want) and (ws[n.value:] == 171).all()
+        assert capi.lib().qmoe_kv_attend(*a, n.value - 1) == capi.QMOE_ERR_INVALID
