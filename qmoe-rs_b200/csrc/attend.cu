@@ -67,11 +67,11 @@ QMOE_DEV int64_t find_request(const int32_t *start, int64_t R, int64_t slot, int
     return lo;
 }
 
-// What the slots of a launch are: tokens, where each request has one at most;
+// What the slots of a launch are: tokens, of requests with up to cut.few;
 // requests with one token; `tiles` tiles of tq tokens for each request, of those
 // with that many tokens at most; tiles of tq tokens of the requests with
-// more than one.
-enum class Slots { kTokens, kSingles, kFew, kTiles };
+// more than cut.few; tokens, of which every tq-th of such a request is one's.
+enum class Slots { kTokens, kSingles, kFew, kTiles, kEvery };
 
 struct Rows {                                    // of one CTA: rows of one request and kv head
     int64_t t0;                                  // token of row 0
@@ -84,11 +84,16 @@ struct Rows {                                    // of one CTA: rows of one requ
 
 QMOE_DEV bool find_rows(const AttendParams &p, int64_t slot, int tq, Slots kind, int tiles, Rows &w) {
     const bool by_request = kind == Slots::kSingles || kind == Slots::kFew;
-    const int64_t r = kind == Slots::kFew ? slot / tiles : by_request ? slot : find_request(p.q_start, p.R, slot, tq);
+    const int each = kind == Slots::kEvery ? 1 : tq;
+    const int64_t r = kind == Slots::kFew ? slot / tiles : by_request ? slot : find_request(p.q_start, p.R, slot, each);
     const int64_t s0 = p.q_start[r], n = p.q_start[r + 1] - s0;
-    if (kind == Slots::kSingles ? n != 1 : kind == Slots::kFew ? n < 2 || n > tiles * tq : kind == Slots::kTiles && n < 2) return false;
-    const int64_t i0 = kind == Slots::kFew ? slot % tiles * tq : by_request ? 0 : (slot - (tq == 1 ? s0 : s0 / tq + r)) * tq;
-    if (i0 < 0 || i0 >= n || s0 < 0) return false;
+    if (kind == Slots::kSingles  ? n != 1
+        : kind == Slots::kFew    ? n < 2 || n > tiles * tq
+        : kind == Slots::kTokens ? n > p.cut.few
+                                 : n <= p.cut.few)
+        return false;
+    const int64_t i0 = kind == Slots::kFew ? slot % tiles * tq : by_request ? 0 : (slot - (each == 1 ? s0 : s0 / tq + r)) * each;
+    if (i0 < 0 || i0 >= n || s0 < 0 || (kind == Slots::kEvery && i0 % tq)) return false;
     int64_t cnt = n - i0 < tq ? n - i0 : tq;
     w.t0 = s0 + i0;
     if (w.t0 + cnt > p.T) cnt = p.T - w.t0;      // rows that the buffer does not hold
@@ -693,30 +698,32 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     // for what came before this call; so the others read nothing too early.  They
     // wait for the launch before them at their end, so that what comes after the
     // last has all of them behind it.
-    const bool prompts = several && BF16;         // the requests of more than cut.few tokens
+    const bool prompts = p.cut.mixed && BF16;     // the requests of more than cut.few tokens
     AttendParams tile = p;                        // those in f32: pieces of their own
     tile.splits = p.cut.tile_splits;
     tile.ws = p.ws ? p.ws + p.cut.rows * p.heads * p.splits * (DV + 2) : nullptr;
     tile.cut.rows = p.T;
     tile.cut.by_token = true;
     if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, p.cut.few, s);
-    if (e == cudaSuccess && several) {
+    if (e == cudaSuccess && (several || (p.cut.mixed && !BF16))) {
         // often none: a bounded grid looks through the slots (eight CTAs an SM: 5
         // requests of 2 tokens at 256 heads 102 us, with two 113)
-        const int64_t n = BF16 ? p.R * p.cut.tiles : p.T / more.tq + p.R, cap = 8 * (int64_t)device_sm_count();
+        const int64_t n = BF16 ? p.R * p.cut.tiles : several ? p.T / more.tq + p.R : p.T, cap = 8 * (int64_t)device_sm_count();
         const AttendParams &q = BF16 ? p : tile;
         int64_t grid = (p.cut.tiles > 1 ? 2 * cap : cap) / ((int64_t)p.c.heads * more.hgroups * q.splits);
         grid = grid < 1 ? 1 : grid < n ? grid : n;
-        e = launch_nt<DK, DV, BF16, kMost>(q, more, BF16 ? Slots::kFew : Slots::kTiles, p.cut.tiles, n, grid, true, s);
+        e = launch_nt<DK, DV, BF16, kMost>(q, more, BF16 ? Slots::kFew : several ? Slots::kTiles : Slots::kEvery, p.cut.tiles, n,
+                                          grid, true, s);
     }
     if (e == cudaSuccess && p.splits > 1) {
         int64_t grid = p.T;
-        if (prompts) {                            // a request's tokens side by side while the device has room
+        const bool by_request = several && BF16;
+        if (by_request) {                         // a request's tokens side by side while the device has room
             const int64_t room = 8 * (int64_t)device_sm_count() / (p.R * p.heads);
             grid = p.R * (room < 1 ? 1 : room < p.cut.few ? room : p.cut.few);
         }
         e = launch_pdl(attend_join_kernel<DV, BF16>, dim3((unsigned)grid, (unsigned)p.heads), dim3(kJoinWarps * 32), 0, s, p,
-                       tile, prompts ? Joins::kRequests : several ? Joins::kBoth : Joins::kTokens);
+                       tile, by_request ? Joins::kRequests : p.cut.mixed ? Joins::kBoth : Joins::kTokens);
     }
     return e;
 }
@@ -734,6 +741,15 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
 // into as many pieces as kTileScratch holds, which is all of them while their
 // rows are too few to fill the device.
 constexpr size_t kTileScratch = (size_t)128 << 20;
+
+// A batch without more tokens than requests is taken for single tokens, but one
+// of a captured step's many places may hold a prompt.  Requests of up to this many
+// tokens go a token at a time there: their keys come from L2 after the first, and
+// they are cut into pieces (33 tokens after 30000, 32 heads to 8: 242 us, by tiles
+// 552).  Longer ones go by tiles (256 after 1000 38 us, a token at a time 90, and
+// ever more the longer); the launch that looks for them costs a batch of 200
+// single tokens 2 us of 44, smaller batches nothing.
+constexpr int kPerToken = 128;
 
 AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int dtype, int64_t max_kv) {
     const RowShape r = row_shape(true, heads / c.heads, dtype), more = row_shape(false, heads / c.heads, dtype);
@@ -753,7 +769,9 @@ AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int d
     cut.splits = (int)s;
     cut.chunk = (int)ch;
     cut.several = T > R;
-    cut.tiles = cut.few = 1;
+    cut.mixed = cut.several || T > kPerToken;
+    cut.tiles = 1;
+    cut.few = cut.several ? 1 : cut.mixed ? kPerToken : INT32_MAX;
     if (cut.several && dtype != 0) {
         // Up to 32 tokens (a tile of the prompts' kernel at most) stay here, where their
         // keys are cut into pieces, while the batch is small: 6 requests of up to 9
@@ -769,7 +787,7 @@ AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int d
     cut.rows = cut.by_token ? T : R * cut.few;
     const size_t row = (size_t)heads * (c.v_dim + 2);                 // floats of a piece of a row
     cut.tile_splits = 1;
-    if (cut.several && dtype == 0 && s > 1) {
+    if (cut.mixed && dtype == 0 && s > 1) {
         const int64_t room = (int64_t)(kTileScratch / (sizeof(float) * row * T));
         cut.tile_splits = (int)(room < 1 ? 1 : room < s ? room : s);
     }

@@ -405,7 +405,8 @@ struct KvAppendParams {
 struct AttendCut {
     int splits, chunk;      // pieces of the requests of up to `few` tokens, 64 chunk tokens each at least
     int few, tiles;         // tiles: of the streaming kernel that hold `few` tokens
-    bool several;           // a request may have more than one token
+    bool several;           // more tokens than requests
+    bool mixed;             // or at least a request may have more than `few`
     int64_t rows;           // of scratch: tokens of the batch, or `few` for each request
     bool by_token;
     int tile_splits;        // pieces of the other requests (f32), their scratch behind the first

@@ -153,3 +153,40 @@ def test_scratch_is_all_that_is_written():
         capi.call("qmoe_kv_attend", *a, n.value)
         assert torch.equal(out, want) and (ws[n.value:] == 171).all()
         assert capi.lib().qmoe_kv_attend(*a, n.value - 1) == capi.QMOE_ERR_INVALID
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G,lens", [(4, [(300, 150)]), (1, [(700, 133), (90, 32), (80, 1), (140, 140)]), (16, [(1, 1)] * 30 + [(2100, 170)])], ids=str)
+def test_prompts_among_more_places_than_tokens(dtype, G, lens):
+    """A captured step's batch: more requests than rows, nearly all of them empty.
+    Prompts of more than 128 tokens among them go by tiles like any other: the same
+    bits as without the empty places (bf16; in f32 the places change how the keys
+    are cut)."""
+    bs, H, dk, dv = 16, 2, 128, 128
+    tokens = sum(n for _, n in lens)
+    places = [lens[0]] + [(50, 0)] * (tokens + 3 - len(lens)) + lens[1:]
+    cache, flat, q, starts, kv, table = attend_case(dtype, bs, H, G, dk, dv, places, 51, pad=2)
+    q[tokens:] = float("nan")
+    assert q.shape[0] <= len(kv)
+    out = torch.full((q.shape[0], H * G, dv), 0.25, dtype=q.dtype, device="cuda")
+    cache.attend(q.cuda(), *device_args(starts, kv, table), out=out)
+    want = ref.attend_dense(q, *flat, starts, kv, table, bs, ref.new_scale(dk), torch.zeros(q.shape[0], H * G, dv, dtype=torch.float64))
+    check_rows(out[:tokens], want[:tokens], flat[3], dtype)
+    assert (out[tokens:] == 0.25).all()
+    if dtype == "bf16":
+        full = [i for i, (_, n) in enumerate(places) if n]
+        few = cache.attend(q.cuda(), *device_args([starts[i] for i in full] + [tokens], [kv[i] for i in full], [table[i] for i in full]))
+        for i, (_, n) in enumerate(places):
+            if n > 128:
+                assert torch.equal(out[starts[i]:starts[i + 1]], few[starts[i]:starts[i + 1]])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_request_longer_than_the_buffer(dtype):
+    """Rows that the buffer does not hold are left out, however few it holds."""
+    for T, n in ((20, 40), (50, 90), (20, 20), (150, 190)):
+        cache, flat, q, starts, kv, table = attend_case(dtype, 16, 2, 2, 64, 64, [(200, n)] + [(0, 0)] * 159, 52)
+        want = ref.attend_dense(q, *flat, starts, kv, table, 16, ref.new_scale(64), torch.zeros(q.shape[0], 4, 64, dtype=torch.float64))
+        for places in (160, 1):
+            got = cache.attend(q[:T].cuda(), *device_args(starts[:places + 1], kv[:places], table[:places]))
+            check_rows(got, want[:T], flat[3], dtype)
