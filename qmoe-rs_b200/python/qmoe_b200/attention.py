@@ -41,9 +41,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _use_stream(ctx: Context) -> None:
-    stream = _raw_stream(ctx.device)
-    if stream != ctx._stream:
-        ctx.use_stream(stream)
+    capi.check(_fn("qmoe_ctx_set_stream")(ctx.handle, _raw_stream(ctx.device)))
 
 
 def _on(ctx: Context, name: str, t) -> None:

@@ -86,17 +86,15 @@ class Context:
         capi.call("qmoe_ctx_create", int(device), ctypes.c_void_p(stream or 0), ctypes.byref(h))
         self.handle = h
         self.device = int(device)
-        self._stream = stream or 0                # as the library has it
 
     def use_stream(self, stream: Optional[int]) -> None:
+        # always set: a note of the last one would be wrong after a set from another
+        # thread or through the C call
         capi.call("qmoe_ctx_set_stream", self.handle, ctypes.c_void_p(stream or 0))
-        self._stream = stream or 0
 
     def use_current_torch_stream(self) -> None:
         if torch is not None and torch.cuda.is_available():
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-            if stream != self._stream:
-                self.use_stream(stream)
+            self.use_stream(torch.cuda.current_stream(self.device).cuda_stream)
 
     def synchronize(self) -> None:
         capi.call("qmoe_ctx_synchronize", self.handle)

@@ -90,3 +90,72 @@ def test_attention_scratch_of_few_rows():
     assert scratch_bytes(BF16, 5, 1, 32, 8, (128, 128), 64, 1) == 0
     n = scratch_bytes(BF16, 2, 2, 32, 8, (128, 128), 64, 2048)
     assert n > 0 and n % (2 * 32 * 130 * 4) == 0
+
+
+class Library:
+    """The one entry point of a library whose stream others may set as well."""
+
+    def __init__(self):
+        self.stream = None
+
+    def qmoe_ctx_set_stream(self, handle, stream):
+        self.stream = getattr(stream, "value", stream) or 0
+        return capi.QMOE_OK
+
+
+def context(monkeypatch):
+    from qmoe_b200 import Context, layer
+    lib = Library()
+    monkeypatch.setattr(capi, "lib", lambda: lib)
+    monkeypatch.setattr(attention, "_fns", {})
+    ctx = Context.__new__(Context)
+    ctx.handle, ctx.device = None, 0
+    return lib, ctx, layer
+
+
+def test_every_call_sets_its_own_stream(monkeypatch):
+    """Whatever another thread or a C call left there, a call runs on the current stream."""
+    lib, ctx, layer = context(monkeypatch)
+
+    class Current:
+        cuda_stream = 70
+
+    monkeypatch.setattr(attention, "_raw_stream", lambda device: 70)
+    monkeypatch.setattr(layer.torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(layer.torch.cuda, "current_stream", lambda device: Current)
+    for use in (lambda: attention._use_stream(ctx), ctx.use_current_torch_stream, lambda: ctx.use_stream(70)):
+        for other in (0, 90):
+            use()
+            assert lib.stream == 70
+            capi.lib().qmoe_ctx_set_stream(None, other)
+        use()
+        assert lib.stream == 70
+
+
+def test_two_threads_whose_sets_cross(monkeypatch):
+    """One thread sets, another sets before the first is done: from the next call on
+    each is on its own stream again."""
+    import threading
+    lib, ctx, _ = context(monkeypatch)
+    crossed = []
+
+    class Crossing(Library):
+        def qmoe_ctx_set_stream(self, handle, stream):
+            Library.qmoe_ctx_set_stream(self, handle, stream)
+            if not crossed:
+                crossed.append(True)
+                t = threading.Thread(target=lambda: ctx.use_stream(2))
+                t.start()
+                t.join()
+            return capi.QMOE_OK
+
+    lib = Crossing()
+    monkeypatch.setattr(capi, "lib", lambda: lib)
+    monkeypatch.setattr(attention, "_fns", {})
+    current = [1]
+    monkeypatch.setattr(attention, "_raw_stream", lambda device: current[0])
+    attention._use_stream(ctx)
+    for s in (1, 2, 1, 1, 2, 2):
+        current[0] = s
+        attention._use_stream(ctx)
+        assert lib.stream == s
