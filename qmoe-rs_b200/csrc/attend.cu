@@ -216,7 +216,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     // ---- q: rows brought to fp16 by a power of two, as B fragments: lane 4 g + c
     // has dims 64 J + 16 c + 4 t + {0, 1 | 2, 3} of row 8 x + g for step 4 J + t
     uint32_t qf[kTerms][NT][DK / 16][2];
-    float back[NT][2], bias[NT][2];               // of this lane's columns 2 c, 2 c + 1
+    float back[NT][2];                            // of this lane's columns 2 c, 2 c + 1
     int last[NT][2];                              // their last keys
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -238,25 +238,20 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const int e = q_exponent(m);
         const float up = pow2i(14 - e);
-        float sum = 0.0f;
 #pragma unroll
         for (int J = 0; J < DK / 64; ++J)
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const float a = __fmul_rn(v[J][2 * t], up), b = __fmul_rn(v[J][2 * t + 1], up);
                 const uint32_t hi = h2(a, b);
-                sum += h_lo(hi) + h_hi(hi);
                 qf[0][x][4 * J + t / 2][t & 1] = hi;
                 if (kTerms == 2)
                     qf[kTerms - 1][x][4 * J + t / 2][t & 1] = h2(__fsub_rn(a, h_lo(hi)), __fsub_rn(b, h_hi(hi)));
             }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const float down = pow2i(e - 14);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {             // row g's lanes 4 g .. have it: fetch those of the columns
             back[x][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + i));
-            bias[x][i] = -1152.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * c + i));
             last[x][i] = w.pos0 + (8 * x + 2 * c + i) / gq;
         }
     }
@@ -283,10 +278,11 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         const int tg = (t_lo + warp + k * kWarps) * 64 + 16 * grp + (g & 1);   // token of row g, tile u: tg + 4 u
         const float kr1 = blk1 >= 0 ? p.c.k_range[blk1] : 0.0f, vr1 = blk1 >= 0 ? p.c.v_range[blk1] : 127.0f;
         const int64_t blk3 = block_of(k + 3);
-        // ---- scores.  One term: the codes as 1152 + c, the sum of q taken off at
-        // the start (its rounding, 2^-24 of 1152 sum q, is small beside bf16's);
-        // two terms: the codes themselves, the small term first and each 64 dims
-        // in sums of their own, added in f32.
+        // ---- scores, on the codes themselves.  (Left as 1152 + c, less 1152 sum q at
+        // the end, they cost two instructions less for four: 64 ragged requests 96 us
+        // instead of 100.  But the f32 sums then round at 1152 sum q, which for rows of
+        // q with a mean is far above the score: up to 1 % in P.)  Two terms: the small
+        // one first, and each 64 dims in sums of their own, added in f32.
         if (!(ok = sm100::mbar_wait_warp(&S.full[warp][(done + n) % kSlots], ((done + n) / kSlots) & 1, &S.abort, p.err))) break;
         const uint8_t *slot = S.ring[warp][(done + n) % kSlots] + (16 * grp + (g & 1)) * 64 + c * 16;
         float s[4][NT][4];
@@ -295,7 +291,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
 #pragma unroll
             for (int x = 0; x < NT; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[u][x][i] = kTerms == 1 ? bias[x][i & 1] : 0.0f;
+                for (int i = 0; i < 4; ++i) s[u][x][i] = 0.0f;
 #pragma unroll
         for (int J = 0; J < DK / 64; ++J) {
             uint4 kc[8];
@@ -307,8 +303,8 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         uint4 a;
-                        codes_biased(word_of(kc[2 * u], t), a.x, a.z);
-                        codes_biased(word_of(kc[2 * u + 1], t), a.y, a.w);
+                        codes_to_half(word_of(kc[2 * u], t), a.x, a.z);
+                        codes_to_half(word_of(kc[2 * u + 1], t), a.y, a.w);
 #pragma unroll
                         for (int x = 0; x < NT; ++x) mma_f16(s[u][x], a, qf[0][x][4 * J + t][0], qf[0][x][4 * J + t][1]);
                     }

@@ -27,17 +27,10 @@ QMOE_DEV uint32_t h2(float lo, float hi) {
 QMOE_DEV float h_lo(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xffff))); }
 QMOE_DEV float h_hi(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 
-// Four codes as 1152 + c in fp16 (0x6400 | (c + 128)), in order.
-QMOE_DEV void codes_biased(uint32_t v, uint32_t &lo, uint32_t &hi) {
-    v ^= 0x80808080u;
-    lo = __byte_perm(v, 0x64646464u, 0x4140);
-    hi = __byte_perm(v, 0x64646464u, 0x4342);
-}
-
-// Four codes as fp16, exactly.
+// Four codes as fp16, exactly: as 1152 + c (0x6400 | (c + 128)) first.
 QMOE_DEV void codes_to_half(uint32_t v, uint32_t &lo, uint32_t &hi) {
-    uint32_t a, b;
-    codes_biased(v, a, b);
+    v ^= 0x80808080u;
+    const uint32_t a = __byte_perm(v, 0x64646464u, 0x4140), b = __byte_perm(v, 0x64646464u, 0x4342);
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
 }

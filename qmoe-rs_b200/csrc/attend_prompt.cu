@@ -11,9 +11,7 @@
 //                    memory, then per key tile the scores from tensor memory,
 //                    the running maximum and sum, P back to tensor memory
 //   warps 8-14       codes from the cache to fp16 operands in shared memory (K
-//                    [token][dim] as 1152 + c, whose 1152 sum q goes into the
-//                    row's constant; V [dim][token]; 128-byte swizzle) and the
-//                    scales; the eight 16-token groups of K and V of a tile go
+//                    [token][dim], V [dim][token]; 128-byte swizzle) and the scales; the eight 16-token groups of K and V of a tile go
 //                    round the seven warps
 //   warp 15          tcgen05: S = q K^T (both operands in shared memory), then
 //                    O += P V (P from tensor memory)
@@ -102,23 +100,15 @@ QMOE_DEV float max3(float a, float b, float c) {
 
 QMOE_DEV uint4 ldg_code(const int8_t *at) { return __ldg(reinterpret_cast<const uint4 *>(at)); }
 
-// Sixteen codes c as fp16, or (BIASED) 1152 + c, to units `unit` and unit + 1 (16 bytes each) of row r of
+// Sixteen codes as fp16 to units `unit` and unit + 1 (16 bytes each) of row r of
 // a 128-byte swizzled operand.  A quarter warp's units are distinct banks: two
 // rows of four even units (K), or eight rows of one (V).
-template <bool BIASED>
 QMOE_DEV void store_codes(uint8_t *row, int unit, int r, const uint4 &v) {
     uint4 a, b;
-    if (BIASED) {
-        codes_biased(v.x, a.x, a.y);
-        codes_biased(v.y, a.z, a.w);
-        codes_biased(v.z, b.x, b.y);
-        codes_biased(v.w, b.z, b.w);
-    } else {
-        codes_to_half(v.x, a.x, a.y);
-        codes_to_half(v.y, a.z, a.w);
-        codes_to_half(v.z, b.x, b.y);
-        codes_to_half(v.w, b.z, b.w);
-    }
+    codes_to_half(v.x, a.x, a.y);
+    codes_to_half(v.y, a.z, a.w);
+    codes_to_half(v.z, b.x, b.y);
+    codes_to_half(v.w, b.z, b.w);
     *reinterpret_cast<uint4 *>(row + ((unit ^ (r & 7)) << 4)) = a;
     *reinterpret_cast<uint4 *>(row + (((unit + 1) ^ (r & 7)) << 4)) = b;
 }
@@ -274,7 +264,7 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
             }
             // q: rows by a power of two (and the scale's sign), as fp16, 64 dims a
             // 128-byte row; some of the warp's rows at a time, four dims a lane
-            float back = 0.0f, bias = 0.0f;                                  // bias: -1152 times the row's sum
+            float back = 0.0f;
             constexpr int kRep = (DK + 127) / 128, kAtOnce = 8 / kRep;
 #pragma unroll 1
             for (int x = 0; x < 32; x += kAtOnce) {
@@ -300,23 +290,16 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
                                      bf_hi(raw[y][z].y));
                     const int e = q_exponent(warp_max(mx)), at = q * 32 + x + y;
                     const float up = sign * pow2i(14 - e);
-                    float sum = 0.0f;
 #pragma unroll
                     for (int z = 0; z < kRep; ++z) {
                         const int d = 4 * lane + 128 * z;
                         const uint2 f = make_uint2(h2(bf_lo(raw[y][z].x) * up, bf_hi(raw[y][z].x) * up),
                                                    h2(bf_lo(raw[y][z].y) * up, bf_hi(raw[y][z].y) * up));
-                        sum += (h_lo(f.x) + h_hi(f.x)) + (h_lo(f.y) + h_hi(f.y));
                         if (d < DK)
                             *reinterpret_cast<uint2 *>(S.q[m] + (d >> 6) * (128 * 128) + at * 128 +
                                                        ((((d >> 3) & 7) ^ (at & 7)) << 4) + 2 * (d & 4)) = f;
                     }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (lane == x + y) {
-                        back = pow2i(e - 14);
-                        bias = -1152.0f * sum;
-                    }
+                    if (lane == x + y) back = pow2i(e - 14);
                 }
             }
             fence_proxy_async_smem();
@@ -351,11 +334,11 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         // the group's factors: a > 0, so that a masked score of -inf stays one (a
-                        // poisoned group's NaN is in lv); b takes the 1152 off the codes.  A row that
-                        // sees none of the group takes neither its lv nor its iv, which may be NaN.
+                        // poisoned group's NaN is in lv).  A row that sees none of the group takes
+                        // neither its lv nor its iv, which may be NaN.
                         const bool seen = 16 * x <= see;
                         const float a = fmaxf(S.f[u % kScaleRing][x] * back, 1.17549435e-38f);
-                        const float b = __fmaf_rn(bias, a, seen ? S.lv[u % kScaleRing][x] : neg_inf()) - base;
+                        const float b = (seen ? S.lv[u % kScaleRing][x] : neg_inf()) - base;
                         const uint64_t aa = pair(a, a), bb = pair(b, b);
                         uint64_t acc = pair(0.0f, 0.0f);
                         m4[x] = neg_inf();
@@ -489,11 +472,11 @@ attend_prompt_kernel(const AttendParams p, const int tq, const int span, const i
                 if (is_v) {
 #pragma unroll
                     for (int y = 0; y < kVLoads; ++y)
-                        store_codes<false>(S.v[st] + (32 * y + lane) * 128, 2 * grp, lane, codes[y]);
+                        store_codes(S.v[st] + (32 * y + lane) * 128, 2 * grp, lane, codes[y]);
                 } else {
 #pragma unroll
                     for (int y = 0; y < kKLoads; ++y)
-                        store_codes<true>(S.k[st] + (y >> 1) * (KT * 128) + (grp * 16 + (y & 1) * 8 + g) * 128, 2 * c, g, codes[y]);
+                        store_codes(S.k[st] + (y >> 1) * (KT * 128) + (grp * 16 + (y & 1) * 8 + g) * 128, 2 * c, g, codes[y]);
                     if (lane == 0) {
                         const float v1 = vr < kRangeFloor ? kRangeFloor : vr;
                         S.f[u % kScaleRing][grp] = __fdiv_rn(kr, 127.0f);

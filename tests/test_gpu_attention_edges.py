@@ -190,3 +190,31 @@ def test_a_request_longer_than_the_buffer(dtype):
         for places in (160, 1):
             got = cache.attend(q[:T].cuda(), *device_args(starts[:places + 1], kv[:places], table[:places]))
             check_rows(got, want[:T], flat[3], dtype)
+
+
+@pytest.mark.parametrize("mean", [0.0, 8.0, 32.0])
+@pytest.mark.parametrize("G,new", [(1, 1), (4, 1), (12, 1), (20, 1), (4, 5), (4, 200)])
+@pytest.mark.parametrize("dk", [64, 128, 192])
+def test_scores_of_rows_with_a_mean(mean, G, new, dk):
+    """q with a common offset and one outlying key in each block, whose range the small
+    codes of the others share: bf16 scores are as exact as f32 sums of q . k."""
+    from qmoe_b200 import KVCache
+    g = torch.Generator().manual_seed(61)
+    bs, kv, dv = 16, 640, 128 if dk > 64 else 64
+    nb = kv // bs
+    k = torch.randint(-1, 2, (nb, 1, dk // 64, bs, 64), generator=g, dtype=torch.int8)
+    k[:, :, :, 7] = -127
+    v = torch.randint(-127, 128, (nb, 1, 1, dv, 16), generator=g, dtype=torch.int8)
+    kr, vr = torch.full((nb, 1), 20.0), torch.full((nb, 1), 2.0)
+    q = (torch.randn(new, G, dk, generator=g) + mean).bfloat16()
+    others = (ref.k_flat(k).double() * (20 / 127))[:, 0, [i for i in range(bs) if i != 7]].reshape(-1, dk)
+    scale = 8.0 / 1.4427 / (q.double().reshape(-1, dk) @ others.T).std().item()   # exponents of 8 or so
+    cache = KVCache.from_tensors(k.cuda(), v.cuda(), kr.cuda(), vr.cuda())
+    table = list(range(nb))
+    got = cache.attend(q.cuda(), i32([0, new]), i32([kv]), i32(table, 1, nb), scale=scale)
+    want = ref.attend_dense(q, ref.k_flat(k), kr, ref.v_flat(v), vr, [0, new], [kv], [table], bs, scale,
+                            torch.zeros(new, G, dv, dtype=torch.float64))
+    # at most 16 additions, each off by a step of a partial sum, which no sum of
+    # magnitudes over the dims passes; nor the base of the exponential, the largest score
+    largest = (q.double().abs().reshape(-1, dk) @ others.abs().T).max().item() * scale * 1.4427
+    check_rows(got, want, vr, "bf16", slack=16 * 2.0 ** -23 * largest)
