@@ -216,7 +216,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
     // ---- q: rows brought to fp16 by a power of two, as B fragments: lane 4 g + c
     // has dims 64 J + 16 c + 4 t + {0, 1 | 2, 3} of row 8 x + g for step 4 J + t
     uint32_t qf[kTerms][NT][DK / 16][2];
-    float back[NT][2];                            // of this lane's columns 2 c, 2 c + 1
+    float back[NT][2];                            // scores to exponents, of this lane's columns 2 c, 2 c + 1
     int last[NT][2];                              // their last keys
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -251,7 +251,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         const float down = pow2i(e - 14);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {             // row g's lanes 4 g .. have it: fetch those of the columns
-            back[x][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + i));
+            back[x][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + i)) * (p.scale * kLog2e);
             last[x][i] = w.pos0 + (8 * x + 2 * c + i) / gq;
         }
     }
@@ -342,7 +342,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
         ++n;
         // ---- softmax
         vr = vr < kRangeFloor ? kRangeFloor : vr; // a block of zeros of another writer; NaN stays
-        const float ks = __fdiv_rn(kr, 127.0f) * (p.scale * kLog2e);
+        const float ks = __fdiv_rn(kr, 127.0f);
         const float lv = log2f(__fdiv_rn(vr, 127.0f)), iv = __fdiv_rn(127.0f, vr);
         // a tile that every row sees whole needs no mask
         const bool whole = __all_sync(0xffffffffu, blk >= 0 && tg + 15 < w.keys && tg + 15 <= w.pos0);

@@ -53,9 +53,10 @@ QMOE_DEV float4 load_q4(const AttendParams &p, int64_t at) {
 
 // A row of q whose largest magnitude is m goes to fp16 times 2^(14 - e): below
 // 2^15 and, but for elements 2^-28 below the largest, with all of bf16's bits.
+// No row is above f32's 2^128; those below 2^-100 are as good as 0.
 QMOE_DEV int q_exponent(float m) {
     const int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-    return e < -100 ? -100 : e > 100 ? 100 : e;
+    return e < -100 ? -100 : e;
 }
 
 }  // namespace qmoe

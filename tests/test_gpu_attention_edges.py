@@ -218,3 +218,17 @@ def test_scores_of_rows_with_a_mean(mean, G, new, dk):
     # magnitudes over the dims passes; nor the base of the exponential, the largest score
     largest = (q.double().abs().reshape(-1, dk) @ others.abs().T).max().item() * scale * 1.4427
     check_rows(got, want, vr, "bf16", slack=16 * 2.0 ** -23 * largest)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G,lens", [(2, [(300, 1)]), (2, [(3000, 1), (90, 7)]), (4, [(400, 150), (70, 1)])], ids=str)
+def test_rows_of_q_far_from_one(dtype, G, lens):
+    """2^n q with the scale 2^-n scale: the same bits, up to the type's largest values."""
+    cache, flat, q, starts, kv, table = attend_case(dtype, 16, 2, G, 128, 128, lens, 71)
+    args = device_args(starts, kv, table)
+    scale = ref.new_scale(128)
+    clean = cache.attend(q.cuda(), *args, scale=scale)
+    assert q.abs().max() < 8
+    for n in (-90, 60, 100, 110, 122):
+        got = cache.attend(q.cuda() * 2.0 ** n, *args, scale=scale * 2.0 ** -n)
+        assert torch.equal(got, clean), n
