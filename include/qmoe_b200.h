@@ -467,8 +467,8 @@ QMOE_API int qmoe_ep_finish(qmoe_ep_peer *p, const int32_t *slot_pos, int64_t T,
  * nearest whole number (ties to even) and stands for code * r / 127.  Where
  * an element is not finite, r is NaN and the codes are 0. */
 
-/* Rows of x [rows, cols] (f32 or bf16, row_stride elements apart) to codes
- * [rows, cols] and scales [rows] = r / 127. */
+/* Rows of x [rows, cols] (f32 or bf16, row_stride >= cols elements apart) to
+ * codes [rows, cols] and scales [rows] = r / 127; cols <= 2^30. */
 QMOE_API int qmoe_quantize_int8(qmoe_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols,
                                 int64_t row_stride, int8_t *codes, float *scales);
 

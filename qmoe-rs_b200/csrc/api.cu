@@ -2135,7 +2135,7 @@ int qmoe_quantize_int8(qmoe_ctx *ctx, const void *x, int dtype, int64_t rows, in
                        int8_t *codes, float *scales) {
     if (!ctx) return fail(QMOE_ERR_INVALID, "ctx is NULL");
     QTRY(check_dtype(dtype));
-    if (rows < 0 || rows > INT32_MAX || cols <= 0 || cols > INT32_MAX || (rows > 1 && row_stride < cols))
+    if (rows < 0 || rows > INT32_MAX || cols <= 0 || cols > (1 << 30) || (rows > 1 && row_stride < cols))
         return fail(QMOE_ERR_INVALID, "rows %lld, cols %lld, row_stride %lld", (long long)rows, (long long)cols,
                     (long long)row_stride);
     if (rows == 0) return QMOE_OK;

@@ -159,3 +159,10 @@ def test_two_threads_whose_sets_cross(monkeypatch):
         current[0] = s
         attention._use_stream(ctx)
         assert lib.stream == s
+
+
+def test_rows_too_long_for_the_quantiser_are_refused():
+    """Columns are counted in 32 bits, in steps of a thread block."""
+    ctx = ctypes.cast(ctypes.create_string_buffer(256), ctypes.c_void_p)
+    for cols in ((1 << 30) + 1, (1 << 31) - 256, (1 << 31) - 1, 1 << 31):
+        assert capi.lib().qmoe_quantize_int8(ctx, 64, F32, 1, cols, cols, 64, 64) == capi.QMOE_ERR_INVALID, cols
