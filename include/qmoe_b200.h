@@ -475,7 +475,7 @@ QMOE_API int qmoe_quantize_int8(qmoe_ctx *ctx, const void *x, int dtype, int64_t
 /* A weight matrix in 8 bits: codes [out_features, in_features] and one f32
  * scale per output channel, copied to memory the handle owns (rows padded to
  * 128 bytes).  in_features <= QMOE_INT8_MAX_IN_FEATURES, so that a sum of
- * products fits 32 bits. */
+ * products fits 32 bits; scales below 2^100 in magnitude. */
 #define QMOE_INT8_MAX_IN_FEATURES 131072
 typedef struct qmoe_int8 qmoe_int8;
 QMOE_API int qmoe_int8_create(qmoe_ctx *ctx, const int8_t *codes, const float *scales,

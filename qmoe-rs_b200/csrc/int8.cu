@@ -166,6 +166,11 @@ struct Smem {
     alignas(16) float sx[8][256];                             // each epilogue warp's copy of a tile's token scales
 };
 
+// The factors of a row and a channel, 2^-24 of the one and 2^24 of the other: a
+// sum (below 2^31) times a row's scale (below 2^121) is then in f32's range, the
+// result the same to the bit.
+QMOE_DEV float row_factor(float sx) { return sx * 5.9604644775390625e-08f; }
+QMOE_DEV float channel_factor(float sw) { return sw * 16777216.0f; }
 // Without a residual res is -0: adding it changes no value.
 QMOE_DEV float finish(int sum, float sx, float sw, float res) {
     return __fadd_rn(__fmul_rn(__fmul_rn((float)sum, sx), sw), res);
@@ -324,13 +329,13 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
             const int n = (tile / tiles_t) * 128 + q * 32 + lane, nn = n < p.N ? n : p.N - 1;
             const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
             const int64_t at = t0 * p.N + nn;
-            const float sw = __ldg(p.sw + nn);
+            const float sw = channel_factor(__ldg(p.sw + nn));
             float next[CH];                       // residual of the chunk to come
 #pragma unroll
             for (int j = 0; j < CH; ++j) next[j] = -0.0f;
             if (adds) load_rows<BF16>(p.residual, at, N, c0, count, next);
             __syncwarp();
-            for (int j = lane; j < count; j += 32) sx[j] = p.sx[t0 + j];
+            for (int j = lane; j < count; j += 32) sx[j] = row_factor(p.sx[t0 + j]);
             __syncwarp();
             if (!(ok = mbar_wait_warp(&S->dfull[i & 1], (i >> 1) & 1, abort, p.err))) break;
             tc_fence_after();
@@ -391,13 +396,13 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
         const int n = (tile0 / tiles_t) * 128 + (tid & 127);
         const int count = (int)(p.T - t0 < BN ? p.T - t0 : BN);
         const int *sums = reinterpret_cast<const int *>(ring);
-        const float sw = n < p.N ? __ldg(p.sw + n) : 0.0f;
+        const float sw = n < p.N ? channel_factor(__ldg(p.sw + n)) : 0.0f;
         for (int j = rank + parts * (tid >> 7); j < count; j += Cfg::threads / 128 * parts) {
             int sum = 0;
             for (int r = 0; r < parts; ++r) sum += load_cluster(sums + j * 128 + (tid & 127), r);
             if (n < p.N)
                 store1<BF16>(p.y, (t0 + j) * p.N + n,
-                             finish(sum, p.sx[t0 + j], sw,
+                             finish(sum, row_factor(p.sx[t0 + j]), sw,
                                     p.residual ? load1<BF16>(p.residual, (t0 + j) * p.N + n) : -0.0f));
         }
         cluster_barrier();                        // the others may still read this CTA's sums

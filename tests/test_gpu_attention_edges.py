@@ -232,3 +232,35 @@ def test_rows_of_q_far_from_one(dtype, G, lens):
     for n in (-90, 60, 100, 110, 122):
         got = cache.attend(q.cuda() * 2.0 ** n, *args, scale=scale * 2.0 ** -n)
         assert torch.equal(got, clean), n
+
+
+# ---- product ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("t,k,n", [(3, 200, 130), (40, 2048, 640), (700, 130, 4200), (1, 4096, 256), (300, 5000, 300)])
+def test_product_of_rows_far_from_one(dtype, t, k, n):
+    """2^a x with weights of 2^b: 2^(a + b) times the result, bit for bit, wherever that
+    is in range, some rows and not others; codes times a row's scale alone are not."""
+    from qmoe_b200 import Int8Tensor
+    g = torch.Generator().manual_seed(t + k)
+    dt = DT[dtype]
+    codes = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8).cuda()
+    scales = (torch.rand(n, generator=g) * 0.01 + 1e-4).cuda()
+    x = torch.randn(t, k, generator=g).to(dt).cuda()
+    res = torch.randn(t, n, generator=g).to(dt).cuda()
+    w = Int8Tensor.from_bytes(codes, (n, k), scales)
+    clean, added = w.forward(x), w.forward(x, residual=res)
+    assert x.abs().max() < 32
+    for a, b in ((122, -100), (122, -60), (-50, 100), (60, 40)):
+        far = Int8Tensor.from_bytes(codes, (n, k), scales * 2.0 ** b)
+        y = far.forward(x * 2.0 ** a).double() * 2.0 ** -(a + b)
+        assert torch.equal(y, clean.double()), (a, b)
+        y = far.forward(x * 2.0 ** a, residual=(res.double() * 2.0 ** (a + b)).to(dt)).double() * 2.0 ** -(a + b)
+        assert torch.equal(y, added.double()), (a, b)
+        mixed = x.clone()
+        mixed[::2] *= 2.0 ** a
+        y = far.forward(mixed).double() * 2.0 ** -b
+        y[::2] *= 2.0 ** -a
+        keep = torch.isfinite(clean.double() * 2.0 ** b)
+        assert torch.equal(y[::2], clean[::2].double())
+        assert torch.equal(y[1::2], clean[1::2].double()) and keep.all()
