@@ -510,7 +510,8 @@ QMOE_API int qmoe_int8_forward(qmoe_int8 *t, const void *x, int dtype, int64_t b
  *                             token; -1 for rows of denied requests, rows
  *                             behind the last request, and where a table
  *                             entry is not in 0 .. num_blocks - 1
- *   positions [capacity]      the token's place in its request, -1 likewise
+ *   positions [capacity]      the token's place in its request; -1 for rows of
+ *                             denied requests and behind the last request
  *   taken     [1]             blocks taken of free_blocks
  * The sum of new_lens must be below 2^31.  block_size: 16, 32, ... 256. */
 QMOE_API int qmoe_kv_plan(qmoe_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,

@@ -95,13 +95,14 @@ class Int8Tensor:
     """Device-resident 8-bit weight matrix with a scale per output channel,
     the 8-bit counterpart of PackedQMoETensor (qmoe-rs src/tensor.rs:16-121)."""
 
-    def __init__(self, handle, ctx: Context, shape, scales):
+    def __init__(self, handle, ctx: Context, scales):
         self._h = handle
         self.ctx = ctx
-        self.shape = tuple(int(v) for v in shape)
         self.scales = scales
-        n = _I64()
+        rows, cols, n = _I64(), _I64(), _I64()
+        capi.call("qmoe_int8_shape", handle, ctypes.byref(rows), ctypes.byref(cols))
         capi.call("qmoe_int8_workspace", handle, 1, ctypes.byref(n))
+        self.shape = (int(rows.value), int(cols.value))
         self._row_bytes = int(n.value)
 
     @classmethod
@@ -123,7 +124,7 @@ class Int8Tensor:
         _use_stream(ctx)
         h = ctypes.c_void_p()
         capi.call("qmoe_int8_create", ctx.handle, cp, sp, out_f, in_f, kind, ctypes.byref(h))
-        return cls(h, ctx, shape, scales)
+        return cls(h, ctx, scales)
 
     @classmethod
     def from_float(cls, weight, ctx: Optional[Context] = None) -> "Int8Tensor":
@@ -187,7 +188,7 @@ class PagePlan:
     block_table: torch.Tensor   # [requests, max_blocks] int32, updated in place
     q_start: torch.Tensor       # [requests + 1] first row of each request
     kv_lens: torch.Tensor       # [requests] tokens held after the step, 0 for a denied request
-    slots: torch.Tensor         # [rows] block * block_size + offset, -1 for none
+    slots: torch.Tensor         # [rows] block * block_size + offset; -1 for none, and where the table's entry is no block
     positions: torch.Tensor     # [rows] place in the request, -1 for none
     taken: torch.Tensor         # [1] blocks taken from the front of the free list
     max_kv: int = 0             # longest kv_lens if known on the host

@@ -264,3 +264,16 @@ def test_product_of_rows_far_from_one(dtype, t, k, n):
         keep = torch.isfinite(clean.double() * 2.0 ** b)
         assert torch.equal(y[::2], clean[::2].double())
         assert torch.equal(y[1::2], clean[1::2].double()) and keep.all()
+
+
+def test_shape_comes_from_the_handle():
+    from qmoe_b200 import Int8Tensor
+    w = Int8Tensor.from_bytes(torch.zeros(5 * 17, dtype=torch.int8).cuda(), (5, 17), torch.ones(5).cuda())
+    assert w.shape == (5, 17) and w.forward(torch.ones(2, 17).cuda()).shape == (2, 5)
+
+
+def test_plan_keeps_the_position_where_a_table_entry_is_no_block():
+    from qmoe_b200 import plan_pages
+    p = plan_pages(i32([20, 16]), i32([2, 1]), i32([3, -1, 9, 4, 99, 7], 2, 3), i32([5]), 16, 4, 8)
+    assert p.slots.tolist() == [-1, -1, 5 * 16, -1]           # rows of entry -1; of a new block; of nobody
+    assert p.positions.tolist() == [20, 21, 16, -1] and p.kv_lens.tolist() == [22, 17] and p.taken.tolist() == [1]
