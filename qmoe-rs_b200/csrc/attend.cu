@@ -514,7 +514,7 @@ QMOE_DEV void attend_rows(const AttendParams &p, const Rows &w, int h, int split
 __host__ __device__ constexpr int most_columns(bool bf16) { return bf16 ? 4 : 2; }
 
 // CTAs an SM holds: three where the registers of a single token's few columns
-// allow it, which evens out batches of ragged lengths (64 requests 99 -> 91 us).
+// allow it, which evens out batches of ragged lengths (64 requests 106 -> 100 us).
 __host__ __device__ constexpr int ctas_per_sm(int dk, bool bf16, int nt) { return bf16 && nt == 1 && dk <= 128 ? 3 : 2; }
 
 // Up to tq tokens of a request by gq heads of a kv head, on NT * 8 columns.
@@ -703,7 +703,7 @@ cudaError_t launch_dims(const AttendParams &p, cudaStream_t s) {
     if (e == cudaSuccess && prompts) e = launch_attend_prompt(p, p.cut.few, s);
     if (e == cudaSuccess && (several || (p.cut.mixed && !BF16))) {
         // often none: a bounded grid looks through the slots (eight CTAs an SM: 5
-        // requests of 2 tokens at 256 heads 102 us, with two 113)
+        // requests of 2 tokens after 4000, 256 heads to 16, 80 us, with two 82)
         const int64_t n = BF16 ? p.R * p.cut.tiles : several ? p.T / more.tq + p.R : p.T, cap = 8 * (int64_t)device_sm_count();
         const AttendParams &q = BF16 ? p : tile;
         int64_t grid = (p.cut.tiles > 1 ? 2 * cap : cap) / ((int64_t)p.c.heads * more.hgroups * q.splits);
@@ -771,10 +771,10 @@ AttendCut attend_cut(const KvCacheDev &c, int64_t T, int64_t R, int heads, int d
     if (cut.several && dtype != 0) {
         // Up to 32 tokens (a tile of the prompts' kernel at most) stay here, where their
         // keys are cut into pieces, while the batch is small: 6 requests of up to 9
-        // tokens after 3756, 8 heads to a kv head, 34 us, by the prompts' kernel 102.  In
-        // larger ones only a tile does: the search for such requests costs single tokens
-        // 5 us (64 of them), and 63 requests of up to 231 tokens take 43 us instead of 35
-        // with up to 64 tokens here.
+        // tokens after 3756, 8 heads to one kv head, 28 us, by the prompts' kernel 114.
+        // In larger ones only a tile does: with up to 32 tokens here 64 single tokens of
+        // up to 8192 keys, 32 heads to 8, take 105 us instead of 100 for the search, and
+        // 63 requests of up to 231 after 500 287 instead of 246.
         cut.tiles = more.tq >= 32 ? 1 : more.tq > 8 ? 32 / more.tq : 4;
         if (R * cut.tiles * c.heads * more.hgroups * s > 16 * sms) cut.tiles = 1;
         cut.few = cut.tiles * more.tq;

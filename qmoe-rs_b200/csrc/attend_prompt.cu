@@ -11,7 +11,8 @@
 //                    memory, then per key tile the scores from tensor memory,
 //                    the running maximum and sum, P back to tensor memory
 //   warps 8-14       codes from the cache to fp16 operands in shared memory (K
-//                    [token][dim], V [dim][token]; 128-byte swizzle) and the scales; the eight 16-token groups of K and V of a tile go
+//                    [token][dim], V [dim][token]; 128-byte swizzle) and the
+//                    scales; the eight 16-token groups of K and V of a tile go
 //                    round the seven warps
 //   warp 15          tcgen05: S = q K^T (both operands in shared memory), then
 //                    O += P V (P from tensor memory)
@@ -21,10 +22,12 @@
 // two query tiles' softmaxes run side by side.  O is scaled to a maximum that a
 // row's own may outgrow by 2^8: P is made with it before the tile's maximum is
 // known and made again, with O rescaled, only where that was too small (P then
-// reaches 2^(8 + 6), which fp16 holds).  For 256 rows by 128 keys of 128 dims the
-// exponentials take 2048 cycles of an SM (16 a cycle) and the MMAs as many.
+// reaches 2^(8 + 6), which fp16 holds; its rounding, 2^-11 of P or 2^-31 of that
+// maximum, is below that of the bf16 output; the sum takes P in f32).  For 256
+// rows by 128 keys of 128 dims the exponentials take 2048 cycles of an SM (16 a
+// cycle) and the MMAs as many.
 // Measured: three prompts of up to 2048 tokens after up to 6000, 32 query and 8 kv
-// heads of 128, 356 us = 700 TFLOP/s, the tensor pipe busy 37 % of the time: the
+// heads of 128, 355 us = 700 TFLOP/s, the tensor pipe busy 38 % of the time: the
 // chain score, softmax, P V of two query tiles and the barriers between its warps
 // bound it, then the tail of 256 long items on 148 SMs.
 #include "attend.cuh"

@@ -305,7 +305,7 @@ def test_f32_keeps_its_second_terms(lens, G, dk, dv):
     """Root mean square of the error over many keys.  Weights are off by 2^-22 (P) and
     their exponents by four (root of 16 additions) times 2^-24 of sums below 8, 2^-19;
     both average over some 80 keys or more of like weight, to 2^-22 of the largest |v|.
-    P in one fp16 term: 2^-11 at most, 2^-12.3 in the mean, 2^-16 averaged."""
+    P in one fp16 term: 2^-11 at most, 2^-12.3 in the mean, 2^-17 averaged."""
     cache, flat, q, starts, kv, table = attend_case("f32", 64, 2, G, dk, dv, lens, 91)
     got = cache.attend(q.cuda(), *device_args(starts, kv, table)).cpu().double()
     want = ref.attend_dense(q, *flat, starts, kv, table, 64, ref.new_scale(dk), torch.zeros(q.shape[0], 2 * G, dv, dtype=torch.float64))
